@@ -702,6 +702,66 @@ void thhip_rgb2float(void *dst, const unsigned char *src, int width, int height,
 void thhip_rgb2float_batch(void *dst, const unsigned char *src, int n, long src_pitch, int width, int height,
 	int stride, int cp, const float *mean, const float *std, int bgr, int dtype);
 
+/* ---- Linear layers with 4-bit weights, norms and 8-bit activations ----
+ *
+ * The reference's Linear knows fp32 weights (modules/Linear.c:72-113) and, in its LOWP engine, 8-bit codes
+ * with one range for the whole matrix (lowp_basic.c:5-38); its norm is over the batch
+ * (SpatialBatchNormalization.c:57-116).  These entry points serve networks of Linear layers, where a batch of
+ * a few rows is bound by the bytes of the weights.  Like thhip_linear_batched_noalloc they allocate nothing and
+ * use no scratch memory, and return 0, or -1 with a message on stderr and nothing launched for arguments they
+ * refuse; no rows (B = 0, rows = 0) is 0 and no launch.  `dtype` is THHIP_F32, THHIP_F16 or THHIP_BF16.  Sums,
+ * norms and scales of x are fp32.  Row strides (ld*) are in elements; any stride that holds a row and any
+ * pointer aligned to its element is taken, 16-byte vectors are used where both allow it.
+ *
+ * Weights with 4 bits: a code n of 0 .. 15 a weight, row-major [nOut][(nIn + 1) / 2] bytes, even k in the low
+ * half of a byte; `group` consecutive weights of a row (32, 64, 128 or 256; 0: the whole row) share a scale and a
+ * zero point: w = s * (n - z).  scales: [nOut][groups] in `dtype`, groups = ceil(nIn / group); zeros:
+ * [nOut][groups] bytes, or NULL: 8 everywhere.
+ *
+ * thhip_quantize_w4 makes them on the device from weights of type `wtype`, rows ldw apart: without zeros
+ * s = max|w| / 7 and n = rint(w / s) + 8; with zeros s = (max(w, 0) - min(w, 0)) / 15, z = rint(-min(w, 0) / s),
+ * n = rint(w / s) + z, at most 15.  s is rounded to `dtype` first.  Finite weights; a group whose scale has no
+ * reciprocal in fp32, or rounds to 0, becomes 0.
+ *
+ * thhip_w4_pack lays codes, scales and zeros out in the order the kernels read them, into one buffer of
+ * thhip_w4_packed_bytes(nOut, nIn, group, dtype, zeros != NULL) bytes (0 for a layer that is refused), aligned to
+ * 16 bytes; like thhip_conv_pack_weight's it is only valid for calls with the same sizes, group, dtype and zeros. */
+size_t thhip_w4_packed_bytes(int nOut, int nIn, int group, int dtype, int zeros);
+int thhip_w4_pack(const unsigned char *codes, const void *scales, const unsigned char *zeros, void *packed,
+	int nOut, int nIn, int group, int dtype);
+int thhip_quantize_w4(const void *w, long ldw, int wtype, unsigned char *codes, void *scales, unsigned char *zeros,
+	int nOut, int nIn, int group, int dtype);
+
+/* y[b][o] = act(bias[o] + sum_k w[o][k] * x[b][k]) for any batch: thhip_gemv, thhip_linear_batched and the 1x1
+ * convolution of nn_Linear_updateOutput (Linear.c:72-113) for packed 4-bit weights.  x [B][nIn] and y [B][nOut] in
+ * `dtype`, bias fp32 [nOut] or NULL; act != 0 applies the Threshold y > thr ? y : val.  Weights are never rounded:
+ * the products with the codes are summed in fp32 and a group's sum is multiplied with its scale.  An infinity
+ * or NaN in a row of x makes outputs of that row NaN (or infinite); other rows do not see it.  y may not overlap x. */
+int thhip_linear_w4(const void *x, long ldx, const void *wpacked, const float *bias, void *y, long ldy,
+	int B, int nIn, int nOut, int group, int zeros, int act, float thr, float val, int dtype);
+/* The same with 8-bit activations, x[b][k] = xscale[b][g] * q[b][k]: q signed codes, xscale fp32 [B] (xgroup 0) or
+ * [B][groups] (xgroup == group), as thhip_rmsnorm_i8 and thhip_quantize_rows write them.  Products of codes are
+ * summed in int32, exactly, up to 128 at a time.  y, the layer's scales and `dtype` as above. */
+int thhip_linear_w4_i8(const signed char *q, long ldq, const float *xscale, int xgroup, const void *wpacked,
+	const float *bias, void *y, long ldy, int B, int nIn, int nOut, int group, int zeros, int act, float thr, float val,
+	int dtype);
+
+/* Root-mean-square norm of rows with a residual: h = x + res in fp32 (res NULL: x), sum = h rounded to `dtype` (if
+ * not NULL), y = h * weight / sqrt(mean(h * h) + eps), weight fp32 [cols] or NULL (1).  sum may be x or res and y
+ * may be x or res, with the same stride, but not one the other's; nothing else may overlap. */
+int thhip_rmsnorm(const void *x, long ldx, const void *res, long ldr, const float *weight, float eps,
+	void *sum, long lds, void *y, long ldy, long rows, long cols, int dtype);
+/* The same with y as signed 8-bit codes: qscale = max|y| / 127 and q = rint(127 * y / max|y|) over groups of 32, 64,
+ * 128 or 256 columns or the whole row (group 0); qscale fp32 [rows][ceil(cols / group)].  Where max|y| is under
+ * 2^-116 scale and codes are 0; a NaN or infinity makes its group's scale NaN or infinite, and its codes mean nothing. */
+int thhip_rmsnorm_i8(const void *x, long ldx, const void *res, long ldr, const float *weight, float eps,
+	void *sum, long lds, signed char *q, long ldq, float *qscale, int group, long rows, long cols, int dtype);
+/* Codes and scales of x itself, and back: y = q * qscale rounded to `dtype`. */
+int thhip_quantize_rows(const void *x, long ldx, signed char *q, long ldq, float *qscale, int group,
+	long rows, long cols, int dtype);
+int thhip_dequantize_rows(const signed char *q, long ldq, const float *qscale, int group, void *y, long ldy,
+	long rows, long cols, int dtype);
+
 /* ---- uint8 (LOWP) path ---- */
 
 /* Replaces THLowpTensor_newFromFloatTensor's arithmetic

@@ -1,0 +1,203 @@
+"""4-bit Linear layers (thhip_linear_w4, thhip_linear_w4_i8, thhip_w4_pack, thhip_quantize_w4) against the plain product in
+64 bits."""
+import numpy as np
+import pytest
+
+import gpu_util as G
+import w4_util as U
+from thnets_amd import api
+from w4_util import BF16, F16, F32
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [F32, F16, BF16]
+
+# B, nIn, nOut: one of everything, one short of and one past the packed blocks (16 rows, 128 k) and the batch slices
+SHAPES = [(1, 1, 1), (1, 32, 16), (2, 33, 17), (1, 127, 5), (3, 128, 16), (5, 129, 31), (16, 512, 48), (17, 1000, 33), (15, 4090, 100),
+          (33, 640, 80), (64, 1280, 65), (65, 256, 40), (1, 9216, 64), (1, 4096, 1000), (130, 384, 200), (257, 1100, 300), (128, 512, 128),
+          (300, 2048, 256)]
+GROUPS = [32, 64, 128, 256, 0]
+
+
+def data(seed, B, nIn, nOut, dtype):
+    g = U.rng(seed)
+    return g, U.rounded(g.standard_normal((B, nIn), dtype=np.float32), dtype), (g.standard_normal(nOut) * 0.1).astype(np.float32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("i", range(len(SHAPES)))
+def test_shapes(hiplib, i, dtype):
+    B, nIn, nOut = SHAPES[i]
+    g, x, b = data(100 + i, B, nIn, nOut, dtype)
+    layer = U.Layer.random(g, nOut, nIn, GROUPS[i % 5], dtype, i % 2 == 0).lay(hiplib)
+    want, mag = U.linear64(layer, x, b)
+    U.check_linear(U.linear(hiplib, layer, x, b), want, mag, layer)
+
+
+@pytest.mark.parametrize("xgroup", [0, 1])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("i", range(len(SHAPES)))
+def test_shapes_i8(hiplib, i, dtype, xgroup):
+    B, nIn, nOut = SHAPES[i]
+    g, _, b = data(200 + i, B, nIn, nOut, dtype)
+    layer = U.Layer.random(g, nOut, nIn, GROUPS[(i + 1) % 5], dtype, i % 2 == 1).lay(hiplib)
+    q = g.integers(-128, 128, (B, nIn)).astype(np.int8)
+    xs = (g.uniform(0.5, 1.5, (B, U.groups_of(nIn, layer.group) if xgroup else 1)) / 64).astype(np.float32)
+    want, mag = U.linear64(layer, q * U.spread_x(xs.astype(np.float64), nIn, layer.group), b)
+    got = U.linear(hiplib, layer, q, b, xs=xs, xgroup=layer.group if xgroup else 0)
+    U.check_linear(got, want, mag, layer)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("zeros", [0, 1])
+@pytest.mark.parametrize("B", [1, 8, 20, 200])
+def test_groups(hiplib, dtype, group, zeros, B):
+    """Every group size with and without zero points; the last group is a part of one."""
+    g, x, b = data(300 + group + B, B, 712, 50, dtype)
+    layer = U.Layer.random(g, 50, 712, group, dtype, zeros).lay(hiplib)
+    want, mag = U.linear64(layer, x, b)
+    U.check_linear(U.linear(hiplib, layer, x, b), want, mag, layer)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("B", [1, 16, 17, 100, 260])
+def test_small_integers_are_exact(hiplib, dtype, group, B):
+    """Integers times powers of two whose sums stay below 2^24 units (scales are at least 2^-4; a row's own scale moves
+    all of its sums alike): no rounding but the last, so the very bits."""
+    g = U.rng(400 + B)
+    x = g.integers(-8, 9, (B, 300)).astype(np.float32)
+    layer = U.Layer.random(g, 70, 300, group, dtype, True, pow2=True).lay(hiplib)
+    want, _ = U.linear64(layer, x)
+    assert (np.abs(x) @ np.abs(layer.weights()).T).max() * 16 < 2 ** 24
+    assert np.array_equal(U.linear(hiplib, layer, x), U.rounded(want, dtype))
+    xs = np.exp2(g.integers(-2, 3, (B, 1))).astype(np.float32)
+    q = g.integers(-128, 128, (B, 300)).astype(np.int8)
+    want, _ = U.linear64(layer, q * xs.astype(np.float64))
+    assert (np.abs(q.astype(np.float64)) @ np.abs(layer.weights()).T).max() * 16 < 2 ** 24
+    assert np.array_equal(U.linear(hiplib, layer, q, xs=xs), U.rounded(want, dtype))
+
+
+@pytest.mark.parametrize("B", [1, 5, 40, 150])
+def test_fp32_values_keep_all_their_bits(hiplib, B):
+    """One element of a row of x is not zero, with 24 random bits and exponents far apart: the output is its product with
+    one weight.  n x and z x are sums of three exact products (two additions each), their difference and the scale round
+    once more, each by at most 2^-23 of (n + z) |x| s."""
+    g = U.rng(500)
+    nIn = 260
+    layer = U.Layer.random(g, 40, nIn, 64, F32, True).lay(hiplib)
+    at = g.integers(0, nIn, B)
+    v = (g.uniform(1, 2, B) * np.exp2(g.integers(-90, 90, B)) * g.choice([-1, 1], B)).astype(np.float32)
+    x = np.zeros((B, nIn), np.float32)
+    x[np.arange(B), at] = v
+    want, mag = U.linear64(layer, x)
+    assert (np.abs(U.linear(hiplib, layer, x) - want) <= 6 * 2.0 ** -23 * mag).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B", [1, 19, 140])
+@pytest.mark.parametrize("ldx,offx,ldy,offy", [(520, 0, 64, 0), (513, 3, 61, 1), (512, 4, 60, 2), (528, 8, 72, 8)])
+def test_strides_and_offsets(hiplib, dtype, B, ldx, offx, ldy, offy):
+    """Rows apart and off every vector's alignment; what lies between and behind them (NaNs) is neither used nor written."""
+    g, x, b = data(600, B, 500, 60, dtype)
+    layer = U.Layer.random(g, 60, 500, 128, dtype, False).lay(hiplib)
+    want, mag = U.linear64(layer, x, b)
+    U.check_linear(U.linear(hiplib, layer, x, b, ldx=ldx, offx=offx, ldy=ldy, offy=offy), want, mag, layer)
+    q = g.integers(-127, 128, (B, 500)).astype(np.int8)
+    xs = np.full((B, 1), 0.03125, np.float32)
+    want, mag = U.linear64(layer, q * 0.03125, b)
+    U.check_linear(U.linear(hiplib, layer, q, b, ldx=ldx, offx=offx, ldy=ldy, offy=offy, xs=xs), want, mag, layer)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B", [1, 18, 129])
+def test_threshold(hiplib, dtype, B):
+    g, x, b = data(700, B, 384, 45, dtype)
+    layer = U.Layer.random(g, 45, 384, 128, dtype, False).lay(hiplib)
+    plain = U.linear(hiplib, layer, x, b)
+    # (fp32 is compared before it is rounded, so values at the border itself are left out for the half types)
+    got = U.linear(hiplib, layer, x, b, act=1, thr=0.25, val=-1.5)
+    clear = np.abs(plain - 0.25) > 2 ** -8
+    assert np.array_equal(got[clear], np.where(plain > 0.25, plain, np.float32(-1.5))[clear])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B", [3, 33, 200])
+def test_a_row_with_nan_stays_alone(hiplib, dtype, B):
+    g, x, _ = data(800, B, 512, 40, dtype)
+    layer = U.Layer.random(g, 40, 512, 128, dtype, False).lay(hiplib)
+    clean = U.linear(hiplib, layer, x)
+    x[1, 77] = np.nan
+    x[2, 300] = np.inf
+    got = U.linear(hiplib, layer, x)
+    assert np.isnan(got[1]).all() and not np.isfinite(got[2]).any()
+    rest = np.arange(B) > 2
+    assert np.array_equal(got[rest], clean[rest]) and np.array_equal(got[0], clean[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B", [1, 40, 300])
+def test_twice_the_same_bits_and_nothing_allocated(hiplib, dtype, B):
+    g, x, b = data(900, B, 2048, 256, dtype)
+    layer = U.Layer.random(g, 256, 2048, 128, dtype, False).lay(hiplib)
+    first = U.linear(hiplib, layer, x, b)
+    assert np.array_equal(U.linear(hiplib, layer, x, b), first)
+    dx, dy = U.Rows(hiplib, U.raw(x, dtype)), api.DeviceArray(hiplib, nbytes=B * 256 * 4)
+    before = hiplib.thhip_alloc_calls()
+    assert hiplib.thhip_linear_w4(dx.ptr, dx.ld, layer.packed.ptr, None, dy.ptr, 256, B, 2048, 256, 128, 0, 0, 0.0, 0.0, dtype) == 0
+    assert hiplib.thhip_alloc_calls() == before
+    hiplib.thhip_sync()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("wtype", TYPES)
+@pytest.mark.parametrize("group,zeros,nIn", [(32, 0, 300), (64, 1, 333), (128, 1, 512), (256, 0, 700), (0, 1, 97)])
+def test_quantize(hiplib, dtype, wtype, group, zeros, nIn):
+    """Codes, scales and zeros are those of the formula, up to a code's choice at the middle between two; a constant-zero
+    group is 0; the layer made of them is within half a step of the weights (plus what a rounded scale moves)."""
+    g = U.rng(1000)
+    nOut, ldw = 21, nIn + 5
+    w = U.rounded(g.standard_normal((nOut, nIn)) * 0.05 + 0.02, wtype)
+    w[3] = 0
+    n = U.groups_of(nIn, group)
+    dw = U.Rows(hiplib, U.raw(w, wtype), ldw)
+    dc = U.Rows(hiplib, None, None, 0, (nOut, (nIn + 1) // 2), np.uint8)
+    ds = U.Rows(hiplib, None, None, 0, (nOut, n), np.uint32 if dtype == F32 else np.uint16)
+    dz = U.Rows(hiplib, None, None, 0, (nOut, n), np.uint8)
+    assert hiplib.thhip_quantize_w4(dw.ptr, ldw, wtype, dc.ptr, ds.ptr, dz.ptr if zeros else None, nOut, nIn, group, dtype) == 0
+    hiplib.thhip_sync()
+    codes, s = U.unpack_codes(dc.get(), nIn), U.unraw(ds.get(), dtype).astype(np.float64)
+    z = dz.get().astype(np.float64) if zeros else np.full((nOut, n), 8.0)
+    step = group or nIn
+    for i in range(n):
+        part = w[:, i * step:(i + 1) * step].astype(np.float64)
+        lo, hi = np.minimum(part.min(1), 0), np.maximum(part.max(1), 0)
+        top = (hi - lo) / 15 if zeros else np.maximum(hi, -lo) / 7
+        assert (np.abs(s[:, i] - top) <= (2 * U.HALF_STEP[dtype] + 2.0 ** -22) * top).all()
+        some = s[:, i] > 0
+        assert np.array_equal(some, np.arange(nOut) != 3)
+        exact = part[some] / s[some, i:i + 1] + z[some, i:i + 1]
+        if zeros:
+            assert (np.abs(z[some, i] - np.minimum(-lo[some] / s[some, i], 15)) <= 0.5 + 1e-5).all()
+        got = codes[some, i * step:(i + 1) * step]
+        assert (np.abs(got - np.clip(exact, 0, 15)) <= 0.5 + 1e-4).all()
+        assert (codes[3, i * step:(i + 1) * step] == z[3, i]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_from_weights_to_outputs(hiplib, dtype):
+    """quantise, pack and multiply in one go, as a program does; the product is that of the weights the codes stand for."""
+    g, x, b = data(1100, 9, 640, 72, dtype)
+    w = U.rounded(g.standard_normal((72, 640)) * 0.05, dtype)
+    dw = U.Rows(hiplib, U.raw(w, dtype))
+    dc, ds, dz = (api.DeviceArray(hiplib, nbytes=n) for n in (72 * 320, 72 * 10 * 4, 72 * 10))
+    assert hiplib.thhip_quantize_w4(dw.ptr, 640, dtype, dc.ptr, ds.ptr, dz.ptr, 72, 640, 64, dtype) == 0
+    layer = U.Layer(U.unpack_codes(dc.get((72, 320), np.uint8), 640), U.unraw(ds.get((72, 10), np.uint32 if dtype == F32 else np.uint16), dtype),
+                    dz.get((72, 10), np.uint8), 64, dtype)
+    layer.packed = api.DeviceArray(hiplib, nbytes=hiplib.thhip_w4_packed_bytes(72, 640, 64, dtype, 1))
+    assert hiplib.thhip_w4_pack(dc.ptr, ds.ptr, dz.ptr, layer.packed.ptr, 72, 640, 64, dtype) == 0
+    want, mag = U.linear64(layer, x, b)
+    U.check_linear(U.linear(hiplib, layer, x, b), want, mag, layer)
+    # half a step of 4 bits is a thirtieth of the range: the float layer's outputs are near
+    assert np.linalg.norm(want - (x.astype(np.float64) @ w.T.astype(np.float64) + b)) < 0.1 * np.linalg.norm(want)

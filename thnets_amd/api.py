@@ -165,6 +165,18 @@ PROTOTYPES = {
     "thhip_u8_rowsums": (vp, [vp, C.c_int, C.c_int]),
     "thhip_linear_pack_weight_u8": (vp, [vp, C.c_int, C.c_int]),
     "thhip_linear_batched_u8": (None, [vp, vp, vp, vp, vp] + [C.c_int] * 3 + [C.c_int] * 5 + [C.c_int] * 3),
+    "thhip_w4_packed_bytes": (C.c_size_t, [C.c_int] * 5),
+    "thhip_w4_pack": (C.c_int, [vp, vp, vp, vp] + [C.c_int] * 4),
+    "thhip_quantize_w4": (C.c_int, [vp, C.c_long, C.c_int, vp, vp, vp] + [C.c_int] * 4),
+    "thhip_linear_w4": (C.c_int, [vp, C.c_long, vp, vp, vp, C.c_long] + [C.c_int] * 6 + [C.c_float, C.c_float, C.c_int]),
+    "thhip_linear_w4_i8": (C.c_int, [vp, C.c_long, vp, C.c_int, vp, vp, vp, C.c_long] + [C.c_int] * 6 +
+                           [C.c_float, C.c_float, C.c_int]),
+    "thhip_rmsnorm": (C.c_int, [vp, C.c_long, vp, C.c_long, vp, C.c_float, vp, C.c_long, vp, C.c_long, C.c_long, C.c_long,
+                                C.c_int]),
+    "thhip_rmsnorm_i8": (C.c_int, [vp, C.c_long, vp, C.c_long, vp, C.c_float, vp, C.c_long, vp, C.c_long, vp, C.c_int,
+                                   C.c_long, C.c_long, C.c_int]),
+    "thhip_quantize_rows": (C.c_int, [vp, C.c_long, vp, C.c_long, vp, C.c_int, C.c_long, C.c_long, C.c_int]),
+    "thhip_dequantize_rows": (C.c_int, [vp, C.c_long, vp, C.c_int, vp, C.c_long, C.c_long, C.c_long, C.c_int]),
     "thhip_rgb2code": (None, [vp, vp, C.c_int, C.c_int, C.c_int, vp, vp, C.c_int, c_fp, c_fp]),
     "thhip_rgb2code_batch": (None, [vp, vp, C.c_int, C.c_long, C.c_int, C.c_int, C.c_int, vp, vp, C.c_int, c_fp, c_fp]),
     "thhip_threshold_u8": (None, [vp, vp, C.c_long, C.c_int, C.c_int, C.c_int]),

@@ -1,0 +1,576 @@
+/*
+ * Linear layers whose weights have 4 bits.
+ *
+ *   y[b][o] = act(bias[o] + sum_g s[o][g] * sum_{k in g} (n[o][k] - z[o][g]) * x[b][k])
+ *
+ * n: codes 0 .. 15; a group of `group` consecutive k of a row shares a scale s and a zero
+ * point z (8 where the layer has none).  x is fp32 / fp16 / bf16, or signed 8-bit codes q with
+ * fp32 scales, x[b][k] = sx[b][g'] * q[b][k].  The reference's Linear (modules/Linear.c:72-113)
+ * knows fp32 weights only; its 8-bit path (lowp_basic.c:299-321) one range for the whole matrix.
+ *
+ * Arithmetic.  Inside a group the matrix cores sum n * x with the codes as they are (0 .. 15 is
+ * exact in every type) and, with a matrix of ones, sum x; both in fp32 (int32 for 8-bit x, where
+ * they are exact).  A finished group adds s * (sum n x - z * sum x) to the fp32 result, so a
+ * weight is never rounded and the scale is applied once a group.  fp32 x is cut into three bf16
+ * parts of eight bits each that add up to it exactly.
+ *
+ * A code becomes a half value without an integer conversion: the byte 0000nnnn read as an e4m3
+ * number is n * 2^-9 for all sixteen codes (eight denormals, eight of the first binade), and
+ * v_cvt_scalef32_pk_{f16,bf16}_fp8 widens two of them with a factor of 2^9.  For 8-bit x the
+ * nibble goes to the high half of its byte, where it is 16 (n - 8) once its top bit is flipped.
+ *
+ * Weights are packed by thhip_w4_pack into one buffer:
+ *   codes   [16-row block][step of 128 k][lane][4 words], word j of lane l: row l % 16,
+ *           k = 32 j + 8 (l / 16) + 0 .. 7, low nibbles of the four bytes first, then the high
+ *           ones: 1 KiB that a wavefront loads with one instruction and multiplies as it lies
+ *   scales  [16-row block][group][16 rows], fp32 / fp16 / bf16
+ *   zeros   [16-row block][group][16 rows], bytes (only where the layer has zero points)
+ * Rows past nOut and k past nIn are padded with 0.
+ */
+#include <stdint.h>
+#include <stdio.h>
+#include "thhip_internal.h"
+
+#define W4_KSTEP 128	/* k of a packed step: four matrix instructions of 32 */
+#define W4_X_I8 3	/* kind of x beside THHIP_F32, _F16, _BF16 */
+
+struct w4_layout {
+	int blocks, steps, groups;
+	size_t scales, zeros, bytes;	/* offsets of the sections, and the whole */
+};
+
+static size_t round16(size_t n)
+{
+	return (n + 15) & ~(size_t)15;
+}
+
+static struct w4_layout w4_layout_of(int nOut, int nIn, int group, int dtype, int zeros)
+{
+	struct w4_layout l;
+	l.blocks = (int)(((long)nOut + 15) / 16);
+	l.steps = (int)(((long)nIn + W4_KSTEP - 1) / W4_KSTEP);
+	l.groups = group ? (int)(((long)nIn + group - 1) / group) : 1;
+	l.scales = (size_t)l.blocks * l.steps * 1024;
+	l.zeros = l.scales + round16((size_t)l.blocks * l.groups * 16 * thhip_esize(dtype));
+	l.bytes = l.zeros + (zeros ? (size_t)l.blocks * l.groups * 16 : 0);
+	return l;
+}
+
+static const char *w4_bad(int nOut, int nIn, int group, int dtype)
+{
+	if (nOut < 1 || nIn < 1 || nOut > 1 << 30 || nIn > 1 << 30)
+		return "a layer has 1 to 2^30 inputs and outputs";
+	if (group != 0 && group != 32 && group != 64 && group != 128 && group != 256)
+		return "a group has 32, 64, 128 or 256 weights, or is the row (0)";
+	if (dtype != THHIP_F32 && dtype != THHIP_F16 && dtype != THHIP_BF16)
+		return "the type is fp32, fp16 or bf16";
+	return 0;
+}
+
+extern "C" size_t thhip_w4_packed_bytes(int nOut, int nIn, int group, int dtype, int zeros)
+{
+	return w4_bad(nOut, nIn, group, dtype) ? 0 : w4_layout_of(nOut, nIn, group, dtype, zeros).bytes;
+}
+
+/* ---- laying out and making weights ---- */
+
+__global__ __launch_bounds__(256) void w4_pack_codes_kernel(const unsigned char *codes, unsigned *out, int nOut, int nIn,
+	int steps, size_t words)
+{
+	const size_t row_bytes = ((size_t)nIn + 1) / 2;
+	for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (size_t)gridDim.x * 256) {
+		const int j = i & 3, lane = (i >> 2) & 63;
+		const size_t step = i >> 8;
+		const long row = (long)(step / steps) * 16 + (lane & 15);
+		const long k0 = (long)(step % steps) * W4_KSTEP + 32 * j + 8 * (lane >> 4);
+		unsigned w = 0;
+		if (row < nOut)
+			for (int e = 0; e < 8; e++)
+				if (k0 + e < nIn) {
+					const unsigned n = (codes[row * row_bytes + (k0 + e) / 2] >> (4 * ((k0 + e) & 1))) & 15;
+					w |= n << (8 * (e & 3) + 4 * (e >> 2));
+				}
+		out[i] = w;
+	}
+}
+
+/* scales or zeros: [nOut][groups] -> [16-row block][group][16 rows], esize bytes each */
+__global__ __launch_bounds__(256) void w4_pack_groups_kernel(const unsigned char *in, unsigned char *out, int nOut, int groups,
+	int esize, size_t n)
+{
+	for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+		const size_t g = (i >> 4) % groups;
+		const long row = (long)((i >> 4) / groups) * 16 + (long)(i & 15);
+		for (int b = 0; b < esize; b++)
+			out[i * esize + b] = row < nOut ? in[(row * groups + g) * esize + b] : 0;
+	}
+}
+
+static unsigned w4_grid(size_t n)
+{
+	const size_t g = (n + 255) / 256;
+	return (unsigned)(g < 65536 ? g : 65536);
+}
+
+extern "C" int thhip_w4_pack(const unsigned char *codes, const void *scales, const unsigned char *zeros, void *packed,
+	int nOut, int nIn, int group, int dtype)
+{
+	const char *bad = w4_bad(nOut, nIn, group, dtype);
+	if (!bad && (!codes || !scales || !packed))
+		bad = "codes, scales and the packed buffer are needed";
+	if (!bad && (uintptr_t)packed % 16)
+		bad = "the packed buffer is not aligned to 16 bytes";
+	if (bad) {
+		fprintf(stderr, "thhip_w4_pack: %d -> %d, group %d, dtype %d: %s\n", nIn, nOut, group, dtype, bad);
+		return -1;
+	}
+	const struct w4_layout l = w4_layout_of(nOut, nIn, group, dtype, zeros != 0);
+	ThhipLaunchScope scope(THHIP_FAM_OTHER, (double)nOut * nIn / 2 + (double)l.bytes);
+	const size_t words = l.scales / 4, ns = (size_t)l.blocks * l.groups * 16;
+	w4_pack_codes_kernel<<<dim3(w4_grid(words)), dim3(256), 0, thhip_stream()>>>(codes, (unsigned *)packed, nOut, nIn, l.steps, words);
+	w4_pack_groups_kernel<<<dim3(w4_grid(ns)), dim3(256), 0, thhip_stream()>>>((const unsigned char *)scales,
+		(unsigned char *)packed + l.scales, nOut, l.groups, thhip_esize(dtype), ns);
+	if (zeros)
+		w4_pack_groups_kernel<<<dim3(w4_grid(ns)), dim3(256), 0, thhip_stream()>>>(zeros, (unsigned char *)packed + l.zeros,
+			nOut, l.groups, 1, ns);
+	return 0;
+}
+
+/* One wavefront a (row, group): the group's extremes, its scale rounded to the type it is kept in,
+ * and the codes nearest to w / scale (+ zero).  Two weights of a byte belong to one lane. */
+template <int WDT, int DT>
+__global__ __launch_bounds__(256) void w4_quantize_kernel(const void *w, long ldw, unsigned char *codes, void *scales,
+	unsigned char *zeros, int nOut, int nIn, int group, int groups)
+{
+	const int lane = threadIdx.x & 63;
+	const size_t n = (size_t)nOut * groups;
+	for (size_t i = (size_t)blockIdx.x * 4 + threadIdx.x / 64; i < n; i += (size_t)gridDim.x * 4) {
+		const long row = (long)(i / groups);
+		const int g = (int)(i % groups);
+		const int k0 = g * group, k1 = group && k0 + group < nIn ? k0 + group : nIn;
+		float lo = 0, hi = 0;
+		for (int k = k0 + lane; k < k1; k += 64) {
+			const float v = ThhipElem<WDT>::ld(w, row * ldw + k);
+			lo = fminf(lo, v);
+			hi = fmaxf(hi, v);
+		}
+#pragma unroll
+		for (int off = 32; off > 0; off >>= 1) {
+			lo = fminf(lo, __shfl_xor(lo, off, 64));
+			hi = fmaxf(hi, __shfl_xor(hi, off, 64));
+		}
+		typename ThhipElem<DT>::T sr = (typename ThhipElem<DT>::T)(zeros ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f);
+		const float s = (float)sr, inv = s > 0 ? 1.0f / s : 0.0f;
+		const float z = zeros ? fminf(rintf(-lo * inv), 15.0f) : 8.0f;
+		if (lane == 0) {
+			ThhipElem<DT>::st(scales, (long)i, s);
+			if (zeros)
+				zeros[i] = (unsigned char)(int)z;
+		}
+		for (int k = k0 + 2 * lane; k < k1; k += 128) {
+			unsigned b = 0;
+			for (int e = 0; e < 2 && k + e < k1; e++) {
+				const float v = ThhipElem<WDT>::ld(w, row * ldw + k + e);
+				b |= (unsigned)(int)fminf(fmaxf(rintf(v * inv) + z, 0.0f), 15.0f) << (4 * e);
+			}
+			codes[row * (((long)nIn + 1) / 2) + k / 2] = (unsigned char)b;
+		}
+	}
+}
+
+extern "C" int thhip_quantize_w4(const void *w, long ldw, int wtype, unsigned char *codes, void *scales, unsigned char *zeros,
+	int nOut, int nIn, int group, int dtype)
+{
+	const char *bad = w4_bad(nOut, nIn, group, dtype);
+	if (!bad && wtype != THHIP_F32 && wtype != THHIP_F16 && wtype != THHIP_BF16)
+		bad = "the weights are fp32, fp16 or bf16";
+	if (!bad && (!w || !codes || !scales))
+		bad = "weights, codes and scales are needed";
+	if (!bad && ldw < nIn)
+		bad = "the row stride is smaller than the row";
+	if (bad) {
+		fprintf(stderr, "thhip_quantize_w4: %d -> %d, group %d, types %d %d: %s\n", nIn, nOut, group, wtype, dtype, bad);
+		return -1;
+	}
+	const int groups = group ? (int)(((long)nIn + group - 1) / group) : 1;
+	const unsigned grid = w4_grid(((size_t)nOut * groups + 3) / 4 * 256);
+	ThhipLaunchScope scope(THHIP_FAM_OTHER, (double)nOut * nIn * (thhip_esize(wtype) + 0.5));
+#define W4_QUANTIZE(WDT) THHIP_DISPATCH_FLOAT(dtype, (w4_quantize_kernel<WDT, DT><<<dim3(grid), dim3(256), 0, thhip_stream()>>>( \
+	w, ldw, codes, scales, zeros, nOut, nIn, group, groups)))
+	if (wtype == THHIP_F32)
+		W4_QUANTIZE(THHIP_F32);
+	else if (wtype == THHIP_F16)
+		W4_QUANTIZE(THHIP_F16);
+	else
+		W4_QUANTIZE(THHIP_BF16);
+#undef W4_QUANTIZE
+	return 0;
+}
+
+/* ---- the product ---- */
+
+struct w4_args {
+	const void *x;
+	const float *xscale;
+	const unsigned char *codes;
+	const void *scales;
+	const unsigned char *zeros;
+	const float *bias;
+	void *y;
+	long ldx, ldy;
+	int B, nIn, nOut, steps, blocks, groups, group;
+	int xgroups;		/* scales of a row of 8-bit x: 1, or one a group */
+	int xvec;		/* rows of x may be loaded eight elements at a time */
+	int act;
+	float thr, val;
+};
+
+/* What differs with the kind of x: the matrix core's operand of eight k, its accumulator, and how a
+ * word of eight codes and eight elements of x become operands.  PARTS: operands an x vector makes. */
+template <int X> struct W4X;
+
+template <> struct W4X<THHIP_F16> {
+	typedef _Float16 E;
+	typedef halfx8 V;
+	typedef floatx4 A;
+	static constexpr int PARTS = 1;
+	static __device__ __forceinline__ V ones() { return (V)(_Float16)1.0f; }
+	static __device__ __forceinline__ V weights(unsigned w)
+	{
+		typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+		const unsigned lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+		const h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, true);
+		const h2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, true);
+		return (V){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+	}
+	static __device__ __forceinline__ A mma(V a, V b, A c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+	static __device__ __forceinline__ void operand(const E *x, V *out)
+	{
+#pragma unroll
+		for (int e = 0; e < 8; e++)
+			out[0][e] = x[e];
+	}
+};
+
+template <> struct W4X<THHIP_BF16> {
+	typedef __bf16 E;
+	typedef bf16x8 V;
+	typedef floatx4 A;
+	static constexpr int PARTS = 1;
+	static __device__ __forceinline__ V ones() { return (V)(__bf16)1.0f; }
+	static __device__ __forceinline__ V weights(unsigned w)
+	{
+		typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+		const unsigned lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+		const b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, true);
+		const b2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, true);
+		return (V){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+	}
+	static __device__ __forceinline__ A mma(V a, V b, A c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+	static __device__ __forceinline__ void operand(const E *x, V *out)
+	{
+#pragma unroll
+		for (int e = 0; e < 8; e++)
+			out[0][e] = x[e];
+	}
+};
+
+/* fp32: x = a + b + c, each the top sixteen bits of what is left (so eight bits of x; exact).  An
+ * infinity leaves NaN behind: it makes every output of its row NaN. */
+template <> struct W4X<THHIP_F32> {
+	typedef float E;
+	typedef bf16x8 V;
+	typedef floatx4 A;
+	static constexpr int PARTS = 3;
+	static __device__ __forceinline__ V ones() { return W4X<THHIP_BF16>::ones(); }
+	static __device__ __forceinline__ V weights(unsigned w) { return W4X<THHIP_BF16>::weights(w); }
+	static __device__ __forceinline__ A mma(V a, V b, A c) { return W4X<THHIP_BF16>::mma(a, b, c); }
+	static __device__ __forceinline__ void operand(const E *x, V *out)
+	{
+		typedef unsigned U __attribute__((ext_vector_type(4)));
+		U p[3];
+#pragma unroll
+		for (int e = 0; e < 8; e += 2) {
+			float u = x[e], v = x[e + 1];
+#pragma unroll
+			for (int i = 0; i < 3; i++) {
+				const unsigned ub = __float_as_uint(u), vb = __float_as_uint(v);
+				p[i][e / 2] = (ub >> 16) | (vb & 0xffff0000u);
+				u -= __uint_as_float(ub & 0xffff0000u);
+				v -= __uint_as_float(vb & 0xffff0000u);
+			}
+		}
+#pragma unroll
+		for (int i = 0; i < 3; i++)
+			out[i] = __builtin_bit_cast(V, p[i]);
+	}
+};
+
+template <> struct W4X<W4_X_I8> {
+	typedef signed char E;
+	typedef long V;
+	typedef intx4 A;
+	static constexpr int PARTS = 1;
+	static __device__ __forceinline__ V ones() { return 0x0101010101010101l; }
+	static __device__ __forceinline__ V weights(unsigned w)
+	{
+		const unsigned s = w ^ 0x88888888u;
+		return (V)((unsigned long)((s << 4) & 0xf0f0f0f0u) | (unsigned long)(s & 0xf0f0f0f0u) << 32);
+	}
+	static __device__ __forceinline__ A mma(V a, V b, A c) { return __builtin_amdgcn_mfma_i32_16x16x32_i8(a, b, c, 0, 0, 0); }
+	static __device__ __forceinline__ void operand(const E *x, V *out)
+	{
+		unsigned long v = 0;
+#pragma unroll
+		for (int e = 0; e < 8; e++)
+			v |= (unsigned long)(unsigned char)x[e] << (8 * e);
+		out[0] = (V)v;
+	}
+};
+
+/* Scales (or zeros) of the four rows a lane's accumulators belong to, as fp32 */
+template <int DT>
+__device__ __forceinline__ floatx4 w4_scales(const void *p, long i)
+{
+	typedef typename ThhipElem<DT>::T T4 __attribute__((ext_vector_type(4)));
+	const T4 v = *(const T4 *)((const typename ThhipElem<DT>::T *)p + i);
+	floatx4 f;
+#pragma unroll
+	for (int e = 0; e < 4; e++)
+		f[e] = (float)v[e];
+	return f;
+}
+
+/* A workgroup of W wavefronts computes RB blocks of 16 rows for 16 NB batch columns (gridDim.y slices
+ * of the batch); wavefront w takes the steps w, w + W, ... of K, and the partial sums are added through
+ * LDS in the order of the wavefronts.  Of a 16 x 16 tile a lane holds rows 4 (lane / 16) + 0 .. 3 of column
+ * lane % 16.  GM: matrix instructions a group spans within a step (1: groups of 32 or 64, 4: larger). */
+template <int X, int DT, int RB, int NB, int GM, int W>
+__global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args a)
+{
+	typedef W4X<X> K;
+	typedef typename K::V V;
+	typedef typename K::A A;
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+	const int col = lane & 15, quarter = lane >> 4;
+	const int rb0 = blockIdx.x * RB, b0 = blockIdx.y * NB * 16;
+	floatx4 acc[RB][NB];
+#pragma unroll
+	for (int r = 0; r < RB; r++)
+#pragma unroll
+		for (int n = 0; n < NB; n++)
+			acc[r][n] = (floatx4)0.0f;
+
+	for (int step = wave; step < a.steps; step += W) {
+		uintx4 codes[RB];
+#pragma unroll
+		for (int r = 0; r < RB; r++) {
+			const int rb = rb0 + r < a.blocks ? rb0 + r : a.blocks - 1;
+			codes[r] = *(const uintx4 *)(a.codes + ((size_t)rb * a.steps + step) * 1024 + lane * 16);
+		}
+		const long k0 = (long)step * W4_KSTEP + 8 * quarter;
+		A p[RB][NB], sx[NB];
+#pragma unroll
+		for (int j = 0; j < 4; j++) {
+			if (j % GM == 0) {
+#pragma unroll
+				for (int n = 0; n < NB; n++) {
+					sx[n] = (A)0;
+#pragma unroll
+					for (int r = 0; r < RB; r++)
+						p[r][n] = (A)0;
+				}
+			}
+			V w[RB];
+#pragma unroll
+			for (int r = 0; r < RB; r++)
+				w[r] = K::weights(codes[r][j]);
+#pragma unroll
+			for (int n = 0; n < NB; n++) {
+				const int b = b0 + n * 16 + col;
+				const long k = k0 + 32 * j;
+				typename K::E e[8];
+#pragma unroll
+				for (int i = 0; i < 8; i++)
+					e[i] = (typename K::E)0;
+				if (b < a.B) {
+					const typename K::E *row = (const typename K::E *)a.x + b * a.ldx;
+					if (a.xvec && k + 8 <= a.nIn) {
+						typedef typename K::E E8 __attribute__((ext_vector_type(8)));
+						const E8 v = *(const E8 *)(row + k);
+#pragma unroll
+						for (int i = 0; i < 8; i++)
+							e[i] = v[i];
+					} else {
+#pragma unroll
+						for (int i = 0; i < 8; i++)
+							if (k + i < a.nIn)
+								e[i] = row[k + i];
+					}
+				}
+				V x[K::PARTS];
+				K::operand(e, x);
+#pragma unroll
+				for (int i = 0; i < K::PARTS; i++) {
+					sx[n] = K::mma(K::ones(), x[i], sx[n]);
+#pragma unroll
+					for (int r = 0; r < RB; r++)
+						p[r][n] = K::mma(w[r], x[i], p[r][n]);
+				}
+			}
+			if ((j + 1) % GM == 0) {
+				const long kg = (long)step * W4_KSTEP + 32 * j;
+				const int g = a.group ? (int)(kg / a.group) : 0;
+				if (kg >= a.nIn && g >= a.groups)	/* (padding past the last group) */
+					continue;
+#pragma unroll
+				for (int r = 0; r < RB; r++) {
+					const int rb = rb0 + r < a.blocks ? rb0 + r : a.blocks - 1;
+					const long at = ((long)rb * a.groups + g) * 16 + 4 * quarter;
+					floatx4 s = w4_scales<DT>(a.scales, at), z = (floatx4)8.0f;
+					if (a.zeros) {
+						const unsigned zw = *(const unsigned *)(a.zeros + at);
+#pragma unroll
+						for (int i = 0; i < 4; i++)
+							z[i] = (float)((zw >> (8 * i)) & 255);
+					}
+#pragma unroll
+					for (int n = 0; n < NB; n++) {
+						const int b = b0 + n * 16 + col;
+						const float xs = X == W4_X_I8 && a.xgroups > 1 ? a.xscale[(long)(b < a.B ? b : a.B - 1) * a.xgroups + g] : 1.0f;
+#pragma unroll
+						for (int i = 0; i < 4; i++) {
+							if constexpr (X == W4_X_I8)
+								acc[r][n][i] += s[i] * xs * (0.0625f * (float)p[r][n][i] - (z[i] - 8.0f) * (float)sx[n][i]);
+							else
+								acc[r][n][i] += s[i] * (p[r][n][i] - z[i] * sx[n][i]);
+						}
+					}
+				}
+			}
+		}
+	}
+
+	__shared__ floatx4 red[W][RB * NB][64];
+#pragma unroll
+	for (int r = 0; r < RB; r++)
+#pragma unroll
+		for (int n = 0; n < NB; n++)
+			red[wave][r * NB + n][lane] = acc[r][n];
+	__syncthreads();
+	for (int t = wave; t < RB * NB; t += W) {
+		floatx4 v = red[0][t][lane];
+#pragma unroll
+		for (int i = 1; i < W; i++)
+			v += red[i][t][lane];
+		const int b = b0 + (t % NB) * 16 + col;
+		if (b >= a.B)
+			continue;
+		const float xs = X == W4_X_I8 && a.xgroups == 1 ? a.xscale[b] : 1.0f;
+#pragma unroll
+		for (int i = 0; i < 4; i++) {
+			const int o = (rb0 + t / NB) * 16 + 4 * quarter + i;
+			if (o >= a.nOut)
+				continue;
+			float y = v[i] * xs + (a.bias ? a.bias[o] : 0.0f);
+			if (a.act)
+				y = y > a.thr ? y : a.val;
+			ThhipElem<DT>::st(a.y, b * a.ldy + o, y);
+		}
+	}
+}
+
+/* A grid has at most 65535 slices of the batch: larger batches go into further launches */
+#define W4_SLICES 65535
+
+template <int X, int DT, int RB, int NB, int GM>
+static void w4_skinny_launch(w4_args a)
+{
+	constexpr int W = 8;
+	const long esx = X == W4_X_I8 ? 1 : thhip_esize(X), esy = thhip_esize(DT);
+	for (long left = a.B; left > 0; left -= (long)W4_SLICES * NB * 16) {
+		a.B = (int)(left < (long)W4_SLICES * NB * 16 ? left : (long)W4_SLICES * NB * 16);
+		w4_skinny_kernel<X, DT, RB, NB, GM, W><<<dim3((a.blocks + RB - 1) / RB, (a.B + NB * 16 - 1) / (NB * 16)), dim3(W * 64), 0,
+			thhip_stream()>>>(a);
+		a.x = (const char *)a.x + a.B * a.ldx * esx;
+		a.y = (char *)a.y + a.B * a.ldy * esy;
+		a.xscale = a.xscale ? a.xscale + (long)a.B * a.xgroups : 0;
+	}
+}
+
+template <int X, int DT, int GM>
+static void w4_choose(const w4_args &a)
+{
+	if (a.B <= 16)
+		w4_skinny_launch<X, DT, 1, 1, GM>(a);
+	else
+		w4_skinny_launch<X, DT, 2, 2, GM>(a);
+}
+
+template <int X, int DT>
+static void w4_groups(const w4_args &a)
+{
+	if (a.group == 32 || a.group == 64)
+		w4_choose<X, DT, 1>(a);
+	else
+		w4_choose<X, DT, 4>(a);
+}
+
+static int w4_run(const char *who, w4_args &a, const void *packed, int group, int zeros, int xkind, int xgroup, int dtype)
+{
+	const char *bad = w4_bad(a.nOut, a.nIn, group, dtype);
+	const size_t es = dtype == THHIP_F32 ? 4 : 2, esx = xkind == W4_X_I8 ? 1 : es;
+	if (!bad && a.B < 0)
+		bad = "a batch has at least no rows";
+	if (!bad && (a.ldx < a.nIn || a.ldy < a.nOut))
+		bad = "a row stride is smaller than the row";
+	if (!bad && a.B && (!a.x || !packed || !a.y || (xkind == W4_X_I8 && !a.xscale)))
+		bad = "x, the weights and y are needed";
+	if (!bad && ((uintptr_t)a.x % esx || (uintptr_t)a.y % es || (uintptr_t)packed % 16 || (uintptr_t)a.bias % 4 || (uintptr_t)a.xscale % 4))
+		bad = "a pointer is not aligned to its element (packed weights: 16 bytes)";
+	if (!bad && xkind == W4_X_I8 && xgroup != 0 && xgroup != group)
+		bad = "the scales of x are one a row (0) or one a group of the weights";
+	if (bad) {
+		fprintf(stderr, "%s: B=%d %d -> %d, group %d, dtype %d: %s\n", who, a.B, a.nIn, a.nOut, group, dtype, bad);
+		return -1;
+	}
+	if (!a.B)
+		return 0;
+	const struct w4_layout l = w4_layout_of(a.nOut, a.nIn, group, dtype, zeros);
+	a.codes = (const unsigned char *)packed;
+	a.scales = (const char *)packed + l.scales;
+	a.zeros = zeros ? (const unsigned char *)packed + l.zeros : 0;
+	a.steps = l.steps;
+	a.blocks = l.blocks;
+	a.groups = l.groups;
+	a.group = group;
+	a.xgroups = xgroup ? l.groups : 1;
+	const size_t xv = esx * 8 < 16 ? esx * 8 : 16;
+	a.xvec = (uintptr_t)a.x % xv == 0 && a.ldx * esx % xv == 0;
+	ThhipLaunchScope scope(THHIP_FAM_GEMV, (double)a.nOut * a.nIn / 2 + (double)a.nOut * l.groups * (es + (zeros ? 1 : 0)) +
+		(double)a.B * a.nIn * esx + (double)a.B * a.nOut * es);
+	if (xkind == W4_X_I8)
+		THHIP_DISPATCH_FLOAT(dtype, (w4_groups<W4_X_I8, DT>(a)));
+	else
+		THHIP_DISPATCH_FLOAT(dtype, (w4_groups<DT, DT>(a)));
+	return 0;
+}
+
+extern "C" int thhip_linear_w4(const void *x, long ldx, const void *wpacked, const float *bias, void *y, long ldy,
+	int B, int nIn, int nOut, int group, int zeros, int act, float thr, float val, int dtype)
+{
+	w4_args a = {};
+	a.x = x; a.ldx = ldx; a.bias = bias; a.y = y; a.ldy = ldy;
+	a.B = B; a.nIn = nIn; a.nOut = nOut; a.act = act; a.thr = thr; a.val = val;
+	return w4_run("thhip_linear_w4", a, wpacked, group, zeros, dtype, 0, dtype);
+}
+
+extern "C" int thhip_linear_w4_i8(const signed char *x, long ldx, const float *xscale, int xgroup, const void *wpacked,
+	const float *bias, void *y, long ldy, int B, int nIn, int nOut, int group, int zeros, int act, float thr, float val,
+	int dtype)
+{
+	w4_args a = {};
+	a.x = x; a.ldx = ldx; a.xscale = xscale; a.bias = bias; a.y = y; a.ldy = ldy;
+	a.B = B; a.nIn = nIn; a.nOut = nOut; a.act = act; a.thr = thr; a.val = val;
+	return w4_run("thhip_linear_w4_i8", a, wpacked, group, zeros, W4_X_I8, xgroup, dtype);
+}

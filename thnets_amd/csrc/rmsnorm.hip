@@ -1,0 +1,488 @@
+/*
+ * Root-mean-square norm of rows with a residual's addition, and rows of signed
+ * 8-bit codes with scales.
+ *
+ *   h = x + res                       (fp32; sum = h rounded to the type of x)
+ *   y = h * w / sqrt(mean(h * h) + eps)
+ *   scale = max|y| / 127,  q = rint(127 y / max|y|)     over a row or a group
+ *
+ * The reference has neither (its norm is nn_SpatialBatchNormalization_updateOutput,
+ * modules/SpatialBatchNormalization.c:57-116, its 8-bit codes are unsigned with one
+ * range for a tensor, lowp_basic.c:15-35): they belong to networks of Linear layers,
+ * beside thhip_linear_w4 and thhip_linear_w4_i8.
+ *
+ * Bound by memory: every element is read once, kept in registers while the row's
+ * sum of squares (and largest |h w|) goes through the wavefronts, and written once.
+ * h stays in fp32 between the addition and the norm, so the norm is that of the
+ * unrounded sum, and y is rounded once.
+ */
+#include <stdint.h>
+#include <stdio.h>
+#include "thhip_internal.h"
+
+enum { ROWS_NORM, ROWS_NORM_I8, ROWS_QUANT };
+
+struct rows_args {
+	const void *x, *res;
+	const float *w;
+	void *sum, *y;
+	signed char *q;
+	float *scale;
+	long ldx, ldr, lds, ldy, ldq;
+	long rows;
+	int cols, group, ngroups, vec;
+	float eps;
+};
+
+/* N consecutive elements of a row (16 bytes): a vector load / store where pointers and strides allow it
+ * and the elements are all inside the row, one by one otherwise; elements past the row read as 0 */
+template <int DT> struct RowVec {
+	static constexpr int N = DT == THHIP_F32 ? 4 : 8;
+	typedef typename ThhipElem<DT>::T T;
+	typedef T V __attribute__((ext_vector_type(N)));
+	static __device__ __forceinline__ void load(const void *p, long base, int col, int cols, int vec, float *out)
+	{
+		if (vec && col + N <= cols) {
+			const V v = *(const V *)((const T *)p + base + col);
+#pragma unroll
+			for (int i = 0; i < N; i++)
+				out[i] = (float)v[i];
+		} else {
+#pragma unroll
+			for (int i = 0; i < N; i++)
+				out[i] = col + i < cols ? ThhipElem<DT>::ld(p, base + col + i) : 0.0f;
+		}
+	}
+	static __device__ __forceinline__ void store(void *p, long base, int col, int cols, int vec, const float *in)
+	{
+		if (vec && col + N <= cols) {
+			V v;
+#pragma unroll
+			for (int i = 0; i < N; i++)
+				v[i] = (T)in[i];
+			*(V *)((T *)p + base + col) = v;
+		} else {
+#pragma unroll
+			for (int i = 0; i < N; i++)
+				if (col + i < cols)
+					ThhipElem<DT>::st(p, base + col + i, in[i]);
+		}
+	}
+};
+
+template <int N>
+__device__ __forceinline__ void store_codes(signed char *p, long base, int col, int cols, int vec, const float *y, float inv)
+{
+	unsigned w[N / 4];
+#pragma unroll
+	for (int i = 0; i < N / 4; i++)
+		w[i] = 0;
+#pragma unroll
+	for (int i = 0; i < N; i++) {
+		const float t = fminf(fmaxf(rintf(y[i] * inv), -127.0f), 127.0f);
+		w[i / 4] |= ((unsigned)(int)t & 255u) << (8 * (i % 4));
+	}
+	if (vec && col + N <= cols) {
+#pragma unroll
+		for (int i = 0; i < N / 4; i++)
+			((unsigned *)(p + base + col))[i] = w[i];
+	} else {
+#pragma unroll
+		for (int i = 0; i < N; i++)
+			if (col + i < cols)
+				p[base + col + i] = (signed char)(w[i / 4] >> (8 * (i % 4)));
+	}
+}
+
+/* |v| as an unsigned number: orders as |v| does, infinity above every number and a NaN above
+ * infinity, so that a NaN reaches the scale of its row or group */
+__device__ __forceinline__ unsigned abs_bits(float v)
+{
+	return __float_as_uint(v) & 0x7fffffffu;
+}
+
+/* What a value is multiplied with to give its code: 127 / top.  A top below 2^-116 (whose
+ * reciprocal would overflow) counts as nothing: scale 0, codes 0. */
+__device__ __forceinline__ float code_factor(float top)
+{
+	return top < 1.2e-35f ? 0.0f : 127.0f / top;	/* (a NaN stays one) */
+}
+
+__device__ __forceinline__ float code_scale(float top)
+{
+	return top < 1.2e-35f ? 0.0f : top / 127.0f;
+}
+
+__device__ __forceinline__ float lanes_sum(float v)
+{
+#pragma unroll
+	for (int off = 32; off > 0; off >>= 1)
+		v += __shfl_xor(v, off, 64);
+	return v;
+}
+
+__device__ __forceinline__ unsigned lanes_max(unsigned v, int lanes)
+{
+	for (int off = lanes >> 1; off > 0; off >>= 1) {
+		const unsigned o = __shfl_xor(v, off, 64);
+		v = o > v ? o : v;
+	}
+	return v;
+}
+
+/* Sum and maximum over the T threads of a row, T = 64 (a wavefront) or the whole workgroup */
+template <int T>
+__device__ __forceinline__ void row_reduce(float &s, unsigned &m)
+{
+	s = lanes_sum(s);
+	m = lanes_max(m, 64);
+	if constexpr (T > 64) {
+		constexpr int W = T / 64;
+		__shared__ float ps[W];
+		__shared__ unsigned pm[W];
+		if ((threadIdx.x & 63) == 0) {
+			ps[threadIdx.x >> 6] = s;
+			pm[threadIdx.x >> 6] = m;
+		}
+		__syncthreads();
+		s = ps[0];
+		m = pm[0];
+#pragma unroll
+		for (int i = 1; i < W; i++) {
+			s += ps[i];
+			m = pm[i] > m ? pm[i] : m;
+		}
+	}
+}
+
+/* One vector of a row on its way out: y, or codes and (by the group's first lane) its scale */
+template <int DT, int MODE>
+__device__ __forceinline__ void row_out(const rows_args &a, long row, int col, const float *h, const float *w, float rstd,
+	float row_inv)
+{
+	constexpr int N = RowVec<DT>::N;
+	float y[N];
+#pragma unroll
+	for (int i = 0; i < N; i++)
+		y[i] = MODE == ROWS_QUANT ? h[i] : h[i] * rstd * w[i];
+	if constexpr (MODE == ROWS_NORM)
+		RowVec<DT>::store(a.y, row * a.ldy, col, a.cols, a.vec, y);
+	else {
+		float inv = row_inv;
+		if (a.group) {
+			unsigned m = 0;
+#pragma unroll
+			for (int i = 0; i < N; i++) {
+				const unsigned b = abs_bits(y[i]);
+				m = b > m ? b : m;
+			}
+			m = lanes_max(m, a.group / N);
+			const float top = __uint_as_float(m);
+			inv = code_factor(top);
+			if (col < a.cols && col % a.group == 0)
+				a.scale[row * a.ngroups + col / a.group] = code_scale(top);
+		}
+		store_codes<N>(a.q, row * a.ldq, col, a.cols, a.vec, y, inv);
+	}
+}
+
+/* Rows of at most T * V vectors, T threads a row, each of which keeps its V vectors in registers. */
+template <int DT, int MODE, int T, int V>
+__global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const rows_args a)
+{
+	constexpr int N = RowVec<DT>::N;
+	constexpr int RPG = T < 256 ? 256 / T : 1;	/* rows a workgroup */
+	const int t = threadIdx.x % T;
+	const long row = (long)blockIdx.x * RPG + threadIdx.x / T;
+	if (RPG > 1 && row >= a.rows)	/* (whole wavefronts: T = 64) */
+		return;
+	float h[V][N], w[V][N];
+#pragma unroll
+	for (int v = 0; v < V; v++)
+		RowVec<DT>::load(a.x, row * a.ldx, (v * T + t) * N, a.cols, a.vec, h[v]);
+	if (a.res) {
+#pragma unroll
+		for (int v = 0; v < V; v++) {
+			float r[N];
+			RowVec<DT>::load(a.res, row * a.ldr, (v * T + t) * N, a.cols, a.vec, r);
+#pragma unroll
+			for (int i = 0; i < N; i++)
+				h[v][i] += r[i];
+		}
+	}
+	if constexpr (MODE != ROWS_QUANT) {
+#pragma unroll
+		for (int v = 0; v < V; v++) {
+			const int col = (v * T + t) * N;
+			if (a.w) {
+				RowVec<THHIP_F32>::load(a.w, 0, col, a.cols, a.vec, w[v]);
+				if constexpr (N == 8)
+					RowVec<THHIP_F32>::load(a.w, 0, col + 4, a.cols, a.vec, w[v] + 4);
+			} else {
+#pragma unroll
+				for (int i = 0; i < N; i++)
+					w[v][i] = 1.0f;
+			}
+		}
+	}
+	float s = 0, rstd = 1, inv = 0;
+	unsigned m = 0;
+#pragma unroll
+	for (int v = 0; v < V; v++) {
+#pragma unroll
+		for (int i = 0; i < N; i++) {
+			if constexpr (MODE != ROWS_QUANT)
+				s += h[v][i] * h[v][i];
+			if constexpr (MODE != ROWS_NORM) {
+				const unsigned b = abs_bits(MODE == ROWS_QUANT ? h[v][i] : h[v][i] * w[v][i]);
+				m = b > m ? b : m;
+			}
+		}
+	}
+	if (MODE != ROWS_QUANT || !a.group)
+		row_reduce<T>(s, m);
+	if constexpr (MODE != ROWS_QUANT)
+		rstd = 1.0f / sqrtf(s / (float)a.cols + a.eps);
+	if constexpr (MODE != ROWS_NORM) {
+		if (!a.group) {
+			const float top = __uint_as_float(m) * rstd;
+			inv = code_factor(top);
+			if (t == 0)
+				a.scale[row] = code_scale(top);
+		}
+	}
+#pragma unroll
+	for (int v = 0; v < V; v++) {
+		const int col = (v * T + t) * N;
+		if (a.sum)
+			RowVec<DT>::store(a.sum, row * a.lds, col, a.cols, a.vec, h[v]);
+		row_out<DT, MODE>(a, row, col, h[v], w[v], rstd, inv);
+	}
+}
+
+/* Rows longer than the registers hold: the sum (and maximum) first, then the row again.  A thread
+ * reads an element of x and res in the second walk before it writes the same element, so the outputs
+ * may be the inputs here too. */
+template <int DT, int MODE>
+__global__ __launch_bounds__(1024) void rows_long_kernel(const rows_args a)
+{
+	constexpr int N = RowVec<DT>::N, T = 1024;
+	const long row = blockIdx.x;
+	const int t = threadIdx.x;
+	const int steps = (a.cols - 1) / (T * N) + 1;
+	float h[N], w[N], r[N], s = 0, rstd = 1, inv = 0;
+	unsigned m = 0;
+	for (int walk = 0; walk < 2; walk++) {
+		for (int v = 0; v < steps; v++) {
+			const int col = (v * T + t) * N;
+			RowVec<DT>::load(a.x, row * a.ldx, col, a.cols, a.vec, h);
+			if (a.res) {
+				RowVec<DT>::load(a.res, row * a.ldr, col, a.cols, a.vec, r);
+#pragma unroll
+				for (int i = 0; i < N; i++)
+					h[i] += r[i];
+			}
+#pragma unroll
+			for (int i = 0; i < N; i++)
+				w[i] = MODE != ROWS_QUANT && a.w && col + i < a.cols ? a.w[col + i] : 1.0f;
+			if (walk == 0) {
+#pragma unroll
+				for (int i = 0; i < N; i++) {
+					s += h[i] * h[i];
+					const unsigned b = abs_bits(h[i] * w[i]);
+					m = b > m ? b : m;
+				}
+			} else {
+				if (a.sum)
+					RowVec<DT>::store(a.sum, row * a.lds, col, a.cols, a.vec, h);
+				row_out<DT, MODE>(a, row, col, h, w, rstd, inv);
+			}
+		}
+		if (walk == 0) {
+			row_reduce<T>(s, m);
+			if constexpr (MODE != ROWS_QUANT)
+				rstd = 1.0f / sqrtf(s / (float)a.cols + a.eps);
+			if constexpr (MODE != ROWS_NORM) {
+				if (!a.group) {
+					const float top = __uint_as_float(m) * rstd;
+					inv = code_factor(top);
+					if (t == 0)
+						a.scale[row] = code_scale(top);
+				}
+			}
+		}
+	}
+}
+
+template <int DT, int MODE, int T, int V>
+static bool rows_try(const rows_args &a)
+{
+	if (a.cols > T * V * RowVec<DT>::N)
+		return false;
+	constexpr int RPG = T < 256 ? 256 / T : 1;
+	rows_kernel<DT, MODE, T, V><<<dim3((unsigned)((a.rows + RPG - 1) / RPG)), dim3(T < 256 ? 256 : T), 0, thhip_stream()>>>(a);
+	return true;
+}
+
+template <int DT, int MODE>
+static void rows_launch(const rows_args &a)
+{
+	if (rows_try<DT, MODE, 64, 1>(a) || rows_try<DT, MODE, 64, 2>(a) || rows_try<DT, MODE, 256, 1>(a) ||
+	    rows_try<DT, MODE, 256, 2>(a) || rows_try<DT, MODE, 256, 4>(a) || rows_try<DT, MODE, 256, 8>(a) ||
+	    rows_try<DT, MODE, 1024, 4>(a))
+		return;
+	rows_long_kernel<DT, MODE><<<dim3((unsigned)a.rows), dim3(1024), 0, thhip_stream()>>>(a);
+}
+
+/* A launch has fewer than 2^32 threads: rows beyond this many go into further launches */
+#define ROWS_A_LAUNCH (1l << 21)
+
+static bool aligned(const void *p, long ld, size_t esize, size_t to)
+{
+	return !p || ((uintptr_t)p % to == 0 && (size_t)ld * esize % to == 0);
+}
+
+/* What is wrong with a call, or NULL; fills in what the kernels derive from the arguments */
+static const char *rows_check(rows_args &a, long rows, long cols, int dtype, int mode)
+{
+	if (dtype != THHIP_F32 && dtype != THHIP_F16 && dtype != THHIP_BF16)
+		return "the type of x is fp32, fp16 or bf16";
+	if (rows < 0 || cols < 1 || cols > 0x3fffffffl)
+		return "rows of 1 to 2^30 - 1 columns";
+	const size_t es = thhip_esize(dtype);
+	if (rows && (!a.x || (mode == ROWS_NORM ? !a.y : !a.q || !a.scale)))
+		return "x and the outputs are needed";
+	if (a.ldx < cols || (a.res && a.ldr < cols) || (a.sum && a.lds < cols) || (a.y && a.ldy < cols) || (a.q && a.ldq < cols))
+		return "a row stride is smaller than the row";
+	if ((uintptr_t)a.x % es || (uintptr_t)a.res % es || (uintptr_t)a.sum % es || (uintptr_t)a.y % es ||
+	    (uintptr_t)a.w % 4 || (uintptr_t)a.scale % 4)
+		return "a pointer is not aligned to its element";
+	if (mode != ROWS_NORM && a.group != 0 && a.group != 32 && a.group != 64 && a.group != 128 && a.group != 256)
+		return "a group has 32, 64, 128 or 256 columns, or is the row (0)";
+	a.rows = rows;
+	a.cols = (int)cols;
+	a.ngroups = a.group ? (int)((cols + a.group - 1) / a.group) : 1;
+	a.vec = aligned(a.x, a.ldx, es, 16) && aligned(a.res, a.ldr, es, 16) && aligned(a.sum, a.lds, es, 16) &&
+		aligned(a.y, a.ldy, es, 16) && aligned(a.w, 0, 4, 16) && aligned(a.q, a.ldq, 1, es == 4 ? 4 : 8);
+	return 0;
+}
+
+static double rows_bytes(const rows_args &a, int dtype)
+{
+	const double n = (double)a.rows * a.cols, es = thhip_esize(dtype);
+	return n * es * (1 + !!a.res + !!a.sum + !!a.y) + (a.w ? 4.0 * a.cols : 0) +
+		(a.q ? n + 4.0 * a.rows * a.ngroups : 0);
+}
+
+static int rows_run(const char *who, rows_args &a, long rows, long cols, int dtype, int mode)
+{
+	const char *bad = rows_check(a, rows, cols, dtype, mode);
+	if (bad) {
+		fprintf(stderr, "%s: %ld x %ld, dtype %d, group %d: %s\n", who, rows, cols, dtype, a.group, bad);
+		return -1;
+	}
+	if (!rows)
+		return 0;
+	ThhipLaunchScope scope(THHIP_FAM_OTHER, rows_bytes(a, dtype));
+	const size_t es = thhip_esize(dtype);
+	while (rows > 0) {
+		a.rows = rows < ROWS_A_LAUNCH ? rows : ROWS_A_LAUNCH;
+		if (mode == ROWS_NORM)
+			THHIP_DISPATCH_FLOAT(dtype, (rows_launch<DT, ROWS_NORM>(a)));
+		else if (mode == ROWS_NORM_I8)
+			THHIP_DISPATCH_FLOAT(dtype, (rows_launch<DT, ROWS_NORM_I8>(a)));
+		else
+			THHIP_DISPATCH_FLOAT(dtype, (rows_launch<DT, ROWS_QUANT>(a)));
+		rows -= a.rows;
+		a.x = (const char *)a.x + a.rows * a.ldx * es;
+		a.res = a.res ? (const char *)a.res + a.rows * a.ldr * es : 0;
+		a.sum = a.sum ? (char *)a.sum + a.rows * a.lds * es : 0;
+		a.y = a.y ? (char *)a.y + a.rows * a.ldy * es : 0;
+		a.q = a.q ? a.q + a.rows * a.ldq : 0;
+		a.scale = a.scale ? a.scale + a.rows * a.ngroups : 0;
+	}
+	return 0;
+}
+
+extern "C" int thhip_rmsnorm(const void *x, long ldx, const void *res, long ldr, const float *weight, float eps,
+	void *sum, long lds, void *y, long ldy, long rows, long cols, int dtype)
+{
+	rows_args a = {};
+	a.x = x; a.ldx = ldx; a.res = res; a.ldr = ldr; a.w = weight; a.eps = eps;
+	a.sum = sum; a.lds = lds; a.y = y; a.ldy = ldy;
+	return rows_run("thhip_rmsnorm", a, rows, cols, dtype, ROWS_NORM);
+}
+
+extern "C" int thhip_rmsnorm_i8(const void *x, long ldx, const void *res, long ldr, const float *weight, float eps,
+	void *sum, long lds, signed char *q, long ldq, float *qscale, int group, long rows, long cols, int dtype)
+{
+	rows_args a = {};
+	a.x = x; a.ldx = ldx; a.res = res; a.ldr = ldr; a.w = weight; a.eps = eps;
+	a.sum = sum; a.lds = lds; a.q = q; a.ldq = ldq; a.scale = qscale; a.group = group;
+	return rows_run("thhip_rmsnorm_i8", a, rows, cols, dtype, ROWS_NORM_I8);
+}
+
+extern "C" int thhip_quantize_rows(const void *x, long ldx, signed char *q, long ldq, float *qscale, int group,
+	long rows, long cols, int dtype)
+{
+	rows_args a = {};
+	a.x = x; a.ldx = ldx; a.q = q; a.ldq = ldq; a.scale = qscale; a.group = group;
+	return rows_run("thhip_quantize_rows", a, rows, cols, dtype, ROWS_QUANT);
+}
+
+/* y = q * scale.  TX threads (a power of two) walk a row eight columns at a time; a group is a whole
+ * number of such vectors. */
+template <int DT>
+__global__ __launch_bounds__(256) void dequantize_rows_kernel(const signed char *q, long ldq, const float *scale, int group,
+	int ngroups, void *y, long ldy, long rows, int cols, int tx, int vec)
+{
+	const long row = (long)blockIdx.x * (256 / tx) + threadIdx.x / tx;
+	if (row >= rows)
+		return;
+	for (int col = (threadIdx.x & (tx - 1)) * 8; col < cols; col += tx * 8) {
+		const float s = scale[row * ngroups + (group ? col / group : 0)];
+		float v[8];
+		if (vec && col + 8 <= cols) {
+			const uintx2 w = *(const uintx2 *)(q + row * ldq + col);
+#pragma unroll
+			for (int i = 0; i < 8; i++)
+				v[i] = (float)(signed char)(w[i / 4] >> (8 * (i % 4)));
+		} else {
+#pragma unroll
+			for (int i = 0; i < 8; i++)
+				v[i] = col + i < cols ? (float)q[row * ldq + col + i] : 0.0f;
+		}
+#pragma unroll
+		for (int i = 0; i < 8; i++)
+			v[i] *= s;
+#pragma unroll
+		for (int i = 0; i < 8; i += RowVec<DT>::N)
+			RowVec<DT>::store(y, row * ldy, col + i, cols, vec, v + i);
+	}
+}
+
+extern "C" int thhip_dequantize_rows(const signed char *q, long ldq, const float *qscale, int group, void *y, long ldy,
+	long rows, long cols, int dtype)
+{
+	rows_args a = {};
+	a.x = y; a.ldx = ldy; a.q = (signed char *)q; a.ldq = ldq; a.scale = (float *)qscale; a.group = group;
+	const char *bad = rows_check(a, rows, cols, dtype, ROWS_QUANT);
+	if (bad) {
+		fprintf(stderr, "thhip_dequantize_rows: %ld x %ld, dtype %d, group %d: %s\n", rows, cols, dtype, group, bad);
+		return -1;
+	}
+	if (!rows)
+		return 0;
+	const int vec = aligned(y, ldy, thhip_esize(dtype), 16) && aligned(q, ldq, 1, 8);
+	int tx = 1;
+	while (tx < 256 && tx * 8 < cols)
+		tx *= 2;
+	ThhipLaunchScope scope(THHIP_FAM_OTHER, (double)rows * cols * (1 + thhip_esize(dtype)) + 4.0 * rows * a.ngroups);
+	for (long r = 0; r < rows; r += ROWS_A_LAUNCH) {
+		const long n = rows - r < ROWS_A_LAUNCH ? rows - r : ROWS_A_LAUNCH;
+		const unsigned grid = (unsigned)((n + 256 / tx - 1) / (256 / tx));
+		THHIP_DISPATCH_FLOAT(dtype, (dequantize_rows_kernel<DT><<<dim3(grid), dim3(256), 0, thhip_stream()>>>(q + r * ldq, ldq,
+			qscale + r * a.ngroups, group, a.ngroups, (char *)y + r * ldy * thhip_esize(dtype), ldy, n, (int)cols, tx, vec)));
+	}
+	return 0;
+}
