@@ -711,7 +711,7 @@ void thhip_rgb2float_batch(void *dst, const unsigned char *src, int n, long src_
  * use no scratch memory, and return 0, or -1 with a message on stderr and nothing launched for arguments they
  * refuse; no rows (B = 0, rows = 0) is 0 and no launch.  `dtype` is THHIP_F32, THHIP_F16 or THHIP_BF16.  Sums,
  * norms and scales of x are fp32.  Row strides (ld*) are in elements; any stride that holds a row and any
- * pointer aligned to its element is taken, 16-byte vectors are used where both allow it.
+ * pointer aligned to its element is taken.
  *
  * Weights with 4 bits: a code n of 0 .. 15 a weight, row-major [nOut][(nIn + 1) / 2] bytes, even k in the low
  * half of a byte; `group` consecutive weights of a row (32, 64, 128 or 256; 0: the whole row) share a scale and a
@@ -751,8 +751,8 @@ int thhip_linear_w4_i8(const signed char *q, long ldq, const float *xscale, int 
  * may be x or res, with the same stride, but not one the other's; nothing else may overlap. */
 int thhip_rmsnorm(const void *x, long ldx, const void *res, long ldr, const float *weight, float eps,
 	void *sum, long lds, void *y, long ldy, long rows, long cols, int dtype);
-/* The same with y as signed 8-bit codes: qscale = max|y| / 127 and q = rint(127 * y / max|y|) over groups of 32, 64,
- * 128 or 256 columns or the whole row (group 0); qscale fp32 [rows][ceil(cols / group)].  Where max|y| is under
+/* The same with y as signed 8-bit codes: qscale = max|y| / 127 and q = rint(y / qscale) over groups of 32, 64, 128 or
+ * 256 columns or the whole row (group 0); qscale fp32 [rows][ceil(cols / group)].  Where max|y| is under
  * 2^-116 scale and codes are 0; a NaN or infinity makes its group's scale NaN or infinite, and its codes mean nothing. */
 int thhip_rmsnorm_i8(const void *x, long ldx, const void *res, long ldr, const float *weight, float eps,
 	void *sum, long lds, signed char *q, long ldq, float *qscale, int group, long rows, long cols, int dtype);

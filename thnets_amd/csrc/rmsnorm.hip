@@ -4,7 +4,7 @@
  *
  *   h = x + res                       (fp32; sum = h rounded to the type of x)
  *   y = h * w / sqrt(mean(h * h) + eps)
- *   scale = max|y| / 127,  q = rint(127 y / max|y|)     over a row or a group
+ *   scale = max|y| / 127,  q = rint(y / scale)          over a row or a group
  *
  * The reference has neither (its norm is nn_SpatialBatchNormalization_updateOutput,
  * modules/SpatialBatchNormalization.c:57-116, its 8-bit codes are unsigned with one
@@ -14,7 +14,10 @@
  * Bound by memory: every element is read once, kept in registers while the row's
  * sum of squares (and largest |h w|) goes through the wavefronts, and written once.
  * h stays in fp32 between the addition and the norm, so the norm is that of the
- * unrounded sum, and y is rounded once.
+ * unrounded sum, and y is rounded once.  Codes do not depend on the root, only on
+ * h w and its maximum; their quotient is taken in 64 bits (full rate here, and the
+ * kernels wait for memory), so that a value next to the middle between two codes goes
+ * to the nearer one: with fp32 quotients one value in 30000 of fp16 rows did not.
  */
 #include <stdint.h>
 #include <stdio.h>
@@ -30,20 +33,21 @@ struct rows_args {
 	float *scale;
 	long ldx, ldr, lds, ldy, ldq;
 	long rows;
-	int cols, group, ngroups, vec;
+	int cols, group, ngroups;
 	float eps;
 };
 
-/* N consecutive elements of a row (16 bytes): a vector load / store where pointers and strides allow it
- * and the elements are all inside the row, one by one otherwise; elements past the row read as 0 */
+/* N consecutive elements of a row (16 bytes): one load / store, which needs no more than the element's
+ * alignment here, or one by one where the row ends among them; elements past the row read as 0 */
 template <int DT> struct RowVec {
 	static constexpr int N = DT == THHIP_F32 ? 4 : 8;
 	typedef typename ThhipElem<DT>::T T;
 	typedef T V __attribute__((ext_vector_type(N)));
-	static __device__ __forceinline__ void load(const void *p, long base, int col, int cols, int vec, float *out)
+	typedef V U __attribute__((aligned(sizeof(T))));
+	static __device__ __forceinline__ void load(const void *p, long base, int col, int cols, float *out)
 	{
-		if (vec && col + N <= cols) {
-			const V v = *(const V *)((const T *)p + base + col);
+		if (col + N <= cols) {
+			const V v = *(const U *)((const T *)p + base + col);
 #pragma unroll
 			for (int i = 0; i < N; i++)
 				out[i] = (float)v[i];
@@ -53,14 +57,14 @@ template <int DT> struct RowVec {
 				out[i] = col + i < cols ? ThhipElem<DT>::ld(p, base + col + i) : 0.0f;
 		}
 	}
-	static __device__ __forceinline__ void store(void *p, long base, int col, int cols, int vec, const float *in)
+	static __device__ __forceinline__ void store(void *p, long base, int col, int cols, const float *in)
 	{
-		if (vec && col + N <= cols) {
+		if (col + N <= cols) {
 			V v;
 #pragma unroll
 			for (int i = 0; i < N; i++)
 				v[i] = (T)in[i];
-			*(V *)((T *)p + base + col) = v;
+			*(U *)((T *)p + base + col) = v;
 		} else {
 #pragma unroll
 			for (int i = 0; i < N; i++)
@@ -70,22 +74,44 @@ template <int DT> struct RowVec {
 	}
 };
 
-template <int N>
-__device__ __forceinline__ void store_codes(signed char *p, long base, int col, int cols, int vec, const float *y, float inv)
+/* What a row's or group's values become codes by: step = top / 127 and its reciprocal.  top is the largest
+ * |h w|, top * rstd the largest |y|: below 2^-116 (where an fp32 scale loses bits) it counts as nothing,
+ * reciprocal 0, codes 0. */
+struct code_step {
+	double step, inv;
+};
+
+__device__ __forceinline__ struct code_step code_step_of(float top, float rstd)
 {
+	struct code_step c;
+	c.step = (double)top / 127.0;
+	c.inv = top * rstd < 1.2e-35f ? 0.0 : 1.0 / c.step;	/* (a NaN stays one) */
+	return c;
+}
+
+template <int N>
+__device__ __forceinline__ void store_codes(signed char *p, long base, int col, int cols, const double *v, const struct code_step c)
+{
+	typedef unsigned W __attribute__((ext_vector_type(N / 4), aligned(1)));
 	unsigned w[N / 4];
 #pragma unroll
 	for (int i = 0; i < N / 4; i++)
 		w[i] = 0;
 #pragma unroll
 	for (int i = 0; i < N; i++) {
-		const float t = fminf(fmaxf(rintf(y[i] * inv), -127.0f), 127.0f);
-		w[i / 4] |= ((unsigned)(int)t & 255u) << (8 * (i % 4));
+		/* v / step, rounded once: the quotient's own error, times the reciprocal, put right */
+		double t = v[i] * c.inv;
+		t = fma(fma(-t, c.step, v[i]), c.inv, t);
+		const int n = (int)rint(t), q = n > 127 ? 127 : n < -127 ? -127 : n;	/* (NaN: 0) */
+		w[i / 4] |= ((unsigned)q & 255u) << (8 * (i % 4));
 	}
-	if (vec && col + N <= cols) {
-#pragma unroll
-		for (int i = 0; i < N / 4; i++)
-			((unsigned *)(p + base + col))[i] = w[i];
+	if (col + N <= cols) {
+		W o;
+		if constexpr (N == 8)
+			o = (W){w[0], w[1]};
+		else
+			o = (W)w[0];
+		*(W *)(p + base + col) = o;
 	} else {
 #pragma unroll
 		for (int i = 0; i < N; i++)
@@ -99,13 +125,6 @@ __device__ __forceinline__ void store_codes(signed char *p, long base, int col, 
 __device__ __forceinline__ unsigned abs_bits(float v)
 {
 	return __float_as_uint(v) & 0x7fffffffu;
-}
-
-/* What a value is multiplied with to give its code: 127 / top.  A top below 2^-116 (whose
- * reciprocal would overflow) counts as nothing: scale 0, codes 0. */
-__device__ __forceinline__ float code_factor(float top)
-{
-	return top < 1.2e-35f ? 0.0f : 127.0f / top;	/* (a NaN stays one) */
 }
 
 __device__ __forceinline__ float code_scale(float top)
@@ -158,31 +177,34 @@ __device__ __forceinline__ void row_reduce(float &s, unsigned &m)
 /* One vector of a row on its way out: y, or codes and (by the group's first lane) its scale */
 template <int DT, int MODE>
 __device__ __forceinline__ void row_out(const rows_args &a, long row, int col, const float *h, const float *w, float rstd,
-	float row_inv)
+	struct code_step step)
 {
 	constexpr int N = RowVec<DT>::N;
-	float y[N];
+	if constexpr (MODE == ROWS_NORM) {
+		float y[N];
 #pragma unroll
-	for (int i = 0; i < N; i++)
-		y[i] = MODE == ROWS_QUANT ? h[i] : h[i] * rstd * w[i];
-	if constexpr (MODE == ROWS_NORM)
-		RowVec<DT>::store(a.y, row * a.ldy, col, a.cols, a.vec, y);
-	else {
-		float inv = row_inv;
+		for (int i = 0; i < N; i++)
+			y[i] = h[i] * rstd * w[i];
+		RowVec<DT>::store(a.y, row * a.ldy, col, a.cols, y);
+	} else {
+		double v[N];
+#pragma unroll
+		for (int i = 0; i < N; i++)
+			v[i] = MODE == ROWS_QUANT ? (double)h[i] : (double)h[i] * (double)w[i];
 		if (a.group) {
 			unsigned m = 0;
 #pragma unroll
 			for (int i = 0; i < N; i++) {
-				const unsigned b = abs_bits(y[i]);
+				const unsigned b = abs_bits((float)v[i]);
 				m = b > m ? b : m;
 			}
 			m = lanes_max(m, a.group / N);
 			const float top = __uint_as_float(m);
-			inv = code_factor(top);
+			step = code_step_of(top, rstd);
 			if (col < a.cols && col % a.group == 0)
-				a.scale[row * a.ngroups + col / a.group] = code_scale(top);
+				a.scale[row * a.ngroups + col / a.group] = code_scale(top * rstd);
 		}
-		store_codes<N>(a.q, row * a.ldq, col, a.cols, a.vec, y, inv);
+		store_codes<N>(a.q, row * a.ldq, col, a.cols, v, step);
 	}
 }
 
@@ -199,12 +221,12 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const rows_args
 	float h[V][N], w[V][N];
 #pragma unroll
 	for (int v = 0; v < V; v++)
-		RowVec<DT>::load(a.x, row * a.ldx, (v * T + t) * N, a.cols, a.vec, h[v]);
+		RowVec<DT>::load(a.x, row * a.ldx, (v * T + t) * N, a.cols, h[v]);
 	if (a.res) {
 #pragma unroll
 		for (int v = 0; v < V; v++) {
 			float r[N];
-			RowVec<DT>::load(a.res, row * a.ldr, (v * T + t) * N, a.cols, a.vec, r);
+			RowVec<DT>::load(a.res, row * a.ldr, (v * T + t) * N, a.cols, r);
 #pragma unroll
 			for (int i = 0; i < N; i++)
 				h[v][i] += r[i];
@@ -215,9 +237,9 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const rows_args
 		for (int v = 0; v < V; v++) {
 			const int col = (v * T + t) * N;
 			if (a.w) {
-				RowVec<THHIP_F32>::load(a.w, 0, col, a.cols, a.vec, w[v]);
+				RowVec<THHIP_F32>::load(a.w, 0, col, a.cols, w[v]);
 				if constexpr (N == 8)
-					RowVec<THHIP_F32>::load(a.w, 0, col + 4, a.cols, a.vec, w[v] + 4);
+					RowVec<THHIP_F32>::load(a.w, 0, col + 4, a.cols, w[v] + 4);
 			} else {
 #pragma unroll
 				for (int i = 0; i < N; i++)
@@ -225,7 +247,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const rows_args
 			}
 		}
 	}
-	float s = 0, rstd = 1, inv = 0;
+	float s = 0, rstd = 1;
+	struct code_step step = {0, 0};
 	unsigned m = 0;
 #pragma unroll
 	for (int v = 0; v < V; v++) {
@@ -245,18 +268,17 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const rows_args
 		rstd = 1.0f / sqrtf(s / (float)a.cols + a.eps);
 	if constexpr (MODE != ROWS_NORM) {
 		if (!a.group) {
-			const float top = __uint_as_float(m) * rstd;
-			inv = code_factor(top);
+			step = code_step_of(__uint_as_float(m), rstd);
 			if (t == 0)
-				a.scale[row] = code_scale(top);
+				a.scale[row] = code_scale(__uint_as_float(m) * rstd);
 		}
 	}
 #pragma unroll
 	for (int v = 0; v < V; v++) {
 		const int col = (v * T + t) * N;
 		if (a.sum)
-			RowVec<DT>::store(a.sum, row * a.lds, col, a.cols, a.vec, h[v]);
-		row_out<DT, MODE>(a, row, col, h[v], w[v], rstd, inv);
+			RowVec<DT>::store(a.sum, row * a.lds, col, a.cols, h[v]);
+		row_out<DT, MODE>(a, row, col, h[v], w[v], rstd, step);
 	}
 }
 
@@ -270,14 +292,15 @@ __global__ __launch_bounds__(1024) void rows_long_kernel(const rows_args a)
 	const long row = blockIdx.x;
 	const int t = threadIdx.x;
 	const int steps = (a.cols - 1) / (T * N) + 1;
-	float h[N], w[N], r[N], s = 0, rstd = 1, inv = 0;
+	float h[N], w[N], r[N], s = 0, rstd = 1;
+	struct code_step step = {0, 0};
 	unsigned m = 0;
 	for (int walk = 0; walk < 2; walk++) {
 		for (int v = 0; v < steps; v++) {
 			const int col = (v * T + t) * N;
-			RowVec<DT>::load(a.x, row * a.ldx, col, a.cols, a.vec, h);
+			RowVec<DT>::load(a.x, row * a.ldx, col, a.cols, h);
 			if (a.res) {
-				RowVec<DT>::load(a.res, row * a.ldr, col, a.cols, a.vec, r);
+				RowVec<DT>::load(a.res, row * a.ldr, col, a.cols, r);
 #pragma unroll
 				for (int i = 0; i < N; i++)
 					h[i] += r[i];
@@ -294,8 +317,8 @@ __global__ __launch_bounds__(1024) void rows_long_kernel(const rows_args a)
 				}
 			} else {
 				if (a.sum)
-					RowVec<DT>::store(a.sum, row * a.lds, col, a.cols, a.vec, h);
-				row_out<DT, MODE>(a, row, col, h, w, rstd, inv);
+					RowVec<DT>::store(a.sum, row * a.lds, col, a.cols, h);
+				row_out<DT, MODE>(a, row, col, h, w, rstd, step);
 			}
 		}
 		if (walk == 0) {
@@ -304,10 +327,9 @@ __global__ __launch_bounds__(1024) void rows_long_kernel(const rows_args a)
 				rstd = 1.0f / sqrtf(s / (float)a.cols + a.eps);
 			if constexpr (MODE != ROWS_NORM) {
 				if (!a.group) {
-					const float top = __uint_as_float(m) * rstd;
-					inv = code_factor(top);
+					step = code_step_of(__uint_as_float(m), rstd);
 					if (t == 0)
-						a.scale[row] = code_scale(top);
+						a.scale[row] = code_scale(__uint_as_float(m) * rstd);
 				}
 			}
 		}
@@ -337,11 +359,6 @@ static void rows_launch(const rows_args &a)
 /* A launch has fewer than 2^32 threads: rows beyond this many go into further launches */
 #define ROWS_A_LAUNCH (1l << 21)
 
-static bool aligned(const void *p, long ld, size_t esize, size_t to)
-{
-	return !p || ((uintptr_t)p % to == 0 && (size_t)ld * esize % to == 0);
-}
-
 /* What is wrong with a call, or NULL; fills in what the kernels derive from the arguments */
 static const char *rows_check(rows_args &a, long rows, long cols, int dtype, int mode)
 {
@@ -362,8 +379,6 @@ static const char *rows_check(rows_args &a, long rows, long cols, int dtype, int
 	a.rows = rows;
 	a.cols = (int)cols;
 	a.ngroups = a.group ? (int)((cols + a.group - 1) / a.group) : 1;
-	a.vec = aligned(a.x, a.ldx, es, 16) && aligned(a.res, a.ldr, es, 16) && aligned(a.sum, a.lds, es, 16) &&
-		aligned(a.y, a.ldy, es, 16) && aligned(a.w, 0, 4, 16) && aligned(a.q, a.ldq, 1, es == 4 ? 4 : 8);
 	return 0;
 }
 
@@ -434,16 +449,17 @@ extern "C" int thhip_quantize_rows(const void *x, long ldx, signed char *q, long
  * number of such vectors. */
 template <int DT>
 __global__ __launch_bounds__(256) void dequantize_rows_kernel(const signed char *q, long ldq, const float *scale, int group,
-	int ngroups, void *y, long ldy, long rows, int cols, int tx, int vec)
+	int ngroups, void *y, long ldy, long rows, int cols, int tx)
 {
+	typedef unsigned W __attribute__((ext_vector_type(2), aligned(1)));
 	const long row = (long)blockIdx.x * (256 / tx) + threadIdx.x / tx;
 	if (row >= rows)
 		return;
 	for (int col = (threadIdx.x & (tx - 1)) * 8; col < cols; col += tx * 8) {
 		const float s = scale[row * ngroups + (group ? col / group : 0)];
 		float v[8];
-		if (vec && col + 8 <= cols) {
-			const uintx2 w = *(const uintx2 *)(q + row * ldq + col);
+		if (col + 8 <= cols) {
+			const W w = *(const W *)(q + row * ldq + col);
 #pragma unroll
 			for (int i = 0; i < 8; i++)
 				v[i] = (float)(signed char)(w[i / 4] >> (8 * (i % 4)));
@@ -457,7 +473,7 @@ __global__ __launch_bounds__(256) void dequantize_rows_kernel(const signed char 
 			v[i] *= s;
 #pragma unroll
 		for (int i = 0; i < 8; i += RowVec<DT>::N)
-			RowVec<DT>::store(y, row * ldy, col + i, cols, vec, v + i);
+			RowVec<DT>::store(y, row * ldy, col + i, cols, v + i);
 	}
 }
 
@@ -473,7 +489,6 @@ extern "C" int thhip_dequantize_rows(const signed char *q, long ldq, const float
 	}
 	if (!rows)
 		return 0;
-	const int vec = aligned(y, ldy, thhip_esize(dtype), 16) && aligned(q, ldq, 1, 8);
 	int tx = 1;
 	while (tx < 256 && tx * 8 < cols)
 		tx *= 2;
@@ -482,7 +497,7 @@ extern "C" int thhip_dequantize_rows(const signed char *q, long ldq, const float
 		const long n = rows - r < ROWS_A_LAUNCH ? rows - r : ROWS_A_LAUNCH;
 		const unsigned grid = (unsigned)((n + 256 / tx - 1) / (256 / tx));
 		THHIP_DISPATCH_FLOAT(dtype, (dequantize_rows_kernel<DT><<<dim3(grid), dim3(256), 0, thhip_stream()>>>(q + r * ldq, ldq,
-			qscale + r * a.ngroups, group, a.ngroups, (char *)y + r * ldy * thhip_esize(dtype), ldy, n, (int)cols, tx, vec)));
+			qscale + r * a.ngroups, group, a.ngroups, (char *)y + r * ldy * thhip_esize(dtype), ldy, n, (int)cols, tx)));
 	}
 	return 0;
 }
