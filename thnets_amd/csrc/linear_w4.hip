@@ -220,10 +220,23 @@ struct w4_args {
 	long ldx, ldy;
 	int B, nIn, nOut, steps, blocks, groups, group;
 	int xgroups;		/* scales of a row of 8-bit x: 1, or one a group */
-	int xvec;		/* rows of x may be loaded eight elements at a time */
 	int act;
 	float thr, val;
+	int shift;		/* log2(group), 31 where the row is one group */
+	/* the group that matrix instruction j of a packed step belongs to (the last one past K's end) */
+	__host__ __device__ int group_of(int step, int j) const
+	{
+		const int g = (int)(((long)step * W4_KSTEP + 32 * j) >> shift);
+		return g < groups ? g : groups - 1;
+	}
 };
+
+static int g_w4_tuning;
+
+extern "C" void thhip_w4_set_tuning(int kernel)
+{
+	g_w4_tuning = kernel;
+}
 
 /* What differs with the kind of x: the matrix core's operand of eight k, its accumulator, and how a
  * word of eight codes and eight elements of x become operands.  PARTS: operands an x vector makes. */
@@ -328,32 +341,117 @@ template <> struct W4X<W4_X_I8> {
 	}
 };
 
-/* Scales (or zeros) of the four rows a lane's accumulators belong to, as fp32 */
-template <int DT>
-__device__ __forceinline__ floatx4 w4_scales(const void *p, long i)
+/* ---- up to 64 columns: bound by reading the weights once ----
+ *
+ * A workgroup of W wavefronts computes RB blocks of 16 rows for all columns and all of K.  K is walked in
+ * chunks of W steps, wavefront w multiplying step w of every chunk, so that the workgroup reads W KiB of
+ * contiguous codes of a row block at a time.  Codes, scales and zeros go straight to registers, D chunks
+ * ahead; x goes through LDS, where all wavefronts of the workgroup put a chunk of it down together, one
+ * chunk ahead (two buffers, one barrier a chunk): taken to pieces there once, fp32 x is 3 B columns of
+ * bf16 from then on, and the matrix core sees columns only.  Columns past the last read a piece of zeros.
+ * A column's chunk is followed by 16 bytes, which puts the 16 columns of an operand on different banks.
+ * Of a 16 x 16 tile a lane holds rows 4 (lane / 16) + 0 .. 3 of column lane % 16.  The wavefronts' sums are
+ * added through LDS, in their order, and an fp32 row's three columns with them.
+ * GM: matrix instructions a group spans within a step (1: groups of 32 or 64, 4: larger). */
+
+/* Eight elements of a row of x from k on; zeros past the row's end */
+template <int X>
+__device__ __forceinline__ void w4_load_x(const void *x, long at, long k, int nIn, typename W4X<X>::E *e)
 {
-	typedef typename ThhipElem<DT>::T T4 __attribute__((ext_vector_type(4)));
-	const T4 v = *(const T4 *)((const typename ThhipElem<DT>::T *)p + i);
-	floatx4 f;
+	typedef typename W4X<X>::E E;
+	typedef E E8 __attribute__((ext_vector_type(8)));
+	typedef E8 U __attribute__((aligned(sizeof(E))));
+	const E *p = (const E *)x + at + k;
+	if (k + 8 <= nIn) {
+		const E8 v = *(const U *)p;
 #pragma unroll
-	for (int e = 0; e < 4; e++)
-		f[e] = (float)v[e];
-	return f;
+		for (int i = 0; i < 8; i++)
+			e[i] = v[i];
+	} else {
+#pragma unroll
+		for (int i = 0; i < 8; i++)
+			e[i] = k + i < nIn ? p[i] : (E)0;
+	}
 }
 
-/* A workgroup of W wavefronts computes RB blocks of 16 rows for 16 NB batch columns (gridDim.y slices
- * of the batch); wavefront w takes the steps w, w + W, ... of K, and the partial sums are added through
- * LDS in the order of the wavefronts.  Of a 16 x 16 tile a lane holds rows 4 (lane / 16) + 0 .. 3 of column
- * lane % 16.  GM: matrix instructions a group spans within a step (1: groups of 32 or 64, 4: larger). */
-template <int X, int DT, int RB, int NB, int GM, int W>
+/* The workgroup's LDS traffic so far is done, for everybody (loads from memory may still be on their way) */
+__device__ __forceinline__ void w4_lds_barrier(void)
+{
+	asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+/* What a wavefront fetches ahead of a step: the codes of its row blocks and what their groups need */
+template <int DT, int RB, int GM> struct W4Step {
+	typedef typename ThhipElem<DT>::T T4 __attribute__((ext_vector_type(4)));
+	uintx4 codes[RB];
+	T4 s[RB][4 / GM];
+	unsigned z[RB][4 / GM];
+	__device__ __forceinline__ void fetch(const w4_args &a, int rb0, int step, int lane)
+	{
+		if (step >= a.steps)
+			step = a.steps - 1;	/* (loaded, not used) */
+#pragma unroll
+		for (int r = 0; r < RB; r++) {
+			const int rb = rb0 + r < a.blocks ? rb0 + r : a.blocks - 1;
+			codes[r] = *(const uintx4 *)(a.codes + ((size_t)rb * a.steps + step) * 1024 + lane * 16);
+#pragma unroll
+			for (int j = 0; j < 4 / GM; j++) {
+				const size_t at = ((size_t)rb * a.groups + a.group_of(step, j * GM)) * 16 + 4 * (lane >> 4);
+				s[r][j] = *(const T4 *)((const typename ThhipElem<DT>::T *)a.scales + at);
+				if (a.zeros)
+					z[r][j] = *(const unsigned *)(a.zeros + at);
+			}
+		}
+	}
+};
+
+template <int X, int DT, int RB, int NB, int GM, int W, int D>
 __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args a)
 {
 	typedef W4X<X> K;
 	typedef typename K::V V;
 	typedef typename K::A A;
-	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+	constexpr int ES = sizeof(V) / 8;		/* bytes of an operand's element */
+	constexpr int T = W * 64, ROWV = W * 16;	/* threads; vectors of eight in a row's chunk */
+	constexpr int STRIDE = W * W4_KSTEP * ES + 16;
+	constexpr int XV = (4 * NB + K::PARTS - 1) / K::PARTS;	/* vectors a thread puts down a chunk */
+	extern __shared__ __align__(16) unsigned char lds[];
+	const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 	const int col = lane & 15, quarter = lane >> 4;
-	const int rb0 = blockIdx.x * RB, b0 = blockIdx.y * NB * 16;
+	const int rb0 = blockIdx.x * RB;
+	const int cols = a.B * K::PARTS, buf = cols * STRIDE, nvec = a.B * ROWV;
+	const int chunks = (a.steps + W - 1) / W;
+
+	typename K::E xr[XV][8];
+	auto load_x = [&](int c) {
+#pragma unroll
+		for (int i = 0; i < XV; i++) {
+			const int v = tid + i * T;
+			if (v < nvec)
+				w4_load_x<X>(a.x, (v / ROWV) * a.ldx, (long)c * W * W4_KSTEP + v % ROWV * 8, a.nIn, xr[i]);
+		}
+	};
+	auto store_x = [&](int b) {
+#pragma unroll
+		for (int i = 0; i < XV; i++) {
+			const int v = tid + i * T;
+			if (v < nvec) {
+				V o[K::PARTS];
+				K::operand(xr[i], o);
+#pragma unroll
+				for (int p = 0; p < K::PARTS; p++)
+					*(V *)(lds + b * buf + (v / ROWV * K::PARTS + p) * STRIDE + v % ROWV * 8 * ES) = o[p];
+			}
+		}
+	};
+	/* where a lane's operands lie: in either buffer, or among the zeros */
+	int at[2][NB];
+#pragma unroll
+	for (int n = 0; n < NB; n++)
+#pragma unroll
+		for (int b = 0; b < 2; b++)
+			at[b][n] = (n * 16 + col < cols ? b * buf + (n * 16 + col) * STRIDE + wave * W4_KSTEP * ES : 2 * buf) + quarter * 8 * ES;
+
 	floatx4 acc[RB][NB];
 #pragma unroll
 	for (int r = 0; r < RB; r++)
@@ -361,150 +459,150 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args a)
 		for (int n = 0; n < NB; n++)
 			acc[r][n] = (floatx4)0.0f;
 
-	for (int step = wave; step < a.steps; step += W) {
-		uintx4 codes[RB];
+	W4Step<DT, RB, GM> st[D];
+	load_x(0);
 #pragma unroll
-		for (int r = 0; r < RB; r++) {
-			const int rb = rb0 + r < a.blocks ? rb0 + r : a.blocks - 1;
-			codes[r] = *(const uintx4 *)(a.codes + ((size_t)rb * a.steps + step) * 1024 + lane * 16);
-		}
-		const long k0 = (long)step * W4_KSTEP + 8 * quarter;
-		A p[RB][NB], sx[NB];
+	for (int d = 0; d < D; d++)
+		st[d].fetch(a, rb0, d * W + wave, lane);
+	if (tid < 32 * ES)
+		((unsigned *)(lds + 2 * buf))[tid] = 0;
+	store_x(0);
+	if (chunks > 1)
+		load_x(1);
+	w4_lds_barrier();
+
+	constexpr int U = D % 2 ? 2 * D : D;	/* chunks after which buffers and stages are the first again */
+	for (int c0 = 0; c0 < chunks; c0 += U) {
 #pragma unroll
-		for (int j = 0; j < 4; j++) {
-			if (j % GM == 0) {
+		for (int u = 0; u < U; u++) {
+			const int c = c0 + u;
+			if (c >= chunks)
+				break;
+			if (c + 1 < chunks)
+				store_x((u + 1) & 1);
+			if (c + 2 < chunks)
+				load_x(c + 2);
+			const int step = c * W + wave;
+			W4Step<DT, RB, GM> &now = st[u % D];
+			if (step < a.steps) {
+				A p[RB][NB], sx[NB];
 #pragma unroll
-				for (int n = 0; n < NB; n++) {
-					sx[n] = (A)0;
-#pragma unroll
-					for (int r = 0; r < RB; r++)
-						p[r][n] = (A)0;
-				}
-			}
-			V w[RB];
-#pragma unroll
-			for (int r = 0; r < RB; r++)
-				w[r] = K::weights(codes[r][j]);
-#pragma unroll
-			for (int n = 0; n < NB; n++) {
-				const int b = b0 + n * 16 + col;
-				const long k = k0 + 32 * j;
-				typename K::E e[8];
-#pragma unroll
-				for (int i = 0; i < 8; i++)
-					e[i] = (typename K::E)0;
-				if (b < a.B) {
-					const typename K::E *row = (const typename K::E *)a.x + b * a.ldx;
-					if (a.xvec && k + 8 <= a.nIn) {
-						typedef typename K::E E8 __attribute__((ext_vector_type(8)));
-						const E8 v = *(const E8 *)(row + k);
-#pragma unroll
-						for (int i = 0; i < 8; i++)
-							e[i] = v[i];
-					} else {
-#pragma unroll
-						for (int i = 0; i < 8; i++)
-							if (k + i < a.nIn)
-								e[i] = row[k + i];
-					}
-				}
-				V x[K::PARTS];
-				K::operand(e, x);
-#pragma unroll
-				for (int i = 0; i < K::PARTS; i++) {
-					sx[n] = K::mma(K::ones(), x[i], sx[n]);
+				for (int j = 0; j < 4; j++) {
+					V w[RB];
 #pragma unroll
 					for (int r = 0; r < RB; r++)
-						p[r][n] = K::mma(w[r], x[i], p[r][n]);
-				}
-			}
-			if ((j + 1) % GM == 0) {
-				const long kg = (long)step * W4_KSTEP + 32 * j;
-				const int g = a.group ? (int)(kg / a.group) : 0;
-				if (kg >= a.nIn && g >= a.groups)	/* (padding past the last group) */
-					continue;
-#pragma unroll
-				for (int r = 0; r < RB; r++) {
-					const int rb = rb0 + r < a.blocks ? rb0 + r : a.blocks - 1;
-					const long at = ((long)rb * a.groups + g) * 16 + 4 * quarter;
-					floatx4 s = w4_scales<DT>(a.scales, at), z = (floatx4)8.0f;
-					if (a.zeros) {
-						const unsigned zw = *(const unsigned *)(a.zeros + at);
-#pragma unroll
-						for (int i = 0; i < 4; i++)
-							z[i] = (float)((zw >> (8 * i)) & 255);
-					}
+						w[r] = K::weights(now.codes[r][j]);
 #pragma unroll
 					for (int n = 0; n < NB; n++) {
-						const int b = b0 + n * 16 + col;
-						const float xs = X == W4_X_I8 && a.xgroups > 1 ? a.xscale[(long)(b < a.B ? b : a.B - 1) * a.xgroups + g] : 1.0f;
+						const V x = *(const V *)(lds + at[u & 1][n] + j * 32 * ES);
+						if (X != W4_X_I8 || a.zeros)
+							sx[n] = K::mma(K::ones(), x, j % GM ? sx[n] : (A)0);
 #pragma unroll
-						for (int i = 0; i < 4; i++) {
-							if constexpr (X == W4_X_I8)
-								acc[r][n][i] += s[i] * xs * (0.0625f * (float)p[r][n][i] - (z[i] - 8.0f) * (float)sx[n][i]);
-							else
-								acc[r][n][i] += s[i] * (p[r][n][i] - z[i] * sx[n][i]);
+						for (int r = 0; r < RB; r++)
+							p[r][n] = K::mma(w[r], x, j % GM ? p[r][n] : (A)0);
+					}
+					if ((j + 1) % GM)
+						continue;
+#pragma unroll
+					for (int n = 0; n < NB; n++) {
+						float xs = X == W4_X_I8 ? 0.0625f : 1.0f;
+						if (X == W4_X_I8 && a.xgroups > 1) {
+							const int b = n * 16 + col;
+							xs *= a.xscale[(long)(b < a.B ? b : 0) * a.xgroups + a.group_of(step, j)];
 						}
+#pragma unroll
+						for (int r = 0; r < RB; r++)
+#pragma unroll
+							for (int i = 0; i < 4; i++) {
+								const float s = (float)now.s[r][j / GM][i] * xs;
+								const float z = a.zeros ? (float)((now.z[r][j / GM] >> (8 * i)) & 255) : 8.0f;
+								if constexpr (X == W4_X_I8)
+									acc[r][n][i] += s * ((float)p[r][n][i] - (a.zeros ? (16.0f * z - 128.0f) * (float)sx[n][i] : 0.0f));
+								else
+									acc[r][n][i] += s * (p[r][n][i] - z * sx[n][i]);
+							}
 					}
 				}
 			}
+			now.fetch(a, rb0, step + D * W, lane);
+			w4_lds_barrier();
 		}
 	}
 
-	__shared__ floatx4 red[W][RB * NB][64];
+	floatx4 *red = (floatx4 *)lds;	/* [W][RB][NB][64 lanes] */
 #pragma unroll
 	for (int r = 0; r < RB; r++)
 #pragma unroll
 		for (int n = 0; n < NB; n++)
-			red[wave][r * NB + n][lane] = acc[r][n];
+			red[((wave * RB + r) * NB + n) * 64 + lane] = acc[r][n];
 	__syncthreads();
-	for (int t = wave; t < RB * NB; t += W) {
-		floatx4 v = red[0][t][lane];
-#pragma unroll
-		for (int i = 1; i < W; i++)
-			v += red[i][t][lane];
-		const int b = b0 + (t % NB) * 16 + col;
-		if (b >= a.B)
+	for (int t = tid; t < RB * 16 * a.B; t += T) {
+		const int row = t % (RB * 16), b = t / (RB * 16), o = rb0 * 16 + row;
+		if (o >= a.nOut)
 			continue;
-		const float xs = X == W4_X_I8 && a.xgroups == 1 ? a.xscale[b] : 1.0f;
+		float y = 0;
 #pragma unroll
-		for (int i = 0; i < 4; i++) {
-			const int o = (rb0 + t / NB) * 16 + 4 * quarter + i;
-			if (o >= a.nOut)
-				continue;
-			float y = v[i] * xs + (a.bias ? a.bias[o] : 0.0f);
-			if (a.act)
-				y = y > a.thr ? y : a.val;
-			ThhipElem<DT>::st(a.y, b * a.ldy + o, y);
-		}
+		for (int w = 0; w < W; w++)
+#pragma unroll
+			for (int p = 0; p < K::PARTS; p++) {
+				const int c = b * K::PARTS + p;
+				y += ((const float *)&red[((w * RB + row / 16) * NB + c / 16) * 64 + (row % 16 / 4) * 16 + c % 16])[row % 4];
+			}
+		if (X == W4_X_I8 && a.xgroups == 1)
+			y *= a.xscale[b];
+		y += a.bias ? a.bias[o] : 0.0f;
+		if (a.act)
+			y = y > a.thr ? y : a.val;
+		ThhipElem<DT>::st(a.y, b * a.ldy + o, y);
 	}
 }
 
-/* A grid has at most 65535 slices of the batch: larger batches go into further launches */
-#define W4_SLICES 65535
-
-template <int X, int DT, int RB, int NB, int GM>
-static void w4_skinny_launch(w4_args a)
+/* The batch as seen from row b0 on, n rows */
+static w4_args w4_rows(w4_args a, int b0, int n, size_t esx, size_t esy)
 {
-	constexpr int W = 8;
-	const long esx = X == W4_X_I8 ? 1 : thhip_esize(X), esy = thhip_esize(DT);
-	for (long left = a.B; left > 0; left -= (long)W4_SLICES * NB * 16) {
-		a.B = (int)(left < (long)W4_SLICES * NB * 16 ? left : (long)W4_SLICES * NB * 16);
-		w4_skinny_kernel<X, DT, RB, NB, GM, W><<<dim3((a.blocks + RB - 1) / RB, (a.B + NB * 16 - 1) / (NB * 16)), dim3(W * 64), 0,
-			thhip_stream()>>>(a);
-		a.x = (const char *)a.x + a.B * a.ldx * esx;
-		a.y = (char *)a.y + a.B * a.ldy * esy;
-		a.xscale = a.xscale ? a.xscale + (long)a.B * a.xgroups : 0;
+	a.x = (const char *)a.x + (long)b0 * a.ldx * esx;
+	a.y = (char *)a.y + (long)b0 * a.ldy * esy;
+	a.xscale = a.xscale ? a.xscale + (long)b0 * a.xgroups : 0;
+	a.B = n;
+	return a;
+}
+
+template <int X, int DT, int RB, int NB, int GM, int W, int D>
+static void w4_skinny_launch(const w4_args &a)
+{
+	typedef W4X<X> K;
+	constexpr int ES = sizeof(typename K::V) / 8;
+	size_t lds = 2 * (size_t)a.B * K::PARTS * (W * W4_KSTEP * ES + 16) + W4_KSTEP * ES;
+	const size_t red = (size_t)W * RB * NB * 1024;
+	lds = lds > red ? lds : red;
+	static bool raised;
+	if (!raised) {
+		hipcheck(hipFuncSetAttribute((const void *)w4_skinny_kernel<X, DT, RB, NB, GM, W, D>,
+			hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+		raised = true;
 	}
+	w4_skinny_kernel<X, DT, RB, NB, GM, W, D><<<dim3((a.blocks + RB - 1) / RB), dim3(W * 64), lds, thhip_stream()>>>(a);
 }
 
 template <int X, int DT, int GM>
 static void w4_choose(const w4_args &a)
 {
-	if (a.B <= 16)
-		w4_skinny_launch<X, DT, 1, 1, GM>(a);
-	else
-		w4_skinny_launch<X, DT, 2, 2, GM>(a);
+	constexpr int P = W4X<X>::PARTS;
+	constexpr size_t esx = sizeof(typename W4X<X>::E), esy = sizeof(typename ThhipElem<DT>::T);
+	for (int b0 = 0; b0 < a.B; b0 += 64 / P) {
+		const w4_args s = w4_rows(a, b0, a.B - b0 < 64 / P ? a.B - b0 : 64 / P, esx, esy);
+		if (s.B * P <= 16) {
+			if (g_w4_tuning == 1 || (!g_w4_tuning && s.blocks < 1024))
+				w4_skinny_launch<X, DT, 1, 1, GM, 16, 2>(s);
+			else if (g_w4_tuning == 3)
+				w4_skinny_launch<X, DT, 1, 1, GM, 8, 3>(s);
+			else
+				w4_skinny_launch<X, DT, 2, 1, GM, 8, 2>(s);
+		} else if (s.B * P <= 32)
+			w4_skinny_launch<X, DT, 1, 2, GM, 8, 2>(s);
+		else
+			w4_skinny_launch<X, DT, 1, 4, GM, 4, 2>(s);
+	}
 }
 
 template <int X, int DT>
@@ -545,8 +643,10 @@ static int w4_run(const char *who, w4_args &a, const void *packed, int group, in
 	a.groups = l.groups;
 	a.group = group;
 	a.xgroups = xgroup ? l.groups : 1;
-	const size_t xv = esx * 8 < 16 ? esx * 8 : 16;
-	a.xvec = (uintptr_t)a.x % xv == 0 && a.ldx * esx % xv == 0;
+	a.shift = 31;
+	for (int i = 5; i <= 8; i++)
+		if (group == 1 << i)
+			a.shift = i;
 	ThhipLaunchScope scope(THHIP_FAM_GEMV, (double)a.nOut * a.nIn / 2 + (double)a.nOut * l.groups * (es + (zeros ? 1 : 0)) +
 		(double)a.B * a.nIn * esx + (double)a.B * a.nOut * es);
 	if (xkind == W4_X_I8)
