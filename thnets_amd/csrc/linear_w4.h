@@ -1,0 +1,169 @@
+/* What the kernels of 4-bit Linear layers (linear_w4.hip, linear_w4_tile.hip) share: the arguments of a call and how
+ * packed codes and rows of x become operands of the matrix core (not installed). */
+#ifndef LINEAR_W4_H
+#define LINEAR_W4_H
+
+#include "thhip_internal.h"
+
+#define W4_KSTEP 128	/* k of a packed step: four matrix instructions of 32 */
+#define W4_X_I8 3	/* kind of x beside THHIP_F32, _F16, _BF16 */
+
+struct w4_args {
+	const void *x;
+	const float *xscale;
+	const unsigned char *codes;
+	const void *scales;
+	const unsigned char *zeros;
+	const float *bias;
+	void *y;
+	long ldx, ldy;
+	int B, nIn, nOut, steps, blocks, groups, group;
+	int xgroups;		/* scales of a row of 8-bit x: 1, or one a group */
+	int act, dtype;
+	float thr, val;
+	int shift;		/* log2(group), 31 where the row is one group */
+	/* the group that matrix instruction j of a packed step belongs to (the last one past K's end) */
+	__host__ __device__ int group_of(int step, int j) const
+	{
+		const int g = (int)(((long)step * W4_KSTEP + 32 * j) >> shift);
+		return g < groups ? g : groups - 1;
+	}
+};
+
+/* What differs with the kind of x: the matrix core's operand of eight k, its accumulator, and how a
+ * word of eight codes and eight elements of x become operands.  PARTS: operands an x vector makes. */
+template <int X> struct W4X;
+
+template <> struct W4X<THHIP_F16> {
+	typedef _Float16 E;
+	typedef halfx8 V;
+	typedef floatx4 A;
+	static constexpr int PARTS = 1;
+	static __device__ __forceinline__ V ones() { return (V)(_Float16)1.0f; }
+	static __device__ __forceinline__ V weights(unsigned w)
+	{
+		typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+		const unsigned lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+		const h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, true);
+		const h2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, true);
+		return (V){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+	}
+	static __device__ __forceinline__ A mma(V a, V b, A c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+	static __device__ __forceinline__ void operand(const E *x, V *out)
+	{
+#pragma unroll
+		for (int e = 0; e < 8; e++)
+			out[0][e] = x[e];
+	}
+};
+
+template <> struct W4X<THHIP_BF16> {
+	typedef __bf16 E;
+	typedef bf16x8 V;
+	typedef floatx4 A;
+	static constexpr int PARTS = 1;
+	static __device__ __forceinline__ V ones() { return (V)(__bf16)1.0f; }
+	static __device__ __forceinline__ V weights(unsigned w)
+	{
+		typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+		const unsigned lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+		const b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, true);
+		const b2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, true);
+		return (V){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+	}
+	static __device__ __forceinline__ A mma(V a, V b, A c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+	static __device__ __forceinline__ void operand(const E *x, V *out)
+	{
+#pragma unroll
+		for (int e = 0; e < 8; e++)
+			out[0][e] = x[e];
+	}
+};
+
+/* fp32: x = a + b + c, each the top sixteen bits of what is left (so eight bits of x; exact).  An
+ * infinity leaves NaN behind: it makes every output of its row NaN. */
+template <> struct W4X<THHIP_F32> {
+	typedef float E;
+	typedef bf16x8 V;
+	typedef floatx4 A;
+	static constexpr int PARTS = 3;
+	static __device__ __forceinline__ V ones() { return W4X<THHIP_BF16>::ones(); }
+	static __device__ __forceinline__ V weights(unsigned w) { return W4X<THHIP_BF16>::weights(w); }
+	static __device__ __forceinline__ A mma(V a, V b, A c) { return W4X<THHIP_BF16>::mma(a, b, c); }
+	static __device__ __forceinline__ void operand(const E *x, V *out)
+	{
+		typedef unsigned U __attribute__((ext_vector_type(4)));
+		U p[3];
+#pragma unroll
+		for (int e = 0; e < 8; e += 2) {
+			float u = x[e], v = x[e + 1];
+#pragma unroll
+			for (int i = 0; i < 3; i++) {
+				const unsigned ub = __float_as_uint(u), vb = __float_as_uint(v);
+				p[i][e / 2] = (ub >> 16) | (vb & 0xffff0000u);
+				u -= __uint_as_float(ub & 0xffff0000u);
+				v -= __uint_as_float(vb & 0xffff0000u);
+			}
+		}
+#pragma unroll
+		for (int i = 0; i < 3; i++)
+			out[i] = __builtin_bit_cast(V, p[i]);
+	}
+};
+
+template <> struct W4X<W4_X_I8> {
+	typedef signed char E;
+	typedef long V;
+	typedef intx4 A;
+	static constexpr int PARTS = 1;
+	static __device__ __forceinline__ V ones() { return 0x0101010101010101l; }
+	static __device__ __forceinline__ V weights(unsigned w)
+	{
+		const unsigned s = w ^ 0x88888888u;
+		return (V)((unsigned long)((s << 4) & 0xf0f0f0f0u) | (unsigned long)(s & 0xf0f0f0f0u) << 32);
+	}
+	static __device__ __forceinline__ A mma(V a, V b, A c) { return __builtin_amdgcn_mfma_i32_16x16x32_i8(a, b, c, 0, 0, 0); }
+	static __device__ __forceinline__ void operand(const E *x, V *out)
+	{
+		unsigned long v = 0;
+#pragma unroll
+		for (int e = 0; e < 8; e++)
+			v |= (unsigned long)(unsigned char)x[e] << (8 * e);
+		out[0] = (V)v;
+	}
+};
+
+/* Eight elements of a row of x from k on; zeros past the row's end */
+template <int X>
+__device__ __forceinline__ void w4_load_x(const void *x, long at, long k, int nIn, typename W4X<X>::E *e)
+{
+	typedef typename W4X<X>::E E;
+	typedef E E8 __attribute__((ext_vector_type(8)));
+	typedef E8 U __attribute__((aligned(sizeof(E))));
+	const E *p = (const E *)x + at + k;
+	if (k + 8 <= nIn) {
+		const E8 v = *(const U *)p;
+#pragma unroll
+		for (int i = 0; i < 8; i++)
+			e[i] = v[i];
+	} else {
+#pragma unroll
+		for (int i = 0; i < 8; i++)
+			e[i] = k + i < nIn ? p[i] : (E)0;
+	}
+}
+
+/* The batch as seen from row b0 on, n rows */
+static inline w4_args w4_rows(w4_args a, int b0, int n, size_t esx, size_t esy)
+{
+	a.x = (const char *)a.x + (long)b0 * a.ldx * esx;
+	a.y = (char *)a.y + (long)b0 * a.ldy * esy;
+	a.xscale = a.xscale ? a.xscale + (long)b0 * a.xgroups : 0;
+	a.B = n;
+	return a;
+}
+
+/* linear_w4_tile.hip: batches for which the matrix cores set the time */
+void w4_tile(const w4_args &a, int xkind);
+
+#endif

@@ -1,0 +1,382 @@
+/*
+ * 4-bit Linear layers (linear_w4.hip) for larger batches: bound by the matrix cores.
+ *
+ * A workgroup of four wavefronts computes 128 rows for BN columns, a wavefront 64 rows x BN / 2.  x goes
+ * through LDS a step of 128 k at a time (two buffers); codes go from memory to registers, one step ahead, and
+ * become operands there: the operands of a whole step stay (64 registers) while its columns are walked 16 at a
+ * time, so that the sums of one group of 16 columns are all there is beside the result.  During a step's last
+ * columns its operands are replaced, one after the other, by the next step's.  The sums of a group start at
+ * -z * sum x, so that what is left when it ends is one multiply-add a value.
+ * fp32 x is three planes of bf16 in LDS (BN = 64); 8-bit x is multiplied 64 k at a time (32 for groups of 32).
+ * LDS rows are 128 k of a column; a 16-byte vector v of row r lies in slot v ^ r % 16 (8-bit x: v ^ r / 2 % 8),
+ * which puts the 16 columns of an operand on different banks.  DMA: rows that memory holds in whole, aligned
+ * 16-byte vectors are loaded straight into LDS; others go through registers.
+ */
+#include <stdint.h>
+#include "linear_w4.h"
+
+template <int X, bool WIDE> struct W4Tile {		/* operands of 32 k, as W4X has them */
+	typedef typename W4X<X>::V V;
+	typedef typename W4X<X>::A A;
+	static constexpr int MK = 32;
+	static __device__ __forceinline__ V ones() { return W4X<X>::ones(); }
+	static __device__ __forceinline__ V weights(const uintx4 &c, int j) { return W4X<X>::weights(c[j]); }
+	static __device__ __forceinline__ A mma(V a, V b, A c) { return W4X<X>::mma(a, b, c); }
+	/* at: the row's address; r: the row in the tile; q: lane / 16 */
+	static __device__ __forceinline__ V read(const unsigned char *at, int r, int j, int q)
+	{
+		if constexpr (X == W4_X_I8)
+			return *(const V *)(at + (((2 * j + (q >> 1)) ^ (r >> 1 & 7)) * 16 + (q & 1) * 8));
+		else
+			return *(const V *)(at + ((4 * j + q) ^ (r & 15)) * 16);
+	}
+};
+
+template <> struct W4Tile<W4_X_I8, true> {		/* 8-bit operands of 64 k: two of 32 side by side */
+	typedef intx4 V;
+	typedef intx4 A;
+	typedef W4Tile<W4_X_I8, false> H;
+	static constexpr int MK = 64;
+	static __device__ __forceinline__ V join(long lo, long hi)
+	{
+		return (V){(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
+	}
+	static __device__ __forceinline__ V ones() { return (V)0x01010101; }
+	static __device__ __forceinline__ V weights(const uintx4 &c, int j) { return join(H::weights(c, 2 * j), H::weights(c, 2 * j + 1)); }
+	static __device__ __forceinline__ A mma(V a, V b, A c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+	static __device__ __forceinline__ V read(const unsigned char *at, int r, int j, int q)
+	{
+		return join(H::read(at, r, 2 * j, q), H::read(at, r, 2 * j + 1, q));
+	}
+};
+
+#define W4_LDS(p) ((__attribute__((address_space(3))) void *)(p))
+
+/* Scales and results in the layer's type, which only the ends of the tile kernel see: that of x, or, where x is
+ * 8-bit, known when the kernel runs */
+template <int X>
+__device__ __forceinline__ float w4_get(const void *p, long i, int dtype)
+{
+	if constexpr (X != W4_X_I8)
+		return ThhipElem<X>::ld(p, i);
+	else {
+		const unsigned u = dtype == THHIP_F32 ? ((const unsigned *)p)[i] : (unsigned)((const unsigned short *)p)[i];
+		const float h = (float)__builtin_bit_cast(_Float16, (unsigned short)u);
+		return dtype == THHIP_F16 ? h : __uint_as_float(dtype == THHIP_F32 ? u : u << 16);
+	}
+}
+
+template <int X>
+__device__ __forceinline__ void w4_put(void *p, long i, float v, int dtype)
+{
+	if constexpr (X != W4_X_I8)
+		ThhipElem<X>::st(p, i, v);
+	else if (dtype == THHIP_F32)
+		ThhipElem<THHIP_F32>::st(p, i, v);
+	else if (dtype == THHIP_F16)
+		ThhipElem<THHIP_F16>::st(p, i, v);
+	else
+		ThhipElem<THHIP_BF16>::st(p, i, v);
+}
+
+template <int X, int GM, bool ZP, bool DMA>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_F32 ? 1 : 2, 2))) void w4_tile_kernel(const w4_args a, int mtiles, int ntiles)
+{
+	typedef W4X<X> K;
+	typedef W4Tile<X, X == W4_X_I8 && GM >= 2> M;
+	typedef typename M::V V;
+	typedef typename M::A A;
+	constexpr int PARTS = K::PARTS, NB = PARTS > 1 ? 2 : 4, BN = 32 * NB;
+	constexpr int ES = sizeof(typename K::V) / 8;
+	constexpr int ROW = W4_KSTEP * ES;			/* bytes of a row in LDS */
+	constexpr int PLANE = BN * ROW, STAGE = PARTS * PLANE;
+	constexpr int NJ = W4_KSTEP / M::MK, GJ = GM * 32 / M::MK;	/* matrix instructions of a step, of a group */
+	constexpr int PIECES = BN * 16 / 256;			/* vectors of eight k a thread moves a step */
+	constexpr int CORR = X != W4_X_I8;
+	constexpr int NG = 4 / GM;				/* groups of a step */
+	__shared__ __align__(16) unsigned char lds[2 * STAGE];
+	__shared__ floatx4 lscale[2][NG][32];			/* the 128 rows' scales of a step's groups */
+	__shared__ floatx4 lzero[2][NG][32];			/* ... and zeros: -z, or (8-bit x) 128 - 16 z as an int */
+	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	const int col = lane & 15, quarter = lane >> 4;
+
+	/* the tiles of an XCD (workgroups b, b + 8, ...) are neighbours, in columns of eight row tiles */
+	int id = blockIdx.x;
+	{
+		const int total = mtiles * ntiles, per = total / 8;
+		if (id < per * 8)
+			id = (id & 7) * per + (id >> 3);
+		const int band = 8 * ntiles, m0 = id / band * 8, left = mtiles - m0 < 8 ? mtiles - m0 : 8;
+		const int in = id - id / band * band;
+		id = (m0 + in % left) * ntiles + in / left;
+	}
+	const int mt = id / ntiles, nt = id - mt * ntiles;
+	const int b0 = nt * BN, nrows = a.B - b0 < BN ? a.B - b0 : BN;
+	const int rb0 = mt * 8 + (wave & 1) * 4, c0 = (wave >> 1) * NB * 16;
+
+	const typename K::E *xbase = (const typename K::E *)a.x + (long)b0 * a.ldx;
+	const unsigned xend = DMA ? (unsigned)(((nrows - 1) * a.ldx + a.nIn) * (long)sizeof(typename K::E)) : 0;
+	const __amdgpu_buffer_rsrc_t xrsrc = __builtin_amdgcn_make_buffer_rsrc((void *)xbase, 0, xend, 0x00020000);
+	typename K::E xr[DMA ? 1 : PIECES / 2][8];
+
+	/* x of step t on its way (half: one of the two halves that go through registers one after the other) */
+	auto x_issue = [&](int t, int buf, int half) {
+		if constexpr (DMA) {
+			constexpr int VROW = ROW / 16, RPI = 64 / VROW;	/* vectors of a row; rows a wavefront's load covers */
+			const int r0 = wave * RPI + lane / VROW, slot = lane % VROW;
+			const int v = ES == 1 ? slot ^ (r0 >> 1 & 7) : slot ^ (r0 & 15);
+			const int k = t * ROW + v * 16;		/* (bytes) */
+#pragma unroll
+			for (int i = 0; i < BN / (4 * RPI); i++) {
+				__builtin_amdgcn_raw_ptr_buffer_load_lds(xrsrc, W4_LDS(lds + buf * STAGE + (i * 4 + wave) * 1024), 16,
+					k < a.nIn * ES ? (unsigned)(r0 * (int)a.ldx * ES + k) : 0x80000000u, i * 4 * RPI * (int)a.ldx * ES, 0, 0);
+			}
+		} else {
+#pragma unroll
+			for (int i = 0; i < PIECES / 2; i++) {
+				const int p = tid + (half * (PIECES / 2) + i) * 256, r = p >> 4;
+				if (r < nrows)
+					w4_load_x<X>(xbase, r * a.ldx, (long)t * W4_KSTEP + (p & 15) * 8, a.nIn, xr[i]);
+				else
+#pragma unroll
+					for (int e = 0; e < 8; e++)
+						xr[i][e] = (typename K::E)0;
+			}
+		}
+	};
+	auto x_land = [&](int buf, int half) {
+		if constexpr (!DMA) {
+#pragma unroll
+			for (int i = 0; i < PIECES / 2; i++) {
+				const int p = tid + (half * (PIECES / 2) + i) * 256, r = p >> 4, v = p & 15;
+				typename K::V o[PARTS];
+				K::operand(xr[i], o);
+				const int to = ES == 1 ? ((v >> 1) ^ (r >> 1 & 7)) * 16 + (v & 1) * 8 : (v ^ (r & 15)) * 16;
+#pragma unroll
+				for (int q = 0; q < PARTS; q++)
+					*(typename K::V *)(lds + buf * STAGE + q * PLANE + r * ROW + to) = o[q];
+			}
+		}
+	};
+	/* scales and zeros: thread i < 128 fetches row i's, and puts them into LDS a step later */
+	float gs[NG], gz[NG];
+	const int grb = mt * 8 + (tid >> 4 & 7) < a.blocks ? mt * 8 + (tid >> 4 & 7) : a.blocks - 1;
+	auto g_issue = [&](int t) {
+		if (tid < 128) {
+#pragma unroll
+			for (int g = 0; g < NG; g++) {
+				const long at = ((long)grb * a.groups + a.group_of(t, g * GM)) * 16 + (tid & 15);
+				gs[g] = w4_get<X>(a.scales, at, a.dtype);
+				if constexpr (ZP)
+					gz[g] = X == W4_X_I8 ? __int_as_float(128 - 16 * (int)a.zeros[at]) : -(float)a.zeros[at];
+			}
+		}
+	};
+	auto g_land = [&](int buf) {
+		if (tid < 128) {
+#pragma unroll
+			for (int g = 0; g < NG; g++) {
+				((float *)lscale[buf][g])[tid] = gs[g];
+				if constexpr (ZP)
+					((float *)lzero[buf][g])[tid] = gz[g];
+			}
+		}
+	};
+	uintx4 codes[4];
+	auto codes_issue = [&](int t) {
+#pragma unroll
+		for (int r = 0; r < 4; r++) {
+			const int rb = rb0 + r < a.blocks ? rb0 + r : a.blocks - 1;
+			codes[r] = *(const uintx4 *)(a.codes + ((size_t)rb * a.steps + t) * 1024 + lane * 16);
+		}
+	};
+	/* (the loads into LDS are not the compiler's to wait for) */
+	auto barrier = [&]() {
+		asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+	};
+
+	floatx4 acc[4][NB];
+#pragma unroll
+	for (int r = 0; r < 4; r++)
+#pragma unroll
+		for (int n = 0; n < NB; n++)
+			acc[r][n] = (floatx4)0.0f;
+
+	x_issue(0, 0, 0);
+	x_land(0, 0);
+	if (!DMA) {
+		x_issue(0, 0, 1);
+		x_land(0, 1);
+	}
+	codes_issue(0);
+	g_issue(0);
+	V w[4][NJ];
+#pragma unroll
+	for (int r = 0; r < 4; r++)
+#pragma unroll
+		for (int j = 0; j < NJ; j++)
+			w[r][j] = M::weights(codes[r], j);
+	g_land(0);
+	barrier();
+
+	for (int t = 0; t < a.steps; t++) {
+		const int buf = t & 1, t1 = t + 1 < a.steps ? t + 1 : t;
+		const unsigned char *base = lds + buf * STAGE;
+		x_issue(t1, buf ^ 1, 0);
+		codes_issue(t1);
+		g_issue(t1);
+#pragma unroll
+		for (int n = 0; n < NB; n++) {
+			const int row = c0 + n * 16 + col;
+			asm volatile("" ::: "memory");	/* (operands and scales are read again for every n, not kept) */
+			__builtin_amdgcn_sched_barrier(0);
+			if (!DMA && n == NB / 2) {
+				x_land(buf ^ 1, 0);
+				x_issue(t1, buf ^ 1, 1);
+			}
+			V x[PARTS][NJ];
+#pragma unroll
+			for (int q = 0; q < PARTS; q++)
+#pragma unroll
+				for (int j = 0; j < NJ; j++)
+					x[q][j] = M::read(base + q * PLANE + row * ROW, col, j, quarter);
+#pragma unroll
+			for (int g = 0; g < NJ / GJ; g++) {
+				A sx = (A)0, p[4];
+				if (NG > 1) {
+					asm volatile("" ::: "memory");
+					__builtin_amdgcn_sched_barrier(0);
+				}
+				if constexpr (CORR || ZP) {
+#pragma unroll
+					for (int j = g * GJ; j < (g + 1) * GJ; j++)
+#pragma unroll
+						for (int q = 0; q < PARTS; q++)
+							sx = M::mma(M::ones(), x[q][j], sx);
+				}
+				const int quad = (wave & 1) * 16 + quarter;	/* of the wavefront's first row block */
+#pragma unroll
+				for (int r = 0; r < 4; r++) {
+					if constexpr (ZP) {
+						const floatx4 z = lzero[buf][g][quad + r * 4];
+#pragma unroll
+						for (int i = 0; i < 4; i++) {
+							if constexpr (X == W4_X_I8)
+								p[r][i] = __mul24(__float_as_int(z[i]), sx[i]);
+							else
+								p[r][i] = z[i] * sx[i];
+						}
+					} else if constexpr (X == W4_X_I8)
+						p[r] = (A)0;
+					else
+						p[r] = -8.0f * sx;
+				}
+#pragma unroll
+				for (int j = g * GJ; j < (g + 1) * GJ; j++) {
+#pragma unroll
+					for (int q = 0; q < PARTS; q++)
+#pragma unroll
+						for (int r = 0; r < 4; r++)
+							p[r] = M::mma(w[r][j], x[q][j], p[r]);
+					if (n == NB - 1) {	/* the operands' last use in this step */
+						__builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+						for (int r = 0; r < 4; r++)
+							w[r][j] = M::weights(codes[r], j);
+					}
+				}
+				float xs = X == W4_X_I8 ? 0.0625f : 1.0f;
+				if (X == W4_X_I8 && a.xgroups > 1)
+					xs *= a.xscale[(long)(b0 + (row < nrows ? row : 0)) * a.xgroups + a.group_of(t, g * GM)];
+#pragma unroll
+				for (int r = 0; r < 4; r++) {
+					const floatx4 s = lscale[buf][g][quad + r * 4];
+#pragma unroll
+					for (int i = 0; i < 4; i++)
+						acc[r][n][i] += s[i] * (X == W4_X_I8 ? xs * (float)p[r][i] : (float)p[r][i]);
+					/* (here, not at the end of the step, where the compiler would gather all n's sums) */
+					asm volatile("" : "+v"(acc[r][n]));
+				}
+			}
+		}
+		x_land(buf ^ 1, DMA ? 0 : 1);
+		g_land(buf ^ 1);
+		barrier();
+	}
+
+#pragma unroll
+	for (int n = 0; n < NB; n++) {
+		const int b = b0 + c0 + n * 16 + col;
+		if (b >= a.B)
+			continue;
+		const float xs = X == W4_X_I8 && a.xgroups == 1 ? a.xscale[b] : 1.0f;
+#pragma unroll
+		for (int r = 0; r < 4; r++) {
+			const int o = (rb0 + r) * 16 + 4 * quarter;
+#pragma unroll
+			for (int i = 0; i < 4; i++)
+				if (o + i < a.nOut) {
+					float y = acc[r][n][i] * xs + (a.bias ? a.bias[o + i] : 0.0f);
+					if (a.act)
+						y = y > a.thr ? y : a.val;
+					w4_put<X>(a.y, b * a.ldy + o + i, y, a.dtype);
+				}
+		}
+	}
+}
+
+/* A launch has at most this many rows of x, so that a grid stays below 2^32 threads */
+#define W4_TILE_ROWS (1 << 20)
+
+template <int X, int GM>
+static void w4_tile_launch(const w4_args &all)
+{
+	constexpr size_t esx = sizeof(typename W4X<X>::E);
+	const size_t esy = thhip_esize(all.dtype);
+	constexpr int BN = W4X<X>::PARTS > 1 ? 64 : 128;
+	for (int b0 = 0; b0 < all.B; b0 += W4_TILE_ROWS) {
+		const w4_args a = w4_rows(all, b0, all.B - b0 < W4_TILE_ROWS ? all.B - b0 : W4_TILE_ROWS, esx, esy);
+		const int mtiles = (a.blocks + 7) / 8, ntiles = (a.B + BN - 1) / BN;
+		const dim3 grid((unsigned)mtiles * ntiles);
+		/* rows in whole vectors, and a tile of them within the reach of a buffer descriptor */
+		const bool dma = X != THHIP_F32 && (uintptr_t)a.x % 16 == 0 && a.ldx * esx % 16 == 0 && a.nIn * esx % 16 == 0 &&
+			a.ldx * esx * BN < (1u << 31);
+#define W4_TILE(ZP, DMA) w4_tile_kernel<X, GM, ZP, DMA><<<grid, dim3(256), 0, thhip_stream()>>>(a, mtiles, ntiles)
+		if constexpr (X != THHIP_F32)
+			if (dma) {
+				if (a.zeros)
+					W4_TILE(true, true);
+				else
+					W4_TILE(false, true);
+				continue;
+			}
+		if (a.zeros)
+			W4_TILE(true, false);
+		else
+			W4_TILE(false, false);
+#undef W4_TILE
+	}
+}
+
+template <int X>
+static void w4_tile_groups(const w4_args &a)
+{
+	if (a.group == 32)
+		w4_tile_launch<X, 1>(a);
+	else if (a.group == 64)
+		w4_tile_launch<X, 2>(a);
+	else
+		w4_tile_launch<X, 4>(a);
+}
+
+void w4_tile(const w4_args &a, int xkind)
+{
+	if (xkind == W4_X_I8)
+		w4_tile_groups<W4_X_I8>(a);
+	else if (xkind == THHIP_F32)
+		w4_tile_groups<THHIP_F32>(a);
+	else if (xkind == THHIP_F16)
+		w4_tile_groups<THHIP_F16>(a);
+	else
+		w4_tile_groups<THHIP_BF16>(a);
+}
