@@ -158,28 +158,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 			}
 		}
 	};
-	/* scales and zeros: thread i < 128 fetches row i's, and puts them into LDS a step later */
+	/* scales and zeros: thread i fetches row i % 128's, and puts them into LDS at the end of the step */
 	float gs[NG], gz[NG];
 	const int grb = mt * 8 + (tid >> 4 & 7) < a.blocks ? mt * 8 + (tid >> 4 & 7) : a.blocks - 1;
 	auto g_issue = [&](int t) {
-		if (tid < 128) {
 #pragma unroll
-			for (int g = 0; g < NG; g++) {
-				const long at = ((long)grb * a.groups + a.group_of(t, g * GM)) * 16 + (tid & 15);
-				gs[g] = w4_get<X>(a.scales, at, a.dtype);
-				if constexpr (ZP)
-					gz[g] = X == W4_X_I8 ? __int_as_float(128 - 16 * (int)a.zeros[at]) : -(float)a.zeros[at];
-			}
+		for (int g = 0; g < NG; g++) {
+			const long at = ((long)grb * a.groups + a.group_of(t, g * GM)) * 16 + (tid & 15);
+			gs[g] = w4_get<X>(a.scales, at, a.dtype);
+			if constexpr (ZP)
+				gz[g] = X == W4_X_I8 ? __int_as_float(128 - 16 * (int)a.zeros[at]) : -(float)a.zeros[at];
 		}
 	};
 	auto g_land = [&](int buf) {
-		if (tid < 128) {
 #pragma unroll
-			for (int g = 0; g < NG; g++) {
-				((float *)lscale[buf][g])[tid] = gs[g];
-				if constexpr (ZP)
-					((float *)lzero[buf][g])[tid] = gz[g];
-			}
+		for (int g = 0; g < NG; g++) {
+			((float *)lscale[buf][g])[tid & 127] = gs[g];
+			if constexpr (ZP)
+				((float *)lzero[buf][g])[tid & 127] = gz[g];
 		}
 	};
 	uintx4 codes[4];
@@ -210,95 +206,114 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 	}
 	codes_issue(0);
 	g_issue(0);
-	V w[4][NJ];
-#pragma unroll
-	for (int r = 0; r < 4; r++)
-#pragma unroll
-		for (int j = 0; j < NJ; j++)
-			w[r][j] = M::weights(codes[r], j);
 	g_land(0);
 	barrier();
 
+	constexpr int NU = NB * NG;		/* units of a step: 16 columns x one group */
+	const int quad = (wave & 1) * 16 + quarter;	/* where the scales of the wavefront's rows begin */
 	for (int t = 0; t < a.steps; t++) {
 		const int buf = t & 1, t1 = t + 1 < a.steps ? t + 1 : t;
-		const unsigned char *base = lds + buf * STAGE;
-		x_issue(t1, buf ^ 1, 0);
-		codes_issue(t1);
-		g_issue(t1);
-#pragma unroll
-		for (int n = 0; n < NB; n++) {
-			const int row = c0 + n * 16 + col;
-			asm volatile("" ::: "memory");	/* (operands and scales are read again for every n, not kept) */
-			__builtin_amdgcn_sched_barrier(0);
-			if (!DMA && n == NB / 2) {
-				x_land(buf ^ 1, 0);
-				x_issue(t1, buf ^ 1, 1);
-			}
-			V x[PARTS][NJ];
+		const unsigned char *base = lds + buf * STAGE + (c0 + col) * ROW;
+		V w[4][NJ], x[2][PARTS][NJ];
+		A p[2][4], sx[2];
+		auto x_read = [&](int n) {
 #pragma unroll
 			for (int q = 0; q < PARTS; q++)
 #pragma unroll
 				for (int j = 0; j < NJ; j++)
-					x[q][j] = M::read(base + q * PLANE + row * ROW, col, j, quarter);
+					x[n & 1][q][j] = M::read(base + q * PLANE + n * 16 * ROW, col, j, quarter);
+		};
+		/* sum of x over unit u's group, in every row of the accumulator */
+		auto x_sum = [&](int u) {
+			if constexpr (CORR || ZP) {
+				const int n = u / NG, g = u % NG;
+				sx[u & 1] = (A)0;
 #pragma unroll
-			for (int g = 0; g < NJ / GJ; g++) {
-				A sx = (A)0, p[4];
-				if (NG > 1) {
-					asm volatile("" ::: "memory");
-					__builtin_amdgcn_sched_barrier(0);
-				}
-				if constexpr (CORR || ZP) {
-#pragma unroll
-					for (int j = g * GJ; j < (g + 1) * GJ; j++)
-#pragma unroll
-						for (int q = 0; q < PARTS; q++)
-							sx = M::mma(M::ones(), x[q][j], sx);
-				}
-				const int quad = (wave & 1) * 16 + quarter;	/* of the wavefront's first row block */
-#pragma unroll
-				for (int r = 0; r < 4; r++) {
-					if constexpr (ZP) {
-						const floatx4 z = lzero[buf][g][quad + r * 4];
-#pragma unroll
-						for (int i = 0; i < 4; i++) {
-							if constexpr (X == W4_X_I8)
-								p[r][i] = __mul24(__float_as_int(z[i]), sx[i]);
-							else
-								p[r][i] = z[i] * sx[i];
-						}
-					} else if constexpr (X == W4_X_I8)
-						p[r] = (A)0;
-					else
-						p[r] = -8.0f * sx;
-				}
-#pragma unroll
-				for (int j = g * GJ; j < (g + 1) * GJ; j++) {
+				for (int j = g * GJ; j < (g + 1) * GJ; j++)
 #pragma unroll
 					for (int q = 0; q < PARTS; q++)
-#pragma unroll
-						for (int r = 0; r < 4; r++)
-							p[r] = M::mma(w[r][j], x[q][j], p[r]);
-					if (n == NB - 1) {	/* the operands' last use in this step */
-						__builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-						for (int r = 0; r < 4; r++)
-							w[r][j] = M::weights(codes[r], j);
-					}
-				}
-				float xs = X == W4_X_I8 ? 0.0625f : 1.0f;
-				if (X == W4_X_I8 && a.xgroups > 1)
-					xs *= a.xscale[(long)(b0 + (row < nrows ? row : 0)) * a.xgroups + a.group_of(t, g * GM)];
-#pragma unroll
-				for (int r = 0; r < 4; r++) {
-					const floatx4 s = lscale[buf][g][quad + r * 4];
-#pragma unroll
-					for (int i = 0; i < 4; i++)
-						acc[r][n][i] += s[i] * (X == W4_X_I8 ? xs * (float)p[r][i] : (float)p[r][i]);
-					/* (here, not at the end of the step, where the compiler would gather all n's sums) */
-					asm volatile("" : "+v"(acc[r][n]));
-				}
+						sx[u & 1] = M::mma(M::ones(), x[n & 1][q][j], sx[u & 1]);
 			}
+		};
+		/* unit u's finished sums into the result */
+		auto flush = [&](int u) {
+			const int n = u / NG, g = u % NG;
+			float xs = 1.0f;
+			if constexpr (X == W4_X_I8) {
+				const int row = c0 + n * 16 + col;
+				const float v = a.xscale[(long)(b0 + (row < nrows ? row : 0)) * a.xgroups + (a.xgroups > 1 ? a.group_of(t, g * GM) : 0)];
+				xs = 0.0625f * (a.xgroups > 1 ? v : 1.0f);
+			}
+#pragma unroll
+			for (int r = 0; r < 4; r++) {
+				const floatx4 s = lscale[buf][g][quad + r * 4];
+#pragma unroll
+				for (int i = 0; i < 4; i++)
+					acc[r][n][i] += s[i] * (X == W4_X_I8 ? xs * (float)p[u & 1][r][i] : (float)p[u & 1][r][i]);
+				/* (here, not at the end of the step, where the compiler would gather all n's sums) */
+				asm("" : "+v"(acc[r][n]));
+			}
+		};
+		x_issue(t1, buf ^ 1, 0);
+		x_read(0);
+#pragma unroll
+		for (int j = 0; j < NJ; j++)
+#pragma unroll
+			for (int r = 0; r < 4; r++)
+				w[r][j] = M::weights(codes[r], j);
+		x_sum(0);
+		codes_issue(t1);
+		g_issue(t1);
+#pragma unroll
+		for (int u = 0; u < NU; u++) {
+			const int n = u / NG, g = u % NG;
+			asm volatile("" ::: "memory");	/* (operands and scales are read again for every unit, not kept) */
+			__builtin_amdgcn_sched_barrier(0);
+			if (!DMA && u == NU / 2) {
+				x_land(buf ^ 1, 0);
+				x_issue(t1, buf ^ 1, 1);
+			}
+			if (g == 0 && n + 1 < NB)
+				x_read(n + 1);
+#pragma unroll
+			for (int r = 0; r < 4; r++) {
+				if constexpr (ZP) {
+					const floatx4 z = lzero[buf][g][quad + r * 4];
+#pragma unroll
+					for (int i = 0; i < 4; i++) {
+						if constexpr (X == W4_X_I8)
+							p[u & 1][r][i] = __mul24(__float_as_int(z[i]), sx[u & 1][i]);
+						else
+							p[u & 1][r][i] = z[i] * sx[u & 1][i];
+					}
+				} else if constexpr (X == W4_X_I8)
+					p[u & 1][r] = (A)0;
+				else
+					p[u & 1][r] = -8.0f * sx[u & 1];
+			}
+#pragma unroll
+			for (int j = g * GJ; j < (g + 1) * GJ; j++)
+#pragma unroll
+				for (int q = 0; q < PARTS; q++)
+#pragma unroll
+					for (int r = 0; r < 4; r++)
+						p[u & 1][r] = M::mma(w[r][j], x[n & 1][q][j], p[u & 1][r]);
+			if (u + 1 < NU)
+				x_sum(u + 1);
+			if (u > 0)
+				flush(u - 1);
+			/* the order to issue them in: what comes from LDS, then a matrix instruction and the sums' work in turn */
+			__builtin_amdgcn_sched_group_barrier(0x100, PARTS * NJ + 4, 0);
+			__builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+#pragma unroll
+			for (int i = 0; i < 4 * GJ * PARTS; i++) {
+				__builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+				__builtin_amdgcn_sched_group_barrier(0x2, 1, 0);
+			}
+			__builtin_amdgcn_sched_group_barrier(0x8, GJ * PARTS, 0);
 		}
+		__builtin_amdgcn_sched_barrier(0);
+		flush(NU - 1);
 		x_land(buf ^ 1, DMA ? 0 : 1);
 		g_land(buf ^ 1);
 		barrier();
