@@ -36,6 +36,7 @@ template <int X> struct W4X;
 
 template <> struct W4X<THHIP_F16> {
 	typedef _Float16 E;
+	typedef E E8 __attribute__((ext_vector_type(8)));
 	typedef halfx8 V;
 	typedef floatx4 A;
 	static constexpr int PARTS = 1;
@@ -49,16 +50,12 @@ template <> struct W4X<THHIP_F16> {
 		return (V){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 	}
 	static __device__ __forceinline__ A mma(V a, V b, A c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-	static __device__ __forceinline__ void operand(const E *x, V *out)
-	{
-#pragma unroll
-		for (int e = 0; e < 8; e++)
-			out[0][e] = x[e];
-	}
+	static __device__ __forceinline__ void operand(const E8 x, V *out) { out[0] = x; }
 };
 
 template <> struct W4X<THHIP_BF16> {
 	typedef __bf16 E;
+	typedef E E8 __attribute__((ext_vector_type(8)));
 	typedef bf16x8 V;
 	typedef floatx4 A;
 	static constexpr int PARTS = 1;
@@ -72,25 +69,21 @@ template <> struct W4X<THHIP_BF16> {
 		return (V){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 	}
 	static __device__ __forceinline__ A mma(V a, V b, A c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-	static __device__ __forceinline__ void operand(const E *x, V *out)
-	{
-#pragma unroll
-		for (int e = 0; e < 8; e++)
-			out[0][e] = x[e];
-	}
+	static __device__ __forceinline__ void operand(const E8 x, V *out) { out[0] = x; }
 };
 
 /* fp32: x = a + b + c, each the top sixteen bits of what is left (so eight bits of x; exact).  An
  * infinity leaves NaN behind: it makes every output of its row NaN. */
 template <> struct W4X<THHIP_F32> {
 	typedef float E;
+	typedef E E8 __attribute__((ext_vector_type(8)));
 	typedef bf16x8 V;
 	typedef floatx4 A;
 	static constexpr int PARTS = 3;
 	static __device__ __forceinline__ V ones() { return W4X<THHIP_BF16>::ones(); }
 	static __device__ __forceinline__ V weights(unsigned w) { return W4X<THHIP_BF16>::weights(w); }
 	static __device__ __forceinline__ A mma(V a, V b, A c) { return W4X<THHIP_BF16>::mma(a, b, c); }
-	static __device__ __forceinline__ void operand(const E *x, V *out)
+	static __device__ __forceinline__ void operand(const E8 x, V *out)
 	{
 		typedef unsigned U __attribute__((ext_vector_type(4)));
 		U p[3];
@@ -113,6 +106,7 @@ template <> struct W4X<THHIP_F32> {
 
 template <> struct W4X<W4_X_I8> {
 	typedef signed char E;
+	typedef E E8 __attribute__((ext_vector_type(8)));
 	typedef long V;
 	typedef intx4 A;
 	static constexpr int PARTS = 1;
@@ -123,33 +117,48 @@ template <> struct W4X<W4_X_I8> {
 		return (V)((unsigned long)((s << 4) & 0xf0f0f0f0u) | (unsigned long)(s & 0xf0f0f0f0u) << 32);
 	}
 	static __device__ __forceinline__ A mma(V a, V b, A c) { return __builtin_amdgcn_mfma_i32_16x16x32_i8(a, b, c, 0, 0, 0); }
-	static __device__ __forceinline__ void operand(const E *x, V *out)
-	{
-		unsigned long v = 0;
-#pragma unroll
-		for (int e = 0; e < 8; e++)
-			v |= (unsigned long)(unsigned char)x[e] << (8 * e);
-		out[0] = (V)v;
-	}
+	static __device__ __forceinline__ void operand(const E8 x, V *out) { out[0] = __builtin_bit_cast(V, x); }
 };
 
-/* Eight elements of a row of x from k on; zeros past the row's end */
-template <int X>
-__device__ __forceinline__ void w4_load_x(const void *x, long at, long k, int nIn, typename W4X<X>::E *e)
+/* Vectors of eight elements of x that may begin anywhere and end behind their row (row r begins at element r * ldx; row(i) and
+ * k(i) say which ones).  fetch loads them without a branch, so that all are on their way together (with one round each,
+ * the compiler waited for one before the next), and takes a row's last eight where it ends before; fix moves
+ * those to their places, with zeros past the end.  Rows of fewer than eight elements are put together one by one. */
+template <int X, int N, typename ROW, typename KAT>
+__device__ __forceinline__ void w4_fetch_x(typename W4X<X>::E8 (&v)[N], const void *x, long ldx, int nIn, ROW row, KAT k)
 {
 	typedef typename W4X<X>::E E;
-	typedef E E8 __attribute__((ext_vector_type(8)));
+	typedef typename W4X<X>::E8 E8;
 	typedef E8 U __attribute__((aligned(sizeof(E))));
-	const E *p = (const E *)x + at + k;
-	if (k + 8 <= nIn) {
-		const E8 v = *(const U *)p;
+	if (nIn >= 8) {
 #pragma unroll
-		for (int i = 0; i < 8; i++)
-			e[i] = v[i];
+		for (int i = 0; i < N; i++)
+			v[i] = *(const U *)((const E *)x + row(i) * ldx + (k(i) < nIn - 8 ? k(i) : nIn - 8));
 	} else {
 #pragma unroll
-		for (int i = 0; i < 8; i++)
-			e[i] = k + i < nIn ? p[i] : (E)0;
+		for (int i = 0; i < N; i++)
+#pragma unroll
+			for (int e = 0; e < 8; e++)
+				v[i][e] = ((const E *)x + row(i) * ldx)[e < nIn ? e : nIn - 1];
+	}
+}
+
+template <int X, int N, typename KAT>
+__device__ __forceinline__ void w4_fix_x(typename W4X<X>::E8 (&v)[N], int nIn, KAT k)
+{
+	typedef typename W4X<X>::E E;
+	const int first = nIn >= 8 ? nIn - 8 : 0;
+#pragma unroll
+	for (int i = 0; i < N; i++) {
+		const int by = k(i) > first ? (k(i) - first < 8 ? k(i) - first : 8) : 0;
+#pragma unroll
+		for (int b = 1; b < 8; b *= 2)
+#pragma unroll
+			for (int e = 0; e < 8; e++)
+				v[i][e] = by & b ? (e + b < 8 ? v[i][e + b] : (E)0) : v[i][e];
+#pragma unroll
+		for (int e = 0; e < 8; e++)
+			v[i][e] = k(i) + e < nIn ? v[i][e] : (E)0;
 	}
 }
 
@@ -161,6 +170,20 @@ static inline w4_args w4_rows(w4_args a, int b0, int n, size_t esx, size_t esy)
 	a.xscale = a.xscale ? a.xscale + (long)b0 * a.xgroups : 0;
 	a.B = n;
 	return a;
+}
+
+/* A result, in the type of x or, where x is 8-bit, in the one the call names */
+template <int X>
+__device__ __forceinline__ void w4_put(void *p, long i, float v, int dtype)
+{
+	if constexpr (X != W4_X_I8)
+		ThhipElem<X>::st(p, i, v);
+	else if (dtype == THHIP_F32)
+		ThhipElem<THHIP_F32>::st(p, i, v);
+	else if (dtype == THHIP_F16)
+		ThhipElem<THHIP_F16>::st(p, i, v);
+	else
+		ThhipElem<THHIP_BF16>::st(p, i, v);
 }
 
 /* linear_w4_tile.hip: batches for which the matrix cores set the time */

@@ -49,7 +49,8 @@ static struct w4_layout w4_layout_of(int nOut, int nIn, int group, int dtype, in
 	l.groups = group ? (int)(((long)nIn + group - 1) / group) : 1;
 	l.scales = (size_t)l.blocks * l.steps * 1024;
 	l.zeros = l.scales + round16((size_t)l.blocks * l.groups * 16 * thhip_esize(dtype));
-	l.bytes = l.zeros + (zeros ? (size_t)l.blocks * l.groups * 16 : 0);
+	/* (16 bytes more: the scales' last four may be loaded with the four behind) */
+	l.bytes = l.zeros + (zeros ? (size_t)l.blocks * l.groups * 16 : 0) + 16;
 	return l;
 }
 
@@ -232,9 +233,13 @@ __device__ __forceinline__ void w4_lds_barrier(void)
 	asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-/* What a wavefront fetches ahead of a step: the codes of its row blocks and what their groups need */
-template <int DT, int RB, int GM> struct W4Step {
-	typedef typename ThhipElem<DT>::T T4 __attribute__((ext_vector_type(4)));
+/* What a wavefront fetches ahead of a step: the codes of its row blocks and what their groups need.  (The number of
+ * loads does not depend on the call, so that the compiler can count how many may be outstanding when it needs one.) */
+template <int X, int RB, int GM, bool ZP> struct W4Step {
+	/* 8-bit x: four scales of any type, or of a half type with four more behind */
+	typedef typename ThhipElem<X == W4_X_I8 ? THHIP_F32 : X>::T T;
+	typedef T T4 __attribute__((ext_vector_type(4)));
+	typedef T4 U4 __attribute__((aligned(8)));
 	uintx4 codes[RB];
 	T4 s[RB][4 / GM];
 	unsigned z[RB][4 / GM];
@@ -242,59 +247,92 @@ template <int DT, int RB, int GM> struct W4Step {
 	{
 		if (step >= a.steps)
 			step = a.steps - 1;	/* (loaded, not used) */
+		const int esize = X == W4_X_I8 ? (a.dtype == THHIP_F32 ? 4 : 2) : (int)sizeof(T);
 #pragma unroll
 		for (int r = 0; r < RB; r++) {
 			const int rb = rb0 + r < a.blocks ? rb0 + r : a.blocks - 1;
 			codes[r] = *(const uintx4 *)(a.codes + ((size_t)rb * a.steps + step) * 1024 + lane * 16);
 #pragma unroll
 			for (int j = 0; j < 4 / GM; j++) {
-				const size_t at = ((size_t)rb * a.groups + a.group_of(step, j * GM)) * 16 + 4 * (lane >> 4);
-				s[r][j] = *(const T4 *)((const typename ThhipElem<DT>::T *)a.scales + at);
-				if (a.zeros)
-					z[r][j] = *(const unsigned *)(a.zeros + at);
+				const size_t at = ((size_t)rb * a.groups + a.group_of(step, j * GM)) * 16;
+				s[r][j] = *(const U4 *)((const char *)a.scales + at * esize + (lane >> 4) * 4 * esize);
+				if constexpr (ZP)
+					z[r][j] = *(const unsigned *)(a.zeros + at + (lane >> 4) * 4);
 			}
 		}
 	}
+	__device__ __forceinline__ float scale(const w4_args &a, int r, int j, int i) const
+	{
+		if constexpr (X != W4_X_I8)
+			return (float)s[r][j][i];
+		else {
+			const unsigned h = __float_as_uint(s[r][j][i / 2]) >> (16 * (i & 1));
+			const float f16 = (float)__builtin_bit_cast(_Float16, (unsigned short)h);
+			return a.dtype == THHIP_F32 ? s[r][j][i] : a.dtype == THHIP_F16 ? f16 : __uint_as_float(h << 16);
+		}
+	}
+	__device__ __forceinline__ float zero(int r, int j, int i) const
+	{
+		return ZP ? (float)((z[r][j] >> (8 * i)) & 255) : 8.0f;
+	}
 };
 
-template <int X, int DT, int RB, int NB, int GM, int W, int D>
+template <int X, int RB, int NB, int XV, int GM, bool ZP, int W, int D, bool EDGE>
 __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args a)
 {
 	typedef W4X<X> K;
 	typedef typename K::V V;
 	typedef typename K::A A;
+	typedef W4Step<X, RB, GM, ZP> Step;
 	constexpr int ES = sizeof(V) / 8;		/* bytes of an operand's element */
 	constexpr int T = W * 64, ROWV = W * 16;	/* threads; vectors of eight in a row's chunk */
-	constexpr int STRIDE = W * W4_KSTEP * ES + 16;
-	constexpr int XV = (4 * NB + K::PARTS - 1) / K::PARTS;	/* vectors a thread puts down a chunk */
+	constexpr int CK = W * W4_KSTEP;		/* k of a chunk */
+	constexpr int STRIDE = CK * ES + 16;
 	extern __shared__ __align__(16) unsigned char lds[];
 	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int col = lane & 15, quarter = lane >> 4;
 	const int rb0 = blockIdx.x * RB;
-	const int cols = a.B * K::PARTS, buf = cols * STRIDE, nvec = a.B * ROWV;
+	const int cols = a.B * K::PARTS, buf = cols * STRIDE;
 	const int chunks = (a.steps + W - 1) / W;
 
-	typename K::E xr[XV][8];
+	/* x of a chunk on its way to LDS: vector tid + i * T of the workgroup's, in the order of the rows.  A vector
+	 * behind its row or the batch is pointed past the buffer and reads as zeros (EDGE: see w4_fetch_x) */
+	typename K::E8 xr[XV];
+	auto x_row = [&](int i) { return (tid + i * T) / ROWV; };
 	auto load_x = [&](int c) {
+		const int k = c * CK + tid % ROWV * 8;
+		if constexpr (EDGE)
+			w4_fetch_x<X>(xr, a.x, a.ldx, a.nIn, [&](int i) { return (long)(x_row(i) < a.B ? x_row(i) : a.B - 1); }, [&](int) { return k; });
+		else {
+			constexpr int EX = sizeof(typename K::E);
+			const __amdgpu_buffer_rsrc_t xrsrc = __builtin_amdgcn_make_buffer_rsrc((void *)a.x, 0, 0x7fffffff, 0x00020000);
 #pragma unroll
-		for (int i = 0; i < XV; i++) {
-			const int v = tid + i * T;
-			if (v < nvec)
-				w4_load_x<X>(a.x, (v / ROWV) * a.ldx, (long)c * W * W4_KSTEP + v % ROWV * 8, a.nIn, xr[i]);
+			for (int i = 0; i < XV; i++) {
+				const unsigned at = x_row(i) < a.B && k < a.nIn ? (unsigned)((x_row(i) * (int)a.ldx + k) * EX) : 0x80000000u;
+				if constexpr (EX == 1)
+					xr[i] = __builtin_bit_cast(typename K::E8, __builtin_amdgcn_raw_buffer_load_b64(xrsrc, at, 0, 0));
+				else if constexpr (EX == 2)
+					xr[i] = __builtin_bit_cast(typename K::E8, __builtin_amdgcn_raw_buffer_load_b128(xrsrc, at, 0, 0));
+				else {
+					struct { uintx4 lo, hi; } v = {__builtin_amdgcn_raw_buffer_load_b128(xrsrc, at, 0, 0),
+						__builtin_amdgcn_raw_buffer_load_b128(xrsrc, at, 16, 0)};
+					xr[i] = __builtin_bit_cast(typename K::E8, v);
+				}
+			}
 		}
 	};
-	auto store_x = [&](int b) {
+	auto store_x = [&](int c) {
+		if (EDGE && (c + 1) * CK > a.nIn)
+			w4_fix_x<X>(xr, a.nIn, [&](int) { return c * CK + tid % ROWV * 8; });
 #pragma unroll
-		for (int i = 0; i < XV; i++) {
-			const int v = tid + i * T;
-			if (v < nvec) {
+		for (int i = 0; i < XV; i++)
+			if (x_row(i) < a.B) {
 				V o[K::PARTS];
 				K::operand(xr[i], o);
 #pragma unroll
 				for (int p = 0; p < K::PARTS; p++)
-					*(V *)(lds + b * buf + (v / ROWV * K::PARTS + p) * STRIDE + v % ROWV * 8 * ES) = o[p];
+					*(V *)(lds + (c & 1) * buf + (x_row(i) * K::PARTS + p) * STRIDE + tid % ROWV * 8 * ES) = o[p];
 			}
-		}
 	};
 	/* where a lane's operands lie: in either buffer, or among the zeros */
 	int at[2][NB];
@@ -311,16 +349,17 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args a)
 		for (int n = 0; n < NB; n++)
 			acc[r][n] = (floatx4)0.0f;
 
-	W4Step<DT, RB, GM> st[D];
+	Step st[D];
+	/* (in the order in which the loop asks for them, so that its waits fit the first time round too) */
 	load_x(0);
 #pragma unroll
-	for (int d = 0; d < D; d++)
+	for (int d = 0; d < D - 1; d++)
 		st[d].fetch(a, rb0, d * W + wave, lane);
 	if (tid < 32 * ES)
 		((unsigned *)(lds + 2 * buf))[tid] = 0;
 	store_x(0);
-	if (chunks > 1)
-		load_x(1);
+	load_x(1);
+	st[D - 1].fetch(a, rb0, (D - 1) * W + wave, lane);
 	w4_lds_barrier();
 
 	constexpr int U = D % 2 ? 2 * D : D;	/* chunks after which buffers and stages are the first again */
@@ -330,12 +369,10 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args a)
 			const int c = c0 + u;
 			if (c >= chunks)
 				break;
-			if (c + 1 < chunks)
-				store_x((u + 1) & 1);
-			if (c + 2 < chunks)
-				load_x(c + 2);
+			store_x(c + 1);		/* (behind K's end: zeros, which nobody reads) */
+			load_x(c + 2);
 			const int step = c * W + wave;
-			W4Step<DT, RB, GM> &now = st[u % D];
+			Step &now = st[u % D];
 			if (step < a.steps) {
 				A p[RB][NB], sx[NB];
 #pragma unroll
@@ -347,7 +384,7 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args a)
 #pragma unroll
 					for (int n = 0; n < NB; n++) {
 						const V x = *(const V *)(lds + at[u & 1][n] + j * 32 * ES);
-						if (X != W4_X_I8 || a.zeros)
+						if constexpr (X != W4_X_I8 || ZP)
 							sx[n] = K::mma(K::ones(), x, j % GM ? sx[n] : (A)0);
 #pragma unroll
 						for (int r = 0; r < RB; r++)
@@ -355,25 +392,29 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args a)
 					}
 					if ((j + 1) % GM)
 						continue;
+					float xs[NB];
 #pragma unroll
 					for (int n = 0; n < NB; n++) {
-						float xs = X == W4_X_I8 ? 0.0625f : 1.0f;
-						if (X == W4_X_I8 && a.xgroups > 1) {
+						xs[n] = 1.0f;
+						if constexpr (X == W4_X_I8) {
 							const int b = n * 16 + col;
-							xs *= a.xscale[(long)(b < a.B ? b : 0) * a.xgroups + a.group_of(step, j)];
+							const float v = a.xscale[(long)(b < a.B ? b : 0) * a.xgroups + (a.xgroups > 1 ? a.group_of(step, j) : 0)];
+							xs[n] = 0.0625f * (a.xgroups > 1 ? v : 1.0f);
 						}
+					}
 #pragma unroll
-						for (int r = 0; r < RB; r++)
+					for (int r = 0; r < RB; r++)
 #pragma unroll
-							for (int i = 0; i < 4; i++) {
-								const float s = (float)now.s[r][j / GM][i] * xs;
-								const float z = a.zeros ? (float)((now.z[r][j / GM] >> (8 * i)) & 255) : 8.0f;
+						for (int i = 0; i < 4; i++) {
+							const float s = now.scale(a, r, j / GM, i), z = now.zero(r, j / GM, i);
+#pragma unroll
+							for (int n = 0; n < NB; n++) {
 								if constexpr (X == W4_X_I8)
-									acc[r][n][i] += s * ((float)p[r][n][i] - (a.zeros ? (16.0f * z - 128.0f) * (float)sx[n][i] : 0.0f));
+									acc[r][n][i] += s * xs[n] * ((float)p[r][n][i] - (ZP ? (16.0f * z - 128.0f) * (float)sx[n][i] : 0.0f));
 								else
 									acc[r][n][i] += s * (p[r][n][i] - z * sx[n][i]);
 							}
-					}
+						}
 				}
 			}
 			now.fetch(a, rb0, step + D * W, lane);
@@ -405,11 +446,11 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args a)
 		y += a.bias ? a.bias[o] : 0.0f;
 		if (a.act)
 			y = y > a.thr ? y : a.val;
-		ThhipElem<DT>::st(a.y, b * a.ldy + o, y);
+		w4_put<X>(a.y, b * a.ldy + o, y, a.dtype);
 	}
 }
 
-template <int X, int DT, int RB, int NB, int GM, int W, int D>
+template <int X, int RB, int NB, int XV, int GM, bool ZP, int W, int D, bool EDGE>
 static void w4_skinny_launch(const w4_args &a)
 {
 	typedef W4X<X> K;
@@ -419,45 +460,58 @@ static void w4_skinny_launch(const w4_args &a)
 	lds = lds > red ? lds : red;
 	static bool raised;
 	if (!raised) {
-		hipcheck(hipFuncSetAttribute((const void *)w4_skinny_kernel<X, DT, RB, NB, GM, W, D>,
+		hipcheck(hipFuncSetAttribute((const void *)w4_skinny_kernel<X, RB, NB, XV, GM, ZP, W, D, EDGE>,
 			hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
 		raised = true;
 	}
-	w4_skinny_kernel<X, DT, RB, NB, GM, W, D><<<dim3((a.blocks + RB - 1) / RB), dim3(W * 64), lds, thhip_stream()>>>(a);
+	w4_skinny_kernel<X, RB, NB, XV, GM, ZP, W, D, EDGE><<<dim3((a.blocks + RB - 1) / RB), dim3(W * 64), lds, thhip_stream()>>>(a);
 }
 
 /* Up to 64 columns */
-template <int X, int DT, int GM>
+template <int X, int GM, bool ZP>
 static void w4_skinny(const w4_args &a)
 {
 	constexpr int P = W4X<X>::PARTS;
-	constexpr size_t esx = sizeof(typename W4X<X>::E), esy = sizeof(typename ThhipElem<DT>::T);
-	for (int b0 = 0; b0 < a.B; b0 += 64 / P) {
-		const w4_args s = w4_rows(a, b0, a.B - b0 < 64 / P ? a.B - b0 : 64 / P, esx, esy);
-		if (s.B * P <= 16) {
-			if (g_w4_tuning == 1 || (!g_w4_tuning && s.blocks < 1024))
-				w4_skinny_launch<X, DT, 1, 1, GM, 16, 2>(s);
-			else if (g_w4_tuning == 3)
-				w4_skinny_launch<X, DT, 1, 1, GM, 8, 3>(s);
-			else
-				w4_skinny_launch<X, DT, 2, 1, GM, 8, 2>(s);
-		} else if (s.B * P <= 32)
-			w4_skinny_launch<X, DT, 1, 2, GM, 8, 2>(s);
+	constexpr size_t esx = sizeof(typename W4X<X>::E);
+	/* vectors a thread moves a chunk for 4, 16, 32, 64 columns: four rows each */
+	constexpr int X1 = (16 / P + 3) / 4, X2 = (32 / P + 3) / 4, X4 = (64 / P + 3) / 4;
+	const int cols = a.B * P;
+	/* rows of whole vectors on whole words, within the reach of a buffer descriptor */
+	const bool edge = a.nIn % 8 || (uintptr_t)a.x % 4 || a.ldx * esx % 4 || a.ldx * esx * a.B >= 1u << 31;
+	if (edge) {
+		if (cols <= 16)
+			w4_skinny_launch<X, 1, 1, X1, GM, ZP, 8, 2, true>(a);
+		else if (cols <= 32)
+			w4_skinny_launch<X, 1, 2, X2, GM, ZP, 8, 2, true>(a);
 		else
-			w4_skinny_launch<X, DT, 1, 4, GM, 4, 2>(s);
-	}
+			w4_skinny_launch<X, 1, 4, X4, GM, ZP, 4, 2, true>(a);
+	} else if (cols <= 16) {
+		const bool wide = g_w4_tuning ? g_w4_tuning == 2 : a.blocks >= 1024;
+		if (a.B <= 4) {
+			if (wide)
+				w4_skinny_launch<X, 2, 1, 1, GM, ZP, 8, 2, false>(a);
+			else
+				w4_skinny_launch<X, 1, 1, 1, GM, ZP, 16, 2, false>(a);
+		} else if (wide)
+			w4_skinny_launch<X, 2, 1, X1, GM, ZP, 8, 2, false>(a);
+		else
+			w4_skinny_launch<X, 1, 1, X1, GM, ZP, 16, 2, false>(a);
+	} else if (cols <= 32)
+		w4_skinny_launch<X, 1, 2, X2, GM, ZP, 8, 2, false>(a);
+	else
+		w4_skinny_launch<X, 1, 4, X4, GM, ZP, 4, 2, false>(a);
 }
 
-template <int X, int DT>
+template <int X>
 static void w4_choose(const w4_args &a)
 {
-	const bool tile = a.B * W4X<X>::PARTS > 64;
+	const bool tile = a.B * W4X<X>::PARTS > 64, small = a.group == 32 || a.group == 64;
 	if (tile)
 		w4_tile(a, X);
-	else if (a.group == 32 || a.group == 64)
-		w4_skinny<X, DT, 1>(a);
+	else if (a.zeros)
+		small ? w4_skinny<X, 1, true>(a) : w4_skinny<X, 4, true>(a);
 	else
-		w4_skinny<X, DT, 4>(a);
+		small ? w4_skinny<X, 1, false>(a) : w4_skinny<X, 4, false>(a);
 }
 
 static int w4_run(const char *who, w4_args &a, const void *packed, int group, int zeros, int xkind, int xgroup, int dtype)
@@ -497,9 +551,9 @@ static int w4_run(const char *who, w4_args &a, const void *packed, int group, in
 	ThhipLaunchScope scope(THHIP_FAM_GEMV, (double)a.nOut * a.nIn / 2 + (double)a.nOut * l.groups * (es + (zeros ? 1 : 0)) +
 		(double)a.B * a.nIn * esx + (double)a.B * a.nOut * es);
 	if (xkind == W4_X_I8)
-		THHIP_DISPATCH_FLOAT(dtype, (w4_choose<W4_X_I8, DT>(a)));
+		w4_choose<W4_X_I8>(a);
 	else
-		THHIP_DISPATCH_FLOAT(dtype, (w4_choose<DT, DT>(a)));
+		THHIP_DISPATCH_FLOAT(dtype, (w4_choose<DT>(a)));
 	return 0;
 }
 

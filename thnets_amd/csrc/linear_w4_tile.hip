@@ -52,8 +52,7 @@ template <> struct W4Tile<W4_X_I8, true> {		/* 8-bit operands of 64 k: two of 32
 
 #define W4_LDS(p) ((__attribute__((address_space(3))) void *)(p))
 
-/* Scales and results in the layer's type, which only the ends of the tile kernel see: that of x, or, where x is
- * 8-bit, known when the kernel runs */
+/* A scale, in the type of x or, where x is 8-bit, in the one the call names */
 template <int X>
 __device__ __forceinline__ float w4_get(const void *p, long i, int dtype)
 {
@@ -64,19 +63,6 @@ __device__ __forceinline__ float w4_get(const void *p, long i, int dtype)
 		const float h = (float)__builtin_bit_cast(_Float16, (unsigned short)u);
 		return dtype == THHIP_F16 ? h : __uint_as_float(dtype == THHIP_F32 ? u : u << 16);
 	}
-}
-
-template <int X>
-__device__ __forceinline__ void w4_put(void *p, long i, float v, int dtype)
-{
-	if constexpr (X != W4_X_I8)
-		ThhipElem<X>::st(p, i, v);
-	else if (dtype == THHIP_F32)
-		ThhipElem<THHIP_F32>::st(p, i, v);
-	else if (dtype == THHIP_F16)
-		ThhipElem<THHIP_F16>::st(p, i, v);
-	else
-		ThhipElem<THHIP_BF16>::st(p, i, v);
 }
 
 template <int X, int GM, bool ZP, bool DMA>
@@ -117,7 +103,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 	const typename K::E *xbase = (const typename K::E *)a.x + (long)b0 * a.ldx;
 	const unsigned xend = DMA ? (unsigned)(((nrows - 1) * a.ldx + a.nIn) * (long)sizeof(typename K::E)) : 0;
 	const __amdgpu_buffer_rsrc_t xrsrc = __builtin_amdgcn_make_buffer_rsrc((void *)xbase, 0, xend, 0x00020000);
-	typename K::E xr[DMA ? 1 : PIECES / 2][8];
+	typename K::E8 xr[DMA ? 1 : PIECES / 2];
 
 	/* x of step t on its way (half: one of the two halves that go through registers one after the other) */
 	auto x_issue = [&](int t, int buf, int half) {
@@ -132,20 +118,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 					k < a.nIn * ES ? (unsigned)(r0 * (int)a.ldx * ES + k) : 0x80000000u, i * 4 * RPI * (int)a.ldx * ES, 0, 0);
 			}
 		} else {
-#pragma unroll
-			for (int i = 0; i < PIECES / 2; i++) {
-				const int p = tid + (half * (PIECES / 2) + i) * 256, r = p >> 4;
-				if (r < nrows)
-					w4_load_x<X>(xbase, r * a.ldx, (long)t * W4_KSTEP + (p & 15) * 8, a.nIn, xr[i]);
-				else
-#pragma unroll
-					for (int e = 0; e < 8; e++)
-						xr[i][e] = (typename K::E)0;
-			}
+			w4_fetch_x<X>(xr, xbase, a.ldx, a.nIn, [&](int i) {
+				const int r = (tid + (half * (PIECES / 2) + i) * 256) >> 4;
+				return (long)(r < nrows ? r : nrows - 1);
+			}, [&](int i) { return t * W4_KSTEP + (tid & 15) * 8; });
 		}
 	};
-	auto x_land = [&](int buf, int half) {
+	auto x_land = [&](int t, int buf, int half) {
 		if constexpr (!DMA) {
+			if ((t + 1) * W4_KSTEP > a.nIn)
+				w4_fix_x<X>(xr, a.nIn, [&](int i) { return t * W4_KSTEP + (tid & 15) * 8; });
 #pragma unroll
 			for (int i = 0; i < PIECES / 2; i++) {
 				const int p = tid + (half * (PIECES / 2) + i) * 256, r = p >> 4, v = p & 15;
@@ -199,10 +181,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 			acc[r][n] = (floatx4)0.0f;
 
 	x_issue(0, 0, 0);
-	x_land(0, 0);
+	x_land(0, 0, 0);
 	if (!DMA) {
 		x_issue(0, 0, 1);
-		x_land(0, 1);
+		x_land(0, 0, 1);
 	}
 	codes_issue(0);
 	g_issue(0);
@@ -270,7 +252,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 			asm volatile("" ::: "memory");	/* (operands and scales are read again for every unit, not kept) */
 			__builtin_amdgcn_sched_barrier(0);
 			if (!DMA && u == NU / 2) {
-				x_land(buf ^ 1, 0);
+				x_land(t1, buf ^ 1, 0);
 				x_issue(t1, buf ^ 1, 1);
 			}
 			if (g == 0 && n + 1 < NB)
@@ -314,7 +296,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 		}
 		__builtin_amdgcn_sched_barrier(0);
 		flush(NU - 1);
-		x_land(buf ^ 1, DMA ? 0 : 1);
+		x_land(t1, buf ^ 1, DMA ? 0 : 1);
 		g_land(buf ^ 1);
 		barrier();
 	}

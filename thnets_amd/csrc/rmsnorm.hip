@@ -15,9 +15,9 @@
  * sum of squares (and largest |h w|) goes through the wavefronts, and written once.
  * h stays in fp32 between the addition and the norm, so the norm is that of the
  * unrounded sum, and y is rounded once.  Codes do not depend on the root, only on
- * h w and its maximum; their quotient is taken in 64 bits (full rate here, and the
- * kernels wait for memory), so that a value next to the middle between two codes goes
- * to the nearer one: with fp32 quotients one value in 30000 of fp16 rows did not.
+ * h w and its maximum; where the fp32 quotient is next to the middle between two
+ * codes it is taken again in 64 bits, so that the value goes to the nearer one: without
+ * that one value in 30000 of fp16 rows did not.
  */
 #include <stdint.h>
 #include <stdio.h>
@@ -33,29 +33,51 @@ struct rows_args {
 	float *scale;
 	long ldx, ldr, lds, ldy, ldq;
 	long rows;
-	int cols, group, ngroups;
+	int cols, group, ngroups, ragged;
 	float eps;
 };
 
-/* N consecutive elements of a row (16 bytes): one load / store, which needs no more than the element's
- * alignment here, or one by one where the row ends among them; elements past the row read as 0 */
+/* N consecutive elements of a row (16 bytes), which need no more than the element's alignment here.
+ * fetch() loads without a branch, so that all of a thread's loads are on their way together: a vector that the
+ * row's end cuts or that lies behind it is read from the row's last N elements (cols >= N), and widen() puts
+ * it right afterwards, elements past the end being 0.  A branch round each load made the compiler wait for one before
+ * the next: 2.5 times the time of a row of 4096. */
 template <int DT> struct RowVec {
 	static constexpr int N = DT == THHIP_F32 ? 4 : 8;
 	typedef typename ThhipElem<DT>::T T;
 	typedef T V __attribute__((ext_vector_type(N)));
 	typedef V U __attribute__((aligned(sizeof(T))));
-	static __device__ __forceinline__ void load(const void *p, long base, int col, int cols, float *out)
+	static __device__ __forceinline__ V fetch(const void *p, long base, int col, int cols)
 	{
-		if (col + N <= cols) {
-			const V v = *(const U *)((const T *)p + base + col);
+		return *(const U *)((const T *)p + base + (col < cols - N ? col : cols - N));
+	}
+	/* ragged: the row has vectors that fetch() moved */
+	static __device__ __forceinline__ void widen(const V v, int col, int cols, int ragged, float *out)
+	{
+#pragma unroll
+		for (int i = 0; i < N; i++)
+			out[i] = (float)v[i];
+		if (ragged) {
+			const int by = col > cols - N ? col - (cols - N) : 0;
+#pragma unroll
+			for (int b = 1; b < N; b *= 2)
+#pragma unroll
+				for (int i = 0; i < N; i++)
+					out[i] = by & b ? (i + b < N ? out[i + b] : 0.0f) : out[i];
 #pragma unroll
 			for (int i = 0; i < N; i++)
-				out[i] = (float)v[i];
-		} else {
+				out[i] = by >= N ? 0.0f : out[i];
+		}
+	}
+	/* the same for rows of any length */
+	static __device__ __forceinline__ void load(const void *p, long base, int col, int cols, float *out)
+	{
+		if (col + N <= cols)
+			widen(*(const U *)((const T *)p + base + col), col, cols, 0, out);
+		else
 #pragma unroll
 			for (int i = 0; i < N; i++)
 				out[i] = col + i < cols ? ThhipElem<DT>::ld(p, base + col + i) : 0.0f;
-		}
 	}
 	static __device__ __forceinline__ void store(void *p, long base, int col, int cols, const float *in)
 	{
@@ -74,49 +96,66 @@ template <int DT> struct RowVec {
 	}
 };
 
-/* What a row's or group's values become codes by: step = top / 127 and its reciprocal.  top is the largest
- * |h w|, top * rstd the largest |y|: below 2^-116 (where an fp32 scale loses bits) it counts as nothing,
- * reciprocal 0, codes 0. */
+/* What a row's or group's values become codes by.  top is the largest |h w|, top * rstd the largest |y|: below
+ * 2^-116 (where an fp32 scale loses bits) it counts as nothing, reciprocal 0, codes 0. */
 struct code_step {
-	double step, inv;
+	float top, inv;		/* inv: 127 / top, off by at most 1.5 units */
 };
 
 __device__ __forceinline__ struct code_step code_step_of(float top, float rstd)
 {
 	struct code_step c;
-	c.step = (double)top / 127.0;
-	c.inv = top * rstd < 1.2e-35f ? 0.0 : 1.0 / c.step;	/* (a NaN stays one) */
+	c.top = top;
+	c.inv = top * rstd < 1.2e-35f ? 0.0f : 127.0f * __builtin_amdgcn_rcpf(top);	/* (a NaN stays one) */
 	return c;
 }
 
+/* The codes of N values v * w.  Adding 1.5 * 2^23 leaves the nearest whole number in the sum's low bits.  The product v * w
+ * and the reciprocal are off by at most 2^-24 and 3 * 2^-24, that is 3e-5 of a code at 127: a quotient that is
+ * further than 2^-14 from a middle between two codes has its nearest one. */
 template <int N>
-__device__ __forceinline__ void store_codes(signed char *p, long base, int col, int cols, const double *v, const struct code_step c)
+__device__ __forceinline__ void store_codes(signed char *p, long base, int col, int cols, const float *v, const float *w,
+	const struct code_step c)
 {
 	typedef unsigned W __attribute__((ext_vector_type(N / 4), aligned(1)));
-	unsigned w[N / 4];
-#pragma unroll
-	for (int i = 0; i < N / 4; i++)
-		w[i] = 0;
+	const float whole = 12582912.0f;
+	unsigned o[N / 4], u[N];
+	float off = 0;
 #pragma unroll
 	for (int i = 0; i < N; i++) {
-		/* v / step, rounded once: the quotient's own error, times the reciprocal, put right */
-		double t = v[i] * c.inv;
-		t = fma(fma(-t, c.step, v[i]), c.inv, t);
-		const int n = (int)rint(t), q = n > 127 ? 127 : n < -127 ? -127 : n;	/* (NaN: 0) */
-		w[i / 4] |= ((unsigned)q & 255u) << (8 * (i % 4));
+		const float x = v[i] * w[i], y = fmaf(x, c.inv, whole);
+		off = fmaxf(off, fabsf(fmaf(x, c.inv, whole - y)));
+		u[i] = __float_as_uint(y);
 	}
+	if (off > 0.5f - 0x1p-14f && c.inv > 0) {
+		/* v * w / step in 64 bits, by the reciprocal and what the product says is left */
+		const double step = (double)c.top * (1.0 / 127.0);
+		double inv = __builtin_amdgcn_rcp(step);
+		inv = fma(fma(-step, inv, 1.0), inv, inv);
+		inv = fma(fma(-step, inv, 1.0), inv, inv);
+#pragma unroll
+		for (int i = 0; i < N; i++) {
+			const double x = (double)v[i] * (double)w[i], y = x * inv;
+			const int n = (int)rint(fma(fma(-y, step, x), inv, y));
+			u[i] = (unsigned)(n > 127 ? 127 : n < -127 ? -127 : n);
+		}
+	}
+#pragma unroll
+	for (int i = 0; i < N / 4; i++)
+		o[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[4 * i + 3], u[4 * i + 2], 0x0c0c0400),
+			__builtin_amdgcn_perm(u[4 * i + 1], u[4 * i], 0x0c0c0400), 0x05040100);
 	if (col + N <= cols) {
-		W o;
+		W r;
 		if constexpr (N == 8)
-			o = (W){w[0], w[1]};
+			r = (W){o[0], o[1]};
 		else
-			o = (W)w[0];
-		*(W *)(p + base + col) = o;
-	} else {
+			r = (W)o[0];
+		*(W *)(p + base + col) = r;
+	} else if (col < cols) {
 #pragma unroll
 		for (int i = 0; i < N; i++)
 			if (col + i < cols)
-				p[base + col + i] = (signed char)(w[i / 4] >> (8 * (i % 4)));
+				p[base + col + i] = (signed char)u[i];
 	}
 }
 
@@ -129,21 +168,48 @@ __device__ __forceinline__ unsigned abs_bits(float v)
 
 __device__ __forceinline__ float code_scale(float top)
 {
-	return top < 1.2e-35f ? 0.0f : top / 127.0f;
+	const float s = top * (1.0f / 127.0f);
+	return top < 1.2e-35f ? 0.0f : top < INFINITY ? fmaf(fmaf(-s, 127.0f, top), 1.0f / 127.0f, s) : s;
 }
 
+/* v of the lane that differs in bits `by` of its number (by = 1, 2), that is mirrored in its half row of 8 lanes (4) or row
+ * of 16 (8), or in the other row or half of the wavefront (16, 32): a butterfly over `by` leaves every lane of a
+ * group of lanes with the group's sum or maximum.  Moves between registers; through LDS (shuffles) a
+ * row of 4096 took 0.1 to 0.3 us longer, of 3. */
+template <int BY>
+__device__ __forceinline__ unsigned lane_across(unsigned v)
+{
+	if constexpr (BY == 1)
+		return __builtin_amdgcn_update_dpp(v, v, 0xb1, 0xf, 0xf, false);	/* quad_perm 1 0 3 2 */
+	else if constexpr (BY == 2)
+		return __builtin_amdgcn_update_dpp(v, v, 0x4e, 0xf, 0xf, false);	/* quad_perm 2 3 0 1 */
+	else if constexpr (BY == 4)
+		return __builtin_amdgcn_update_dpp(v, v, 0x141, 0xf, 0xf, false);	/* row_half_mirror */
+	else if constexpr (BY == 8)
+		return __builtin_amdgcn_update_dpp(v, v, 0x140, 0xf, 0xf, false);	/* row_mirror */
+	else {
+		/* swaps the odd rows (16) / upper half (32) of the first with the even rows / lower half of the second */
+		const auto p = BY == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+		return threadIdx.x & BY ? p[0] : p[1];
+	}
+}
+
+template <int BY = 32>
 __device__ __forceinline__ float lanes_sum(float v)
 {
-#pragma unroll
-	for (int off = 32; off > 0; off >>= 1)
-		v += __shfl_xor(v, off, 64);
-	return v;
+	if constexpr (BY > 1)
+		v = lanes_sum<BY / 2>(v);
+	return v + __uint_as_float(lane_across<BY>(__float_as_uint(v)));
 }
 
+/* over groups of `lanes` lanes (a power of two, uniform) */
+template <int BY = 32>
 __device__ __forceinline__ unsigned lanes_max(unsigned v, int lanes)
 {
-	for (int off = lanes >> 1; off > 0; off >>= 1) {
-		const unsigned o = __shfl_xor(v, off, 64);
+	if constexpr (BY > 1)
+		v = lanes_max<BY / 2>(v, lanes);
+	if (BY < lanes) {
+		const unsigned o = lane_across<BY>(v);
 		v = o > v ? o : v;
 	}
 	return v;
@@ -187,15 +253,11 @@ __device__ __forceinline__ void row_out(const rows_args &a, long row, int col, c
 			y[i] = h[i] * rstd * w[i];
 		RowVec<DT>::store(a.y, row * a.ldy, col, a.cols, y);
 	} else {
-		double v[N];
-#pragma unroll
-		for (int i = 0; i < N; i++)
-			v[i] = MODE == ROWS_QUANT ? (double)h[i] : (double)h[i] * (double)w[i];
 		if (a.group) {
 			unsigned m = 0;
 #pragma unroll
 			for (int i = 0; i < N; i++) {
-				const unsigned b = abs_bits((float)v[i]);
+				const unsigned b = abs_bits(MODE == ROWS_QUANT ? h[i] : h[i] * w[i]);
 				m = b > m ? b : m;
 			}
 			m = lanes_max(m, a.group / N);
@@ -204,7 +266,7 @@ __device__ __forceinline__ void row_out(const rows_args &a, long row, int col, c
 			if (col < a.cols && col % a.group == 0)
 				a.scale[row * a.ngroups + col / a.group] = code_scale(top * rstd);
 		}
-		store_codes<N>(a.q, row * a.ldq, col, a.cols, v, step);
+		store_codes<N>(a.q, row * a.ldq, col, a.cols, h, w, step);
 	}
 }
 
@@ -218,33 +280,45 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const rows_args
 	const long row = (long)blockIdx.x * RPG + threadIdx.x / T;
 	if (RPG > 1 && row >= a.rows)	/* (whole wavefronts: T = 64) */
 		return;
-	float h[V][N], w[V][N];
+	typedef RowVec<DT> R;
+	typedef RowVec<THHIP_F32> R4;
+	typename R::V rx[V], rr[V];
+	typename R4::V rw[V][N / 4];
 #pragma unroll
 	for (int v = 0; v < V; v++)
-		RowVec<DT>::load(a.x, row * a.ldx, (v * T + t) * N, a.cols, h[v]);
-	if (a.res) {
+		rx[v] = R::fetch(a.x, row * a.ldx, (v * T + t) * N, a.cols);
+	if (a.res)
 #pragma unroll
-		for (int v = 0; v < V; v++) {
+		for (int v = 0; v < V; v++)
+			rr[v] = R::fetch(a.res, row * a.ldr, (v * T + t) * N, a.cols);
+	if (MODE != ROWS_QUANT && a.w)
+#pragma unroll
+		for (int v = 0; v < V; v++)
+#pragma unroll
+			for (int i = 0; i < N / 4; i++)
+				rw[v][i] = R4::fetch(a.w, 0, (v * T + t) * N + 4 * i, a.cols);
+	float h[V][N], w[V][N];
+#pragma unroll
+	for (int v = 0; v < V; v++) {
+		if (v && v * T * N >= a.cols)	/* (the whole vector lies behind the row) */
+			break;
+		const int col = (v * T + t) * N;
+		R::widen(rx[v], col, a.cols, a.ragged, h[v]);
+		if (a.res) {
 			float r[N];
-			RowVec<DT>::load(a.res, row * a.ldr, (v * T + t) * N, a.cols, r);
+			R::widen(rr[v], col, a.cols, a.ragged, r);
 #pragma unroll
 			for (int i = 0; i < N; i++)
 				h[v][i] += r[i];
 		}
-	}
-	if constexpr (MODE != ROWS_QUANT) {
+		if (MODE != ROWS_QUANT && a.w) {
 #pragma unroll
-		for (int v = 0; v < V; v++) {
-			const int col = (v * T + t) * N;
-			if (a.w) {
-				RowVec<THHIP_F32>::load(a.w, 0, col, a.cols, w[v]);
-				if constexpr (N == 8)
-					RowVec<THHIP_F32>::load(a.w, 0, col + 4, a.cols, w[v] + 4);
-			} else {
+			for (int i = 0; i < N / 4; i++)
+				R4::widen(rw[v][i], col + 4 * i, a.cols, a.ragged, w[v] + 4 * i);
+		} else {
 #pragma unroll
-				for (int i = 0; i < N; i++)
-					w[v][i] = 1.0f;
-			}
+			for (int i = 0; i < N; i++)
+				w[v][i] = 1.0f;
 		}
 	}
 	float s = 0, rstd = 1;
@@ -252,6 +326,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const rows_args
 	unsigned m = 0;
 #pragma unroll
 	for (int v = 0; v < V; v++) {
+		if (v && v * T * N >= a.cols)
+			break;
 #pragma unroll
 		for (int i = 0; i < N; i++) {
 			if constexpr (MODE != ROWS_QUANT)
@@ -275,6 +351,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const rows_args
 	}
 #pragma unroll
 	for (int v = 0; v < V; v++) {
+		if (v && v * T * N >= a.cols)
+			break;
 		const int col = (v * T + t) * N;
 		if (a.sum)
 			RowVec<DT>::store(a.sum, row * a.lds, col, a.cols, h[v]);
@@ -282,7 +360,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const rows_args
 	}
 }
 
-/* Rows longer than the registers hold: the sum (and maximum) first, then the row again.  A thread
+/* Rows longer than the registers hold, or shorter than a vector: the sum (and maximum) first, then the row again.  A thread
  * reads an element of x and res in the second walk before it writes the same element, so the outputs
  * may be the inputs here too. */
 template <int DT, int MODE>
@@ -337,17 +415,18 @@ __global__ __launch_bounds__(1024) void rows_long_kernel(const rows_args a)
 }
 
 template <int DT, int MODE, int T, int V>
-static bool rows_try(const rows_args &a)
+static bool rows_try(rows_args &a)
 {
-	if (a.cols > T * V * RowVec<DT>::N)
+	if (a.cols > T * V * RowVec<DT>::N || a.cols < RowVec<DT>::N)
 		return false;
+	a.ragged = a.cols != T * V * RowVec<DT>::N;
 	constexpr int RPG = T < 256 ? 256 / T : 1;
 	rows_kernel<DT, MODE, T, V><<<dim3((unsigned)((a.rows + RPG - 1) / RPG)), dim3(T < 256 ? 256 : T), 0, thhip_stream()>>>(a);
 	return true;
 }
 
 template <int DT, int MODE>
-static void rows_launch(const rows_args &a)
+static void rows_launch(rows_args &a)
 {
 	if (rows_try<DT, MODE, 64, 1>(a) || rows_try<DT, MODE, 64, 2>(a) || rows_try<DT, MODE, 256, 1>(a) ||
 	    rows_try<DT, MODE, 256, 2>(a) || rows_try<DT, MODE, 256, 4>(a) || rows_try<DT, MODE, 256, 8>(a) ||
