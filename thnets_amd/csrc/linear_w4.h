@@ -120,20 +120,27 @@ template <> struct W4X<W4_X_I8> {
 	static __device__ __forceinline__ void operand(const E8 x, V *out) { out[0] = __builtin_bit_cast(V, x); }
 };
 
-/* Vectors of eight elements of x that may begin anywhere and end behind their row (row r begins at element r * ldx; row(i) and
- * k(i) say which ones).  fetch loads them without a branch, so that all are on their way together (with one round each,
- * the compiler waited for one before the next), and takes a row's last eight where it ends before; fix moves
- * those to their places, with zeros past the end.  Rows of fewer than eight elements are put together one by one. */
-template <int X, int N, typename ROW, typename KAT>
-__device__ __forceinline__ void w4_fetch_x(typename W4X<X>::E8 (&v)[N], const void *x, long ldx, int nIn, ROW row, KAT k)
+/* N vectors of eight elements of x that may begin anywhere and end behind their row: vector i lies in row row(i), which
+ * begins at element row * ldx, from k on.  fetch loads them without a branch, so that all are on their way together (with
+ * one round each, the compiler waited for one before the next), and takes a row's last eight where it ends
+ * before; fix moves those to their places, with zeros past the end.  FAR: rows may be further from x than 32 bits
+ * reach, or have fewer than eight elements, which are put together one by one. */
+template <int X, bool FAR, int N, typename ROW>
+__device__ __forceinline__ void w4_fetch_x(typename W4X<X>::E8 (&v)[N], const void *x, long ldx, int nIn, int k, ROW row)
 {
 	typedef typename W4X<X>::E E;
 	typedef typename W4X<X>::E8 E8;
 	typedef E8 U __attribute__((aligned(sizeof(E))));
-	if (nIn >= 8) {
+	if constexpr (!FAR) {
+		const unsigned at = (unsigned)(k < nIn - 8 ? k : nIn - 8);
 #pragma unroll
 		for (int i = 0; i < N; i++)
-			v[i] = *(const U *)((const E *)x + row(i) * ldx + (k(i) < nIn - 8 ? k(i) : nIn - 8));
+			v[i] = *(const U *)((const char *)x + (unsigned)(((unsigned)row(i) * (unsigned)ldx + at) * (unsigned)sizeof(E)));
+	} else if (nIn >= 8) {
+		const int at = k < nIn - 8 ? k : nIn - 8;
+#pragma unroll
+		for (int i = 0; i < N; i++)
+			v[i] = *(const U *)((const E *)x + row(i) * ldx + at);
 	} else {
 #pragma unroll
 		for (int i = 0; i < N; i++)
@@ -143,27 +150,43 @@ __device__ __forceinline__ void w4_fetch_x(typename W4X<X>::E8 (&v)[N], const vo
 	}
 }
 
-template <int X, int N, typename KAT>
-__device__ __forceinline__ void w4_fix_x(typename W4X<X>::E8 (&v)[N], int nIn, KAT k)
+template <int X, int N>
+__device__ __forceinline__ void w4_fix_x(typename W4X<X>::E8 (&v)[N], int nIn, int k)
 {
 	typedef typename W4X<X>::E E;
-	const int first = nIn >= 8 ? nIn - 8 : 0;
+	typedef typename W4X<X>::E8 E8;
+	constexpr int ND = sizeof(E8) / 4;
+	typedef unsigned D __attribute__((ext_vector_type(ND)));
+	if (k >= nIn) {
 #pragma unroll
-	for (int i = 0; i < N; i++) {
-		const int by = k(i) > first ? (k(i) - first < 8 ? k(i) - first : 8) : 0;
+		for (int i = 0; i < N; i++)
+			v[i] = (E8)(E)0;
+	} else if (k + 8 > nIn) {
+		/* the row's last eight, by elements further back than wanted (rows of fewer: from 0) */
+		const int by = nIn >= 8 ? k - (nIn - 8) : 0, words = by * (int)sizeof(E) / 4, bits = by * (int)sizeof(E) % 4 * 8;
 #pragma unroll
-		for (int b = 1; b < 8; b *= 2)
+		for (int i = 0; i < N; i++) {
+			D d = __builtin_bit_cast(D, v[i]);
 #pragma unroll
-			for (int e = 0; e < 8; e++)
-				v[i][e] = by & b ? (e + b < 8 ? v[i][e + b] : (E)0) : v[i][e];
+			for (int b = 1; b < ND; b *= 2)
 #pragma unroll
-		for (int e = 0; e < 8; e++)
-			v[i][e] = k(i) + e < nIn ? v[i][e] : (E)0;
+				for (int j = 0; j < ND; j++)
+					d[j] = words & b ? (j + b < ND ? d[j + b] : 0u) : d[j];
+			if constexpr (sizeof(E) < 4)
+#pragma unroll
+				for (int j = 0; j < ND; j++)
+					d[j] = __builtin_amdgcn_alignbit(j + 1 < ND ? d[j + 1] : 0u, d[j], bits);
+			v[i] = __builtin_bit_cast(E8, d);
+			if (nIn < 8)
+#pragma unroll
+				for (int e = 0; e < 8; e++)
+					v[i][e] = e < nIn ? v[i][e] : (E)0;
+		}
 	}
 }
 
 /* The batch as seen from row b0 on, n rows */
-static inline w4_args w4_rows(w4_args a, int b0, int n, size_t esx, size_t esy)
+__host__ __device__ static inline w4_args w4_rows(w4_args a, int b0, int n, size_t esx, size_t esy)
 {
 	a.x = (const char *)a.x + (long)b0 * a.ldx * esx;
 	a.y = (char *)a.y + (long)b0 * a.ldy * esy;

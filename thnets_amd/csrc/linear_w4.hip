@@ -277,8 +277,8 @@ template <int X, int RB, int GM, bool ZP> struct W4Step {
 	}
 };
 
-template <int X, int RB, int NB, int XV, int GM, bool ZP, int W, int D, bool EDGE>
-__global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args a)
+template <int X, int RB, int NB, int XV, int GM, bool ZP, int W, int D, bool FAR>
+__global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args all, int slices)
 {
 	typedef W4X<X> K;
 	typedef typename K::V V;
@@ -291,39 +291,26 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args a)
 	extern __shared__ __align__(16) unsigned char lds[];
 	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int col = lane & 15, quarter = lane >> 4;
-	const int rb0 = blockIdx.x * RB;
+	/* the slices of the batch that need the same codes are neighbours on one XCD (workgroups b, b + 8, ...) */
+	const int turn = blockIdx.x >> 3, rb0 = ((turn / slices) * 8 + (blockIdx.x & 7)) * RB;
+	if (rb0 >= all.blocks)
+		return;
+	constexpr int ROWS = NB * 16 / K::PARTS;
+	const int b0 = turn % slices * ROWS;
+	const w4_args a = w4_rows(all, b0, all.B - b0 < ROWS ? all.B - b0 : ROWS, sizeof(typename K::E),
+		X == W4_X_I8 ? (all.dtype == THHIP_F32 ? 4 : 2) : sizeof(typename K::E));
 	const int cols = a.B * K::PARTS, buf = cols * STRIDE;
 	const int chunks = (a.steps + W - 1) / W;
 
-	/* x of a chunk on its way to LDS: vector tid + i * T of the workgroup's, in the order of the rows.  A vector
-	 * behind its row or the batch is pointed past the buffer and reads as zeros (EDGE: see w4_fetch_x) */
+	/* x of a chunk on its way to LDS: vector tid + i * T of the workgroup's, in the order of the rows */
 	typename K::E8 xr[XV];
 	auto x_row = [&](int i) { return (tid + i * T) / ROWV; };
 	auto load_x = [&](int c) {
-		const int k = c * CK + tid % ROWV * 8;
-		if constexpr (EDGE)
-			w4_fetch_x<X>(xr, a.x, a.ldx, a.nIn, [&](int i) { return (long)(x_row(i) < a.B ? x_row(i) : a.B - 1); }, [&](int) { return k; });
-		else {
-			constexpr int EX = sizeof(typename K::E);
-			const __amdgpu_buffer_rsrc_t xrsrc = __builtin_amdgcn_make_buffer_rsrc((void *)a.x, 0, 0x7fffffff, 0x00020000);
-#pragma unroll
-			for (int i = 0; i < XV; i++) {
-				const unsigned at = x_row(i) < a.B && k < a.nIn ? (unsigned)((x_row(i) * (int)a.ldx + k) * EX) : 0x80000000u;
-				if constexpr (EX == 1)
-					xr[i] = __builtin_bit_cast(typename K::E8, __builtin_amdgcn_raw_buffer_load_b64(xrsrc, at, 0, 0));
-				else if constexpr (EX == 2)
-					xr[i] = __builtin_bit_cast(typename K::E8, __builtin_amdgcn_raw_buffer_load_b128(xrsrc, at, 0, 0));
-				else {
-					struct { uintx4 lo, hi; } v = {__builtin_amdgcn_raw_buffer_load_b128(xrsrc, at, 0, 0),
-						__builtin_amdgcn_raw_buffer_load_b128(xrsrc, at, 16, 0)};
-					xr[i] = __builtin_bit_cast(typename K::E8, v);
-				}
-			}
-		}
+		w4_fetch_x<X, FAR>(xr, a.x, a.ldx, a.nIn, c * CK + tid % ROWV * 8, [&](int i) { return (long)(x_row(i) < a.B ? x_row(i) : a.B - 1); });
 	};
 	auto store_x = [&](int c) {
-		if (EDGE && (c + 1) * CK > a.nIn)
-			w4_fix_x<X>(xr, a.nIn, [&](int) { return c * CK + tid % ROWV * 8; });
+		if ((c + 1) * CK > a.nIn)
+			w4_fix_x<X>(xr, a.nIn, c * CK + tid % ROWV * 8);
 #pragma unroll
 		for (int i = 0; i < XV; i++)
 			if (x_row(i) < a.B) {
@@ -450,42 +437,37 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args a)
 	}
 }
 
-template <int X, int RB, int NB, int XV, int GM, bool ZP, int W, int D, bool EDGE>
+template <int X, int RB, int NB, int XV, int GM, bool ZP, int W, int D, bool FAR>
 static void w4_skinny_launch(const w4_args &a)
 {
 	typedef W4X<X> K;
-	constexpr int ES = sizeof(typename K::V) / 8;
-	size_t lds = 2 * (size_t)a.B * K::PARTS * (W * W4_KSTEP * ES + 16) + W4_KSTEP * ES;
+	constexpr int ES = sizeof(typename K::V) / 8, ROWS = NB * 16 / K::PARTS;
+	const int slices = (a.B + ROWS - 1) / ROWS, rows = a.B < ROWS ? a.B : ROWS;
+	size_t lds = 2 * (size_t)rows * K::PARTS * (W * W4_KSTEP * ES + 16) + W4_KSTEP * ES;
 	const size_t red = (size_t)W * RB * NB * 1024;
 	lds = lds > red ? lds : red;
 	static bool raised;
 	if (!raised) {
-		hipcheck(hipFuncSetAttribute((const void *)w4_skinny_kernel<X, RB, NB, XV, GM, ZP, W, D, EDGE>,
+		hipcheck(hipFuncSetAttribute((const void *)w4_skinny_kernel<X, RB, NB, XV, GM, ZP, W, D, FAR>,
 			hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
 		raised = true;
 	}
-	w4_skinny_kernel<X, RB, NB, XV, GM, ZP, W, D, EDGE><<<dim3((a.blocks + RB - 1) / RB), dim3(W * 64), lds, thhip_stream()>>>(a);
+	const unsigned groups = (a.blocks + RB - 1) / RB;
+	w4_skinny_kernel<X, RB, NB, XV, GM, ZP, W, D, FAR><<<dim3((groups + 7) / 8 * 8 * slices), dim3(W * 64), lds, thhip_stream()>>>(a, slices);
 }
 
-/* Up to 64 columns */
+/* The skinny kernel, in slices of the batch of at most 16 or 32 columns */
 template <int X, int GM, bool ZP>
 static void w4_skinny(const w4_args &a)
 {
 	constexpr int P = W4X<X>::PARTS;
 	constexpr size_t esx = sizeof(typename W4X<X>::E);
-	/* vectors a thread moves a chunk for 4, 16, 32, 64 columns: four rows each */
-	constexpr int X1 = (16 / P + 3) / 4, X2 = (32 / P + 3) / 4, X4 = (64 / P + 3) / 4;
+	/* vectors a thread moves a chunk for 16 and 32 columns: four rows each */
+	constexpr int X1 = (16 / P + 3) / 4, X2 = (32 / P + 3) / 4;
 	const int cols = a.B * P;
-	/* rows of whole vectors on whole words, within the reach of a buffer descriptor */
-	const bool edge = a.nIn % 8 || (uintptr_t)a.x % 4 || a.ldx * esx % 4 || a.ldx * esx * a.B >= 1u << 31;
-	if (edge) {
-		if (cols <= 16)
-			w4_skinny_launch<X, 1, 1, X1, GM, ZP, 8, 2, true>(a);
-		else if (cols <= 32)
-			w4_skinny_launch<X, 1, 2, X2, GM, ZP, 8, 2, true>(a);
-		else
-			w4_skinny_launch<X, 1, 4, X4, GM, ZP, 4, 2, true>(a);
-	} else if (cols <= 16) {
+	if (a.nIn < 8 || a.ldx * esx * 32 >= 1u << 31)
+		w4_skinny_launch<X, 1, 2, X2, GM, ZP, 8, 2, true>(a);
+	else if (cols <= 16) {
 		const bool wide = g_w4_tuning ? g_w4_tuning == 2 : a.blocks >= 1024;
 		if (a.B <= 4) {
 			if (wide)
@@ -496,16 +478,22 @@ static void w4_skinny(const w4_args &a)
 			w4_skinny_launch<X, 2, 1, X1, GM, ZP, 8, 2, false>(a);
 		else
 			w4_skinny_launch<X, 1, 1, X1, GM, ZP, 16, 2, false>(a);
-	} else if (cols <= 32)
-		w4_skinny_launch<X, 1, 2, X2, GM, ZP, 8, 2, false>(a);
-	else
-		w4_skinny_launch<X, 1, 4, X4, GM, ZP, 4, 2, false>(a);
+	} else {
+		const int slices = (cols + 31) / 32;
+		const int rb = g_w4_tuning ? g_w4_tuning % 10 : (long)a.blocks * slices <= 256 ? 1 : (long)a.blocks * slices <= 512 ? 2 : 4;
+		if (rb == 1)
+			w4_skinny_launch<X, 1, 2, X2, GM, ZP, 8, 2, false>(a);
+		else if (rb == 2)
+			w4_skinny_launch<X, 2, 2, X2, GM, ZP, 8, 2, false>(a);
+		else
+			w4_skinny_launch<X, 4, 2, X2, GM, ZP, 8, 2, false>(a);
+	}
 }
 
 template <int X>
 static void w4_choose(const w4_args &a)
 {
-	const bool tile = a.B * W4X<X>::PARTS > 64, small = a.group == 32 || a.group == 64;
+	const bool tile = g_w4_tuning ? g_w4_tuning == 10 : a.B * W4X<X>::PARTS > 256, small = a.group == 32 || a.group == 64;
 	if (tile)
 		w4_tile(a, X);
 	else if (a.zeros)

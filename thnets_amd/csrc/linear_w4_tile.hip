@@ -118,16 +118,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 					k < a.nIn * ES ? (unsigned)(r0 * (int)a.ldx * ES + k) : 0x80000000u, i * 4 * RPI * (int)a.ldx * ES, 0, 0);
 			}
 		} else {
-			w4_fetch_x<X>(xr, xbase, a.ldx, a.nIn, [&](int i) {
+			w4_fetch_x<X, true>(xr, xbase, a.ldx, a.nIn, t * W4_KSTEP + (tid & 15) * 8, [&](int i) {
 				const int r = (tid + (half * (PIECES / 2) + i) * 256) >> 4;
 				return (long)(r < nrows ? r : nrows - 1);
-			}, [&](int i) { return t * W4_KSTEP + (tid & 15) * 8; });
+			});
 		}
 	};
 	auto x_land = [&](int t, int buf, int half) {
 		if constexpr (!DMA) {
 			if ((t + 1) * W4_KSTEP > a.nIn)
-				w4_fix_x<X>(xr, a.nIn, [&](int i) { return t * W4_KSTEP + (tid & 15) * 8; });
+				w4_fix_x<X>(xr, a.nIn, t * W4_KSTEP + (tid & 15) * 8);
 #pragma unroll
 			for (int i = 0; i < PIECES / 2; i++) {
 				const int p = tid + (half * (PIECES / 2) + i) * 256, r = p >> 4, v = p & 15;
