@@ -48,6 +48,30 @@ def test_shapes_i8(hiplib, i, dtype, xgroup):
     U.check_linear(got, want, mag, layer)
 
 
+@pytest.fixture
+def shape(hiplib):
+    """Forces a workgroup shape for a test; the choice by size afterwards."""
+    yield hiplib.thhip_w4_set_shape
+    hiplib.thhip_w4_set_shape(-1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,nIn,nOut,group,zeros", [(21, 1280, 100, 128, 0), (70, 650, 130, 32, 1), (37, 2077, 257, 64, 0), (150, 384, 40, 0, 1)])
+@pytest.mark.parametrize("which", range(6))
+def test_every_shape(hiplib, shape, which, B, nIn, nOut, group, zeros, dtype):
+    """Every shape of workgroup, also where the choice by size takes another: the tile kernel for few rows, one slice of the
+    batch after the other for many."""
+    g, x, b = data(1200 + which, B, nIn, nOut, dtype)
+    layer = U.Layer.random(g, nOut, nIn, group, dtype, zeros).lay(hiplib)
+    want, mag = U.linear64(layer, x, b)
+    q = g.integers(-127, 128, (B, nIn)).astype(np.int8)
+    xs = (g.uniform(0.5, 1.5, (B, U.groups_of(nIn, group))) / 64).astype(np.float32)
+    want8, mag8 = U.linear64(layer, q * U.spread_x(xs.astype(np.float64), nIn, group), b)
+    shape(which)
+    U.check_linear(U.linear(hiplib, layer, x, b), want, mag, layer)
+    U.check_linear(U.linear(hiplib, layer, q, b, xs=xs, xgroup=group), want8, mag8, layer)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("group", GROUPS)
 @pytest.mark.parametrize("zeros", [0, 1])

@@ -35,7 +35,7 @@ TEST_HOOKS = {
     "thhip_conv_set_xcd_parts": (None, [C.c_int]),
     "thhip_conv_set_generic_cl": (None, [C.c_int]),
     "thhip_linear_batched_set_tuning": (None, [C.c_int]),
-    "thhip_w4_set_tuning": (None, [C.c_int]),
+    "thhip_w4_set_shape": (None, [C.c_int]),
     "thhip_conv_set_tuning": (None, [C.c_int, C.c_int, C.c_int, C.c_int]),
 }
 

@@ -207,14 +207,14 @@ extern "C" int thhip_quantize_w4(const void *w, long ldw, int wtype, unsigned ch
 
 /* ---- the product ---- */
 
-static int g_w4_tuning;
+static int g_w4_shape = -1;
 
-extern "C" void thhip_w4_set_tuning(int kernel)
+extern "C" void thhip_w4_set_shape(int shape)
 {
-	g_w4_tuning = kernel;
+	g_w4_shape = shape >= 0 && shape <= 5 ? shape : -1;
 }
 
-/* ---- up to 64 columns: bound by reading the weights once ----
+/* ---- few columns: bound by reading the weights once ----
  *
  * A workgroup of W wavefronts computes RB blocks of 16 rows for all columns and all of K.  K is walked in
  * chunks of W steps, wavefront w multiplying step w of every chunk, so that the workgroup reads W KiB of
@@ -222,7 +222,8 @@ extern "C" void thhip_w4_set_tuning(int kernel)
  * ahead; x goes through LDS, where all wavefronts of the workgroup put a chunk of it down together, one
  * chunk ahead (two buffers, one barrier a chunk): taken to pieces there once, fp32 x is 3 B columns of
  * bf16 from then on, and the matrix core sees columns only.  Columns past the last read a piece of zeros.
- * A column's chunk is followed by 16 bytes, which puts the 16 columns of an operand on different banks.
+ * A 16-byte piece u of a column c's chunk lies in place u ^ c % 16, which puts the 16 columns of an operand on
+ * different banks.
  * Of a 16 x 16 tile a lane holds rows 4 (lane / 16) + 0 .. 3 of column lane % 16.  The wavefronts' sums are
  * added through LDS, in their order, and an fp32 row's three columns with them.
  * GM: matrix instructions a group spans within a step (1: groups of 32 or 64, 4: larger). */
@@ -287,7 +288,7 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args all, in
 	constexpr int ES = sizeof(V) / 8;		/* bytes of an operand's element */
 	constexpr int T = W * 64, ROWV = W * 16;	/* threads; vectors of eight in a row's chunk */
 	constexpr int CK = W * W4_KSTEP;		/* k of a chunk */
-	constexpr int STRIDE = CK * ES + 16;
+	constexpr int STRIDE = CK * ES;
 	extern __shared__ __align__(16) unsigned char lds[];
 	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int col = lane & 15, quarter = lane >> 4;
@@ -318,16 +319,18 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args all, in
 				K::operand(xr[i], o);
 #pragma unroll
 				for (int p = 0; p < K::PARTS; p++)
-					*(V *)(lds + (c & 1) * buf + (x_row(i) * K::PARTS + p) * STRIDE + tid % ROWV * 8 * ES) = o[p];
+					*(V *)(lds + (c & 1) * buf + (x_row(i) * K::PARTS + p) * STRIDE +
+						(tid % ROWV * 8 * ES ^ ((x_row(i) * K::PARTS + p) & 15) * 16)) = o[p];
 			}
 	};
-	/* where a lane's operands lie: in either buffer, or among the zeros */
+	/* where a lane's operands lie: in either buffer, or among the zeros; of matrix instruction j at ^ j * 32 * ES */
 	int at[2][NB];
 #pragma unroll
 	for (int n = 0; n < NB; n++)
 #pragma unroll
 		for (int b = 0; b < 2; b++)
-			at[b][n] = (n * 16 + col < cols ? b * buf + (n * 16 + col) * STRIDE + wave * W4_KSTEP * ES : 2 * buf) + quarter * 8 * ES;
+			at[b][n] = n * 16 + col < cols ? b * buf + (n * 16 + col) * STRIDE + ((wave * W4_KSTEP + quarter * 8) * ES ^ col * 16) :
+				2 * buf + quarter * 8 * ES;
 
 	floatx4 acc[RB][NB];
 #pragma unroll
@@ -370,7 +373,7 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args all, in
 						w[r] = K::weights(now.codes[r][j]);
 #pragma unroll
 					for (int n = 0; n < NB; n++) {
-						const V x = *(const V *)(lds + at[u & 1][n] + j * 32 * ES);
+						const V x = *(const V *)(lds + (at[u & 1][n] ^ j * 32 * ES));
 						if constexpr (X != W4_X_I8 || ZP)
 							sx[n] = K::mma(K::ones(), x, j % GM ? sx[n] : (A)0);
 #pragma unroll
@@ -443,7 +446,7 @@ static void w4_skinny_launch(const w4_args &a)
 	typedef W4X<X> K;
 	constexpr int ES = sizeof(typename K::V) / 8, ROWS = NB * 16 / K::PARTS;
 	const int slices = (a.B + ROWS - 1) / ROWS, rows = a.B < ROWS ? a.B : ROWS;
-	size_t lds = 2 * (size_t)rows * K::PARTS * (W * W4_KSTEP * ES + 16) + W4_KSTEP * ES;
+	size_t lds = 2 * (size_t)rows * K::PARTS * (W * W4_KSTEP * ES) + W4_KSTEP * ES;
 	const size_t red = (size_t)W * RB * NB * 1024;
 	lds = lds > red ? lds : red;
 	static bool raised;
@@ -456,50 +459,80 @@ static void w4_skinny_launch(const w4_args &a)
 	w4_skinny_kernel<X, RB, NB, XV, GM, ZP, W, D, FAR><<<dim3((groups + 7) / 8 * 8 * slices), dim3(W * 64), lds, thhip_stream()>>>(a, slices);
 }
 
-/* The skinny kernel, in slices of the batch of at most 16 or 32 columns */
+/* ---- which kernel and shape ----
+ *
+ * Up to 16 columns: 16 rows a workgroup and 16 wavefronts, one workgroup a CU; from 1024 row blocks on 32 rows and
+ * eight wavefronts, two workgroups a CU (1 x 8192 -> 16384 bf16: 13.2 us; the other 19 us).
+ * More columns: the shape that takes the least time by the estimate below.  A launch runs in rounds of as many
+ * workgroups as the GPU holds; the time of a round was measured at K = 512, 2048 and 8192 and is a start and a
+ * slope.  Of 32 columns 16 rows at a time win in small layers and short K, 64 rows in larger ones (4096 -> 4096 fp16, us:
+ * 32 columns 9.5 / 7.3 / 8.7 / 9.5 / 12.9 in the order of the table, 128 columns 34 / 24.5 / 27.8 / 18.3 / 13.6, tiles
+ * 53), tiles from about 512 columns on (1024 columns: 111 with 64 rows, 63 with tiles). */
+enum { W4_16x16, W4_32x16, W4_16x32, W4_32x32, W4_64x32, W4_TILES };
+
+static int w4_shape(const w4_args &a, int parts)
+{
+	static const float round_us[2][6][2] = {	/* start, and us for 1024 k */
+		{{4.0f, 0.45f}, {5.4f, 0.7f}, {4.2f, 1.1f}, {5.0f, 1.2f}, {6.6f, 1.7f}, {9.0f, 10.0f}},
+		{{4.3f, 0.75f}, {8.0f, 1.5f}, {4.3f, 1.4f}, {6.0f, 1.9f}, {9.6f, 4.2f}, {12.0f, 23.0f}},	/* groups of 32 and 64 */
+	};
+	static const int rows[5] = {1, 2, 1, 2, 4}, cols[5] = {1, 1, 2, 2, 2};	/* blocks of 16 */
+	const float (*us)[2] = round_us[a.group == 32 || a.group == 64];
+	const float k = (float)a.nIn / 1024;
+	/* tiles: 128 rows x 128 columns (fp32 x: 64 rows of x, twice the time), 512 resident, 256 a third faster */
+	const long tiles = (long)((a.blocks + 7) / 8) * ((a.B + (parts > 1 ? 63 : 127)) / (parts > 1 ? 64 : 128));
+	float best = us[5][0] + us[5][1] * k * (parts > 1 ? 2 : 1) * (tiles <= 256 ? 1.0f : 1.35f * (float)((tiles + 511) / 512));
+	int shape = W4_TILES;
+	for (int i = 0; i < 5; i++) {
+		const int slice = cols[i] * 16 / parts;
+		const long n = (long)((a.blocks + rows[i] - 1) / rows[i]) * ((a.B + slice - 1) / slice);
+		const float t = (float)((n + 255) / 256) * (us[i][0] + us[i][1] * k);
+		if (t < best) {
+			best = t;
+			shape = i;
+		}
+	}
+	return shape;
+}
+
 template <int X, int GM, bool ZP>
-static void w4_skinny(const w4_args &a)
+static void w4_skinny(const w4_args &a, int shape)
 {
 	constexpr int P = W4X<X>::PARTS;
-	constexpr size_t esx = sizeof(typename W4X<X>::E);
 	/* vectors a thread moves a chunk for 16 and 32 columns: four rows each */
 	constexpr int X1 = (16 / P + 3) / 4, X2 = (32 / P + 3) / 4;
-	const int cols = a.B * P;
-	if (a.nIn < 8 || a.ldx * esx * 32 >= 1u << 31)
+	if (a.nIn < 8 || a.ldx * sizeof(typename W4X<X>::E) * 32 >= 1u << 31)
 		w4_skinny_launch<X, 1, 2, X2, GM, ZP, 8, 2, true>(a);
-	else if (cols <= 16) {
-		const bool wide = g_w4_tuning ? g_w4_tuning == 2 : a.blocks >= 1024;
-		if (a.B <= 4) {
-			if (wide)
-				w4_skinny_launch<X, 2, 1, 1, GM, ZP, 8, 2, false>(a);
-			else
-				w4_skinny_launch<X, 1, 1, 1, GM, ZP, 16, 2, false>(a);
-		} else if (wide)
+	else if (a.B * P <= 16 && a.blocks >= 1024) {
+		if (a.B <= 4)
+			w4_skinny_launch<X, 2, 1, 1, GM, ZP, 8, 2, false>(a);
+		else
 			w4_skinny_launch<X, 2, 1, X1, GM, ZP, 8, 2, false>(a);
-		else
-			w4_skinny_launch<X, 1, 1, X1, GM, ZP, 16, 2, false>(a);
-	} else {
-		const int slices = (cols + 31) / 32;
-		const int rb = g_w4_tuning ? g_w4_tuning % 10 : (long)a.blocks * slices <= 256 ? 1 : (long)a.blocks * slices <= 512 ? 2 : 4;
-		if (rb == 1)
-			w4_skinny_launch<X, 1, 2, X2, GM, ZP, 8, 2, false>(a);
-		else if (rb == 2)
-			w4_skinny_launch<X, 2, 2, X2, GM, ZP, 8, 2, false>(a);
-		else
-			w4_skinny_launch<X, 4, 2, X2, GM, ZP, 8, 2, false>(a);
-	}
+	} else if (a.B <= 4)
+		w4_skinny_launch<X, 1, 1, 1, GM, ZP, 16, 2, false>(a);
+	else if (a.B * P <= 16 || shape == W4_16x16)
+		w4_skinny_launch<X, 1, 1, X1, GM, ZP, 16, 2, false>(a);
+	else if (shape == W4_32x16)
+		w4_skinny_launch<X, 2, 1, X1, GM, ZP, 16, 2, false>(a);
+	else if (shape == W4_16x32)
+		w4_skinny_launch<X, 1, 2, X2, GM, ZP, 8, 2, false>(a);
+	else if (shape == W4_32x32)
+		w4_skinny_launch<X, 2, 2, X2, GM, ZP, 8, 2, false>(a);
+	else
+		w4_skinny_launch<X, 4, 2, X2, GM, ZP, 8, 2, false>(a);
 }
 
 template <int X>
 static void w4_choose(const w4_args &a)
 {
-	const bool tile = g_w4_tuning ? g_w4_tuning == 10 : a.B * W4X<X>::PARTS > 256, small = a.group == 32 || a.group == 64;
-	if (tile)
+	const bool few = a.B * W4X<X>::PARTS <= 16, small = a.group == 32 || a.group == 64;
+	const int shape = g_w4_shape >= 0 ? g_w4_shape : few ? W4_16x16 : w4_shape(a, W4X<X>::PARTS);
+	if (shape == W4_TILES)
 		w4_tile(a, X);
 	else if (a.zeros)
-		small ? w4_skinny<X, 1, true>(a) : w4_skinny<X, 4, true>(a);
+		small ? w4_skinny<X, 1, true>(a, shape) : w4_skinny<X, 4, true>(a, shape);
 	else
-		small ? w4_skinny<X, 1, false>(a) : w4_skinny<X, 4, false>(a);
+		small ? w4_skinny<X, 1, false>(a, shape) : w4_skinny<X, 4, false>(a, shape);
 }
 
 static int w4_run(const char *who, w4_args &a, const void *packed, int group, int zeros, int xkind, int xgroup, int dtype)

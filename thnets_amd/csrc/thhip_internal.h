@@ -82,8 +82,10 @@ void thhip_conv_set_generic_cl(int on);
 /* Tests and tuning: 16-row blocks a wavefront of thhip_linear_batched owns
  * (1 or 4); 0 restores the choice by the layer's width. */
 void thhip_linear_batched_set_tuning(int row_blocks);
-/* Tests and tuning: which kernel and shape thhip_linear_w4 and thhip_linear_w4_i8 use; 0 restores the choice. */
-void thhip_w4_set_tuning(int kernel);
+/* Tests and tuning: the shape of the workgroups of thhip_linear_w4 and thhip_linear_w4_i8 (rows x columns: 0 16 x 16,
+ * 1 32 x 16, 2 16 x 32, 3 32 x 32, 4 64 x 32, 5 the tiles of the matrix core kernel); up to 16 columns the first five are
+ * the same.  -1 restores the choice by size. */
+void thhip_w4_set_shape(int shape);
 }
 
 /* conv_f32_image.hip: an fp32 image layer (<= 4 planes, plane-major) with factor, shift, Threshold and a
