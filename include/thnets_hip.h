@@ -362,6 +362,14 @@ int THHipSumPartsInKernel(int enable);
  * networks trained against Torch's modules.  Applies to engines created
  * afterwards; returns the previous setting. */
 int THHipTableArithmetic(int as_named);
+/* 0 (default): Linear modules keep their weights in the engine's type.  32, 64, 128 or 256: the float
+ * engines (fp32, fp16, bf16) created afterwards round every Linear's weights to 4 bits, with a scale and a
+ * zero point for every `group` weights of a row (thhip_quantize_w4), and run it through
+ * thhip_linear_w4: an eighth to a quarter of the bytes that a Linear on a few images waits for (nothing in the
+ * reference, whose Linear is modules/Linear.c:72-113 in fp32).  Its input is a vector or a matrix, as there.
+ * Convolutions keep their weights, also those THMakeSpatial makes of a Linear.  Returns the previous setting;
+ * other values change nothing. */
+int THHipLinear4Bit(int group);
 /* New: the uint8 engine on the GPU, counterpart of THCreateLowpNetwork
  * (thapi.c:784-796, lowp_basic.c:133-212): activations quantised to
  * [-range/2, range/2) in 255 steps, int8 MFMA GEMM with gemmlowp offsets

@@ -74,6 +74,7 @@ PROTOTYPES = {
     "THHipImageLayerInFront": (C.c_int, [C.c_int]),
     "THHipSumPartsInKernel": (C.c_int, [C.c_int]),
     "THHipTableArithmetic": (C.c_int, [C.c_int]),
+    "THHipLinear4Bit": (C.c_int, [C.c_int]),
     "THCreateHipLowpNetwork": (vp, [vp, C.c_float]),
     "THHipTensor_newFromFloatTensor": (vp, [vp]),
     "THFloatTensor_newFromHipTensor": (vp, [vp]),
@@ -273,7 +274,7 @@ class HipNetwork:
     Torch7 model directory (``model.net`` + ``stat.t7``, read by ``THLoadNetwork``)."""
 
     def __init__(self, layers, mean=(0.0, 0.0, 0.0), std=(1.0, 1.0, 1.0), half=0, lowp_range=None,
-                 make_spatial=None, fold_bn=True):
+                 make_spatial=None, fold_bn=True, linear4=0):
         self.lib = lib = load_library()
         lib.THInit()
         loaded = None
@@ -297,7 +298,9 @@ class HipNetwork:
             if lib.THHipHalfFloat(half) != 0:
                 raise ValueError("THHipHalfFloat(%r) refused" % half)
             old_fold = lib.THHipFoldBatchNorm(1 if fold_bn else 0)
+            old_linear4 = lib.THHipLinear4Bit(linear4)
             self.handle = lib.THCreateHipNetwork(source)
+            lib.THHipLinear4Bit(old_linear4)
             lib.THHipFoldBatchNorm(old_fold)
             lib.THHipHalfFloat(0)
             self.dtype = (abi.THHIP_F32, abi.THHIP_F16, abi.THHIP_BF16)[half]

@@ -70,6 +70,19 @@ int THHipTableArithmetic(int as_named)
 	return old;
 }
 
+static int g_linear4;
+
+/* 0 (default): Linear modules keep their weights in the engine's type.  32, 64, 128 or 256: they are
+ * rounded to 4 bits with a scale and a zero point for every so many weights of a row.  Read at engine
+ * creation; returns the previous setting. */
+int THHipLinear4Bit(int group)
+{
+	const int old = g_linear4;
+	if (group == 0 || group == 32 || group == 64 || group == 128 || group == 256)
+		g_linear4 = group;
+	return old;
+}
+
 int thhip_engine_dtype(void)
 {
 	return g_halfmode == 1 ? THHIP_F16 : g_halfmode == 2 ? THHIP_BF16 : THHIP_F32;
@@ -78,6 +91,26 @@ int thhip_engine_dtype(void)
 static int esize_of(int dtype)
 {
 	return dtype == THHIP_F32 ? 4 : dtype == THHIP_U8 ? 1 : 2;
+}
+
+/* Row-major host weights [Co][K] -> the packed 4-bit layer (device) */
+static void *linear4_pack(const float *w, int Co, int K, int group, int dtype)
+{
+	const long groups = (K + group - 1) / group;
+	float *dw = thhip_malloc(sizeof(float) * (size_t)Co * K);
+	unsigned char *codes = thhip_malloc((size_t)Co * ((K + 1) / 2)), *zeros = thhip_malloc((size_t)Co * groups);
+	void *scales = thhip_malloc((size_t)Co * groups * esize_of(dtype));
+	void *packed = thhip_malloc(thhip_w4_packed_bytes(Co, K, group, dtype, 1));
+	thhip_memcpy_h2d(dw, w, sizeof(float) * (size_t)Co * K);
+	if (thhip_quantize_w4(dw, K, THHIP_F32, codes, scales, zeros, Co, K, group, dtype) ||
+	    thhip_w4_pack(codes, scales, zeros, packed, Co, K, group, dtype))
+		THError("Linear %d -> %d cannot have 4-bit weights", K, Co);
+	thhip_sync();
+	thhip_free(dw);
+	thhip_free(codes);
+	thhip_free(zeros);
+	thhip_free(scales);
+	return packed;
 }
 
 struct hipnet *hipnet_of(struct module *m)
@@ -216,6 +249,16 @@ static THFloatTensor *Hip_SpatialConvolution_updateOutput(struct module *m, THFl
 			c->nInputPlane, s.H, s.W, c->nOutputPlane, oH, oW);
 	const void *x = thhip_tensor_ptr(in, dt);
 	const int K = c->nInputPlane * c->kH * c->kW;
+	if (hm->w4) {
+		if (s.H * s.W != 1)
+			THError("Linear with 4-bit weights takes a vector or a matrix, not %d x %d images", s.H, s.W);
+		void *y = conv_out(m, dt, &s, c->nOutputPlane, 1, 1);
+		hn->cur_cl = 0;
+		if (thhip_linear_w4(x, K, hm->w4, hm->bias, y, c->nOutputPlane, s.B, K, c->nOutputPlane, hm->w4_group, 1, hm->fused_act,
+				hm->thr, hm->val, dt))
+			THError("Linear %d -> %d with 4-bit weights failed", K, c->nOutputPlane);
+		return m->output;
+	}
 	/* the weights were packed for the planned memory order of the input; with
 	 * one pixel per plane both orders coincide */
 	if (s.H * s.W > 1 && hn->cur_cl != hm->in_cl)
@@ -1234,7 +1277,11 @@ static void convert_module(struct hipnet *hn, struct network *src, int i, int en
 			free(bq);
 			m->updateOutput = HipLowp_SpatialConvolution_updateOutput;
 		} else {
-			hm->wpacked = thhip_conv_pack_weight(THFloatTensor_data(w), Co, Ci, kHW, dtype);
+			if (hm->is_linear && g_linear4) {
+				hm->w4 = linear4_pack(THFloatTensor_data(w), Co, K, g_linear4, dtype);
+				hm->w4_group = g_linear4;
+			} else
+				hm->wpacked = thhip_conv_pack_weight(THFloatTensor_data(w), Co, Ci, kHW, dtype);
 			hm->bias = upload_floats(b, "convolution bias", Co);
 			m->updateOutput = Hip_SpatialConvolution_updateOutput;
 		}
@@ -1391,7 +1438,7 @@ static void plan_channels_last(struct hipnet *hn, struct network *src)
 	for (int i = 0; i < hn->pub.nelem && !lowp; i++) {
 		struct module *m = &hn->pub.modules[i];
 		struct hipmod *hm = &hn->hm[i];
-		if (!is_conv_type(m->type) || !hm->in_cl)
+		if (!is_conv_type(m->type) || !hm->in_cl || hm->w4)
 			continue;
 		/* packed plane-major by convert_module: pack again for channels-last input */
 		const struct SpatialConvolution *c = &m->SpatialConvolution;
@@ -1683,6 +1730,7 @@ void thhip_free_network(struct network *net)
 		THFloatTensor_free(m->output);
 		thhip_free(hm->wpacked);
 		thhip_free(hm->wrow);
+		thhip_free(hm->w4);
 		thhip_free(hm->wfront);
 		thhip_free(hm->bias);
 		thhip_free(hm->scale);

@@ -36,6 +36,8 @@ struct hipmod {
 	size_t tail_at;		/* uint8: offset at which the padding-code tail was last written */
 	void *wpacked;		/* convolution weights in the kernel's packed layout (device) */
 	void *wrow;		/* the same weights row-major, made on first matrix-vector use (device) */
+	void *w4;		/* Linear with 4-bit weights: packed by thhip_w4_pack (device); wpacked and wrow are NULL then */
+	int w4_group;		/* ... weights that share a scale and a zero point */
 	float *bias;		/* fp32 bias (device) */
 	float *scale;		/* fp32 per-plane factor of a folded batch norm, applied before the bias (device), or NULL */
 	float *bn[4];		/* mean, invstd, weight, bias per plane (device) */

@@ -85,7 +85,7 @@ static THFloatTensor *random_input(void)
 
 int main(int argc, char **argv)
 {
-	int runs = 1, print = 0, alg = 8, nbatch = 1, lastlayer = 0x7fffffff, maxoutput = 0x7fffffff, side = 0;
+	int runs = 1, print = 0, alg = 8, nbatch = 1, lastlayer = 0x7fffffff, maxoutput = 0x7fffffff, side = 0, group = 0;
 	float range = 4;
 	const char *modelsdir = 0, *inputfile = 0;
 	for (int i = 1; i < argc; i++) {
@@ -102,6 +102,7 @@ int main(int argc, char **argv)
 		case 'l': if (arg) lastlayer = atoi(argv[++i]); break;
 		case 'L': if (arg) maxoutput = atoi(argv[++i]); break;
 		case 's': if (arg) side = atoi(argv[++i]); break;
+		case 'q': if (arg) group = atoi(argv[++i]); break;
 		case 'b':
 			if (arg) {
 				nbatch = atoi(argv[++i]);
@@ -123,6 +124,7 @@ int main(int argc, char **argv)
 		fprintf(stderr, "             [-l <limit last processed layer to this>]\n");
 		fprintf(stderr, "             [-L <limit printout to max L numbers>]\n");
 		fprintf(stderr, "             [-s <side> (make network spatial)]\n");
+		fprintf(stderr, "             [-q <group> (4-bit Linear weights in groups of 32, 64, 128 or 256; alg 8 to 10)]\n");
 		return -1;
 	}
 	THInit();
@@ -137,6 +139,7 @@ int main(int argc, char **argv)
 		THMakeSpatial(net, side);
 	if (alg == 9 || alg == 10)
 		THHipHalfFloat(alg == 9 ? 1 : 2);
+	THHipLinear4Bit(group);
 	THNETWORK *dev = alg == 11 ? THCreateHipLowpNetwork(net, range) : THCreateHipNetwork(net);
 	THFreeNetwork(net);
 	net = dev;
