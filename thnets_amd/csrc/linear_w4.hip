@@ -496,12 +496,12 @@ static int w4_shape(const w4_args &a, int parts)
 }
 
 template <int X, int GM, bool ZP>
-static void w4_skinny(const w4_args &a, int shape)
+static void w4_skinny(const w4_args &a, int shape, bool far)
 {
 	constexpr int P = W4X<X>::PARTS;
 	/* vectors a thread moves a chunk for 16 and 32 columns: four rows each */
 	constexpr int X1 = (16 / P + 3) / 4, X2 = (32 / P + 3) / 4;
-	if (a.nIn < 8 || a.ldx * sizeof(typename W4X<X>::E) * 32 >= 1u << 31)
+	if (far)
 		w4_skinny_launch<X, 1, 2, X2, GM, ZP, 8, 2, true>(a);
 	else if (a.B * P <= 16 && a.blocks >= 1024) {
 		if (a.B <= 4)
@@ -526,13 +526,15 @@ template <int X>
 static void w4_choose(const w4_args &a)
 {
 	const bool few = a.B * W4X<X>::PARTS <= 16, small = a.group == 32 || a.group == 64;
+	/* rows that 32 bits do not reach in a workgroup's columns, or of less than a vector */
+	const bool far = a.nIn < 8 || a.ldx * sizeof(typename W4X<X>::E) * 128 >= 1u << 31;
 	const int shape = g_w4_shape >= 0 ? g_w4_shape : few ? W4_16x16 : w4_shape(a, W4X<X>::PARTS);
-	if (shape == W4_TILES)
+	if (shape == W4_TILES && !far)
 		w4_tile(a, X);
 	else if (a.zeros)
-		small ? w4_skinny<X, 1, true>(a, shape) : w4_skinny<X, 4, true>(a, shape);
+		small ? w4_skinny<X, 1, true>(a, shape, far) : w4_skinny<X, 4, true>(a, shape, far);
 	else
-		small ? w4_skinny<X, 1, false>(a, shape) : w4_skinny<X, 4, false>(a, shape);
+		small ? w4_skinny<X, 1, false>(a, shape, far) : w4_skinny<X, 4, false>(a, shape, far);
 }
 
 static int w4_run(const char *who, w4_args &a, const void *packed, int group, int zeros, int xkind, int xgroup, int dtype)

@@ -11,6 +11,7 @@
  * LDS rows are 128 k of a column; a 16-byte vector v of row r lies in slot v ^ r % 16 (8-bit x: v ^ r / 2 % 8),
  * which puts the 16 columns of an operand on different banks.  DMA: rows that memory holds in whole, aligned
  * 16-byte vectors are loaded straight into LDS; others go through registers.
+ * KS: where there are fewer tiles than CUs, eight wavefronts share a tile, four taking every other step of K.
  */
 #include <stdint.h>
 #include "linear_w4.h"
@@ -65,8 +66,8 @@ __device__ __forceinline__ float w4_get(const void *p, long i, int dtype)
 	}
 }
 
-template <int X, int GM, bool ZP, bool DMA>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_F32 ? 1 : 2, 2))) void w4_tile_kernel(const w4_args a, int mtiles, int ntiles)
+template <int X, int GM, bool ZP, bool DMA, int KS>
+__global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == THHIP_F32 ? 1 : 2, 2))) void w4_tile_kernel(const w4_args a, int mtiles, int ntiles)
 {
 	typedef W4X<X> K;
 	typedef W4Tile<X, X == W4_X_I8 && GM >= 2> M;
@@ -80,10 +81,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 	constexpr int PIECES = BN * 16 / 256;			/* vectors of eight k a thread moves a step */
 	constexpr int CORR = X != W4_X_I8;
 	constexpr int NG = 4 / GM;				/* groups of a step */
-	__shared__ __align__(16) unsigned char lds[2 * STAGE];
-	__shared__ floatx4 lscale[2][NG][32];			/* the 128 rows' scales of a step's groups */
-	__shared__ floatx4 lzero[2][NG][32];			/* ... and zeros: -z, or (8-bit x) 128 - 16 z as an int */
-	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	__shared__ __align__(16) unsigned char all_lds[KS * 2 * STAGE];
+	__shared__ floatx4 all_scales[KS][2][NG][32];		/* the 128 rows' scales of a step's groups */
+	__shared__ floatx4 all_zeros[KS][2][ZP ? NG : 1][32];	/* ... and zeros: -z, or (8-bit x) 128 - 16 z as an int */
+	const int part = KS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;	/* the wavefronts of one take every KS-th step */
+	const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	unsigned char *lds = all_lds + part * 2 * STAGE;
+	floatx4 (*lscale)[NG][32] = all_scales[part];
+	floatx4 (*lzero)[ZP ? NG : 1][32] = all_zeros[part];
 	const int col = lane & 15, quarter = lane >> 4;
 
 	/* the tiles of an XCD (workgroups b, b + 8, ...) are neighbours, in columns of eight row tiles */
@@ -118,7 +123,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 					k < a.nIn * ES ? (unsigned)(r0 * (int)a.ldx * ES + k) : 0x80000000u, i * 4 * RPI * (int)a.ldx * ES, 0, 0);
 			}
 		} else {
-			w4_fetch_x<X, true>(xr, xbase, a.ldx, a.nIn, t * W4_KSTEP + (tid & 15) * 8, [&](int i) {
+			w4_fetch_x<X, false>(xr, xbase, a.ldx, a.nIn, t * W4_KSTEP + (tid & 15) * 8, [&](int i) {
 				const int r = (tid + (half * (PIECES / 2) + i) * 256) >> 4;
 				return (long)(r < nrows ? r : nrows - 1);
 			});
@@ -180,30 +185,60 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 		for (int n = 0; n < NB; n++)
 			acc[r][n] = (floatx4)0.0f;
 
-	x_issue(0, 0, 0);
-	x_land(0, 0, 0);
+	const int first = part < a.steps ? part : a.steps - 1;
+	x_issue(first, 0, 0);
+	x_land(first, 0, 0);
 	if (!DMA) {
-		x_issue(0, 0, 1);
-		x_land(0, 0, 1);
+		x_issue(first, 0, 1);
+		x_land(first, 0, 1);
 	}
-	codes_issue(0);
-	g_issue(0);
+	codes_issue(first);
+	g_issue(first);
 	g_land(0);
 	barrier();
 
 	constexpr int NU = NB * NG;		/* units of a step: 16 columns x one group */
+	/* a unit's sums are added to the result while the next unit is multiplied, where the registers last */
+	constexpr bool PIPE = DMA && KS == 1;
+	constexpr bool AHEAD = KS == 1;		/* ... and the next unit's operands are read */
 	const int quad = (wave & 1) * 16 + quarter;	/* where the scales of the wavefront's rows begin */
-	for (int t = 0; t < a.steps; t++) {
-		const int buf = t & 1, t1 = t + 1 < a.steps ? t + 1 : t;
+	A p[PIPE ? 2 : 1][4];
+	/* unit u's finished sums into the result (t: its step, buf: where that one's scales are) */
+	auto flush_at = [&](int u, int t, int buf) {
+		const int n = u / NG, g = u % NG;
+		float xs = 1.0f;
+		if constexpr (X == W4_X_I8) {
+			const int row = c0 + n * 16 + col;
+			const float v = a.xscale[(long)(b0 + (row < nrows ? row : 0)) * a.xgroups + (a.xgroups > 1 ? a.group_of(t, g * GM) : 0)];
+			xs = 0.0625f * (a.xgroups > 1 ? v : 1.0f);
+		}
+#pragma unroll
+		for (int r = 0; r < 4; r++) {
+			const floatx4 s = lscale[buf][g][quad + r * 4];
+#pragma unroll
+			for (int i = 0; i < 4; i++)
+				acc[r][n][i] += s[i] * (X == W4_X_I8 ? xs * (float)p[PIPE ? u & 1 : 0][r][i] : (float)p[PIPE ? u & 1 : 0][r][i]);
+			/* (here, not at the end of the step, where the compiler would gather all n's sums) */
+			asm("" : "+v"(acc[r][n]));
+		}
+	};
+	constexpr bool LATE = PIPE && NG == 1 && PARTS == 1;	/* a step's last sums are added at the start of the next */
+	const int rounds = (a.steps + KS - 1) / KS;
+	for (int i = 0; i < rounds; i++) {
+		const int t = i * KS + part, buf = i & 1, t1 = t + KS < a.steps ? t + KS : a.steps - 1;
+		if (KS > 1 && t >= a.steps) {	/* (one step fewer than the others) */
+			barrier();
+			break;
+		}
 		const unsigned char *base = lds + buf * STAGE + (c0 + col) * ROW;
-		V w[4][NJ], x[2][PARTS][NJ];
-		A p[2][4], sx[2];
+		V w[4][NJ], x[AHEAD ? 2 : 1][PARTS][NJ];
+		A sx[2];
 		auto x_read = [&](int n) {
 #pragma unroll
 			for (int q = 0; q < PARTS; q++)
 #pragma unroll
 				for (int j = 0; j < NJ; j++)
-					x[n & 1][q][j] = M::read(base + q * PLANE + n * 16 * ROW, col, j, quarter);
+					x[AHEAD ? n & 1 : 0][q][j] = M::read(base + q * PLANE + n * 16 * ROW, col, j, quarter);
 		};
 		/* sum of x over unit u's group, in every row of the accumulator */
 		auto x_sum = [&](int u) {
@@ -214,28 +249,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 				for (int j = g * GJ; j < (g + 1) * GJ; j++)
 #pragma unroll
 					for (int q = 0; q < PARTS; q++)
-						sx[u & 1] = M::mma(M::ones(), x[n & 1][q][j], sx[u & 1]);
+						sx[u & 1] = M::mma(M::ones(), x[AHEAD ? n & 1 : 0][q][j], sx[u & 1]);
 			}
 		};
-		/* unit u's finished sums into the result */
-		auto flush = [&](int u) {
-			const int n = u / NG, g = u % NG;
-			float xs = 1.0f;
-			if constexpr (X == W4_X_I8) {
-				const int row = c0 + n * 16 + col;
-				const float v = a.xscale[(long)(b0 + (row < nrows ? row : 0)) * a.xgroups + (a.xgroups > 1 ? a.group_of(t, g * GM) : 0)];
-				xs = 0.0625f * (a.xgroups > 1 ? v : 1.0f);
-			}
-#pragma unroll
-			for (int r = 0; r < 4; r++) {
-				const floatx4 s = lscale[buf][g][quad + r * 4];
-#pragma unroll
-				for (int i = 0; i < 4; i++)
-					acc[r][n][i] += s[i] * (X == W4_X_I8 ? xs * (float)p[u & 1][r][i] : (float)p[u & 1][r][i]);
-				/* (here, not at the end of the step, where the compiler would gather all n's sums) */
-				asm("" : "+v"(acc[r][n]));
-			}
-		};
+		auto flush = [&](int u) { flush_at(u, t, buf); };
+		__builtin_amdgcn_s_setprio(0);
 		x_issue(t1, buf ^ 1, 0);
 		x_read(0);
 #pragma unroll
@@ -243,9 +261,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 #pragma unroll
 			for (int r = 0; r < 4; r++)
 				w[r][j] = M::weights(codes[r], j);
-		x_sum(0);
+		if (AHEAD)
+			x_sum(0);
+		if (LATE && i > 0)
+			flush_at(NU - 1, t - KS, buf ^ 1);
 		codes_issue(t1);
 		g_issue(t1);
+		__builtin_amdgcn_s_setprio(1);
 #pragma unroll
 		for (int u = 0; u < NU; u++) {
 			const int n = u / NG, g = u % NG;
@@ -255,8 +277,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 				x_land(t1, buf ^ 1, 0);
 				x_issue(t1, buf ^ 1, 1);
 			}
-			if (g == 0 && n + 1 < NB)
+			if (!AHEAD && g == 0 && n)
+				x_read(n);
+			if (AHEAD && g == 0 && n + 1 < NB)
 				x_read(n + 1);
+			if (!AHEAD)
+				x_sum(u);
 #pragma unroll
 			for (int r = 0; r < 4; r++) {
 				if constexpr (ZP) {
@@ -264,14 +290,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 #pragma unroll
 					for (int i = 0; i < 4; i++) {
 						if constexpr (X == W4_X_I8)
-							p[u & 1][r][i] = __mul24(__float_as_int(z[i]), sx[u & 1][i]);
+							p[PIPE ? u & 1 : 0][r][i] = __mul24(__float_as_int(z[i]), sx[u & 1][i]);
 						else
-							p[u & 1][r][i] = z[i] * sx[u & 1][i];
+							p[PIPE ? u & 1 : 0][r][i] = z[i] * sx[u & 1][i];
 					}
 				} else if constexpr (X == W4_X_I8)
-					p[u & 1][r] = (A)0;
+					p[PIPE ? u & 1 : 0][r] = (A)0;
 				else
-					p[u & 1][r] = -8.0f * sx[u & 1];
+					p[PIPE ? u & 1 : 0][r] = -8.0f * sx[u & 1];
 			}
 #pragma unroll
 			for (int j = g * GJ; j < (g + 1) * GJ; j++)
@@ -279,11 +305,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 				for (int q = 0; q < PARTS; q++)
 #pragma unroll
 					for (int r = 0; r < 4; r++)
-						p[u & 1][r] = M::mma(w[r][j], x[n & 1][q][j], p[u & 1][r]);
-			if (u + 1 < NU)
+						p[PIPE ? u & 1 : 0][r] = M::mma(w[r][j], x[AHEAD ? n & 1 : 0][q][j], p[PIPE ? u & 1 : 0][r]);
+			if (AHEAD && u + 1 < NU)
 				x_sum(u + 1);
-			if (u > 0)
-				flush(u - 1);
+			if (PIPE ? u > 0 : true)
+				flush(PIPE ? u - 1 : u);
+			if constexpr (PIPE && (X == THHIP_F16 || X == THHIP_BF16)) {
 			/* the order to issue them in: what comes from LDS, then a matrix instruction and the sums' work in turn */
 			__builtin_amdgcn_sched_group_barrier(0x100, PARTS * NJ + 4, 0);
 			__builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
@@ -293,12 +320,40 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(X == THHIP_
 				__builtin_amdgcn_sched_group_barrier(0x2, 1, 0);
 			}
 			__builtin_amdgcn_sched_group_barrier(0x8, GJ * PARTS, 0);
+			}
 		}
+		if (PIPE && !LATE)
+			flush(NU - 1);
 		__builtin_amdgcn_sched_barrier(0);
-		flush(NU - 1);
 		x_land(t1, buf ^ 1, DMA ? 0 : 1);
 		g_land(buf ^ 1);
 		barrier();
+	}
+	if (LATE && part < a.steps) {
+		const int last = (a.steps - 1 - part) / KS;
+		flush_at(NU - 1, last * KS + part, last & 1);
+	}
+	if constexpr (KS > 1) {		/* the parts of K, added in their order */
+		floatx4 *sums = (floatx4 *)all_lds;
+		barrier();
+#pragma unroll
+		for (int p = 1; p < KS; p++)
+			if (part == p)
+#pragma unroll
+				for (int r = 0; r < 4; r++)
+#pragma unroll
+					for (int n = 0; n < NB; n++)
+						sums[(((p - 1) * 4 + r) * NB + n) * 256 + tid] = acc[r][n];
+		barrier();
+		if (part)
+			return;
+#pragma unroll
+		for (int p = 1; p < KS; p++)
+#pragma unroll
+			for (int r = 0; r < 4; r++)
+#pragma unroll
+				for (int n = 0; n < NB; n++)
+					acc[r][n] += sums[(((p - 1) * 4 + r) * NB + n) * 256 + tid];
 	}
 
 #pragma unroll
@@ -338,19 +393,25 @@ static void w4_tile_launch(const w4_args &all)
 		/* rows in whole vectors, and a tile of them within the reach of a buffer descriptor */
 		const bool dma = X != THHIP_F32 && (uintptr_t)a.x % 16 == 0 && a.ldx * esx % 16 == 0 && a.nIn * esx % 16 == 0 &&
 			a.ldx * esx * BN < (1u << 31);
-#define W4_TILE(ZP, DMA) w4_tile_kernel<X, GM, ZP, DMA><<<grid, dim3(256), 0, thhip_stream()>>>(a, mtiles, ntiles)
+#define W4_TILE(ZP, DMA, KS) w4_tile_kernel<X, GM, ZP, DMA, KS><<<grid, dim3(KS * 256), 0, thhip_stream()>>>(a, mtiles, ntiles)
 		if constexpr (X != THHIP_F32)
-			if (dma) {
+			if (dma && (long)mtiles * ntiles <= 256) {
 				if (a.zeros)
-					W4_TILE(true, true);
+					W4_TILE(true, true, 2);
 				else
-					W4_TILE(false, true);
+					W4_TILE(false, true, 2);
+				continue;
+			} else if (dma) {
+				if (a.zeros)
+					W4_TILE(true, true, 1);
+				else
+					W4_TILE(false, true, 1);
 				continue;
 			}
 		if (a.zeros)
-			W4_TILE(true, false);
+			W4_TILE(true, false, 1);
 		else
-			W4_TILE(false, false);
+			W4_TILE(false, false, 1);
 #undef W4_TILE
 	}
 }
