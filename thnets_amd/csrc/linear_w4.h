@@ -41,6 +41,7 @@ template <> struct W4X<THHIP_F16> {
 	typedef floatx4 A;
 	static constexpr int PARTS = 1;
 	static __device__ __forceinline__ V ones() { return (V)(_Float16)1.0f; }
+	static __device__ __forceinline__ V minus8() { return (V)(_Float16)-8.0f; }
 	static __device__ __forceinline__ V weights(unsigned w)
 	{
 		typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -60,6 +61,7 @@ template <> struct W4X<THHIP_BF16> {
 	typedef floatx4 A;
 	static constexpr int PARTS = 1;
 	static __device__ __forceinline__ V ones() { return (V)(__bf16)1.0f; }
+	static __device__ __forceinline__ V minus8() { return (V)(__bf16)-8.0f; }
 	static __device__ __forceinline__ V weights(unsigned w)
 	{
 		typedef __bf16 b2 __attribute__((ext_vector_type(2)));
@@ -81,6 +83,7 @@ template <> struct W4X<THHIP_F32> {
 	typedef floatx4 A;
 	static constexpr int PARTS = 3;
 	static __device__ __forceinline__ V ones() { return W4X<THHIP_BF16>::ones(); }
+	static __device__ __forceinline__ V minus8() { return W4X<THHIP_BF16>::minus8(); }
 	static __device__ __forceinline__ V weights(unsigned w) { return W4X<THHIP_BF16>::weights(w); }
 	static __device__ __forceinline__ A mma(V a, V b, A c) { return W4X<THHIP_BF16>::mma(a, b, c); }
 	static __device__ __forceinline__ void operand(const E8 x, V *out)
@@ -111,6 +114,7 @@ template <> struct W4X<W4_X_I8> {
 	typedef intx4 A;
 	static constexpr int PARTS = 1;
 	static __device__ __forceinline__ V ones() { return 0x0101010101010101l; }
+	static __device__ __forceinline__ V minus8() { return 0; }	/* (codes are signed already) */
 	static __device__ __forceinline__ V weights(unsigned w)
 	{
 		const unsigned s = w ^ 0x88888888u;

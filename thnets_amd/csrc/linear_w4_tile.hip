@@ -21,6 +21,7 @@ template <int X, bool WIDE> struct W4Tile {		/* operands of 32 k, as W4X has the
 	typedef typename W4X<X>::A A;
 	static constexpr int MK = 32;
 	static __device__ __forceinline__ V ones() { return W4X<X>::ones(); }
+	static __device__ __forceinline__ V minus8() { return W4X<X>::minus8(); }
 	static __device__ __forceinline__ V weights(const uintx4 &c, int j) { return W4X<X>::weights(c[j]); }
 	static __device__ __forceinline__ A mma(V a, V b, A c) { return W4X<X>::mma(a, b, c); }
 	/* at: the row's address; r: the row in the tile; q: lane / 16 */
@@ -43,6 +44,7 @@ template <> struct W4Tile<W4_X_I8, true> {		/* 8-bit operands of 64 k: two of 32
 		return (V){(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
 	}
 	static __device__ __forceinline__ V ones() { return (V)0x01010101; }
+	static __device__ __forceinline__ V minus8() { return (V)0; }		/* (codes are signed already) */
 	static __device__ __forceinline__ V weights(const uintx4 &c, int j) { return join(H::weights(c, 2 * j), H::weights(c, 2 * j + 1)); }
 	static __device__ __forceinline__ A mma(V a, V b, A c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 	static __device__ __forceinline__ V read(const unsigned char *at, int r, int j, int q)
@@ -81,14 +83,14 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 	constexpr int PIECES = BN * 16 / 256;			/* vectors of eight k a thread moves a step */
 	constexpr int CORR = X != W4_X_I8;
 	constexpr int NG = 4 / GM;				/* groups of a step */
-	__shared__ __align__(16) unsigned char all_lds[KS * 2 * STAGE];
-	__shared__ floatx4 all_scales[KS][2][NG][32];		/* the 128 rows' scales of a step's groups */
-	__shared__ floatx4 all_zeros[KS][2][ZP ? NG : 1][32];	/* ... and zeros: -z, or (8-bit x) 128 - 16 z as an int */
+	/* One array: between the loads into LDS and reads of another array the compiler waits for all of the loads.  x; the
+	 * 128 rows' scales of a step's groups; and zeros: -z, or (8-bit x) 128 - 16 z as an int */
+	constexpr int SCALES = 2 * NG * 512, ZEROS = ZP ? SCALES : 0;
+	__shared__ __align__(16) unsigned char all_lds[KS * (2 * STAGE + SCALES + ZEROS)];
 	const int part = KS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;	/* the wavefronts of one take every KS-th step */
 	const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-	unsigned char *lds = all_lds + part * 2 * STAGE;
-	floatx4 (*lscale)[NG][32] = all_scales[part];
-	floatx4 (*lzero)[ZP ? NG : 1][32] = all_zeros[part];
+	unsigned char *lds = all_lds + part * (2 * STAGE + SCALES + ZEROS);
+	floatx4 (*lscale)[NG][32] = (floatx4 (*)[NG][32])(lds + 2 * STAGE), (*lzero)[NG][32] = (floatx4 (*)[NG][32])(lds + 2 * STAGE + SCALES);
 	const int col = lane & 15, quarter = lane >> 4;
 
 	/* the tiles of an XCD (workgroups b, b + 8, ...) are neighbours, in columns of eight row tiles */
@@ -240,17 +242,21 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 				for (int j = 0; j < NJ; j++)
 					x[AHEAD ? n & 1 : 0][q][j] = M::read(base + q * PLANE + n * 16 * ROW, col, j, quarter);
 		};
-		/* sum of x over unit u's group, in every row of the accumulator */
-		auto x_sum = [&](int u) {
+		/* sum of x over unit u's group, in every row of the accumulator (without zero points -8 times that: 8 is the zero) */
+		auto x_add = [&](int u, int i) {	/* the i-th of the group's GJ pieces */
 			if constexpr (CORR || ZP) {
-				const int n = u / NG, g = u % NG;
-				sx[u & 1] = (A)0;
+				const int n = u / NG, j = u % NG * GJ + i;
+				if (i == 0)
+					sx[u & 1] = (A)0;
 #pragma unroll
-				for (int j = g * GJ; j < (g + 1) * GJ; j++)
-#pragma unroll
-					for (int q = 0; q < PARTS; q++)
-						sx[u & 1] = M::mma(M::ones(), x[AHEAD ? n & 1 : 0][q][j], sx[u & 1]);
+				for (int q = 0; q < PARTS; q++)
+					sx[u & 1] = M::mma(ZP ? M::ones() : M::minus8(), x[AHEAD ? n & 1 : 0][q][j], sx[u & 1]);
 			}
+		};
+		auto x_sum = [&](int u) {
+#pragma unroll
+			for (int i = 0; i < GJ; i++)
+				x_add(u, i);
 		};
 		auto flush = [&](int u) { flush_at(u, t, buf); };
 		__builtin_amdgcn_s_setprio(0);
@@ -297,29 +303,34 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 				} else if constexpr (X == W4_X_I8)
 					p[PIPE ? u & 1 : 0][r] = (A)0;
 				else
-					p[PIPE ? u & 1 : 0][r] = -8.0f * sx[u & 1];
+					p[PIPE ? u & 1 : 0][r] = sx[u & 1];
 			}
+			/* (the next unit's sum of x, whose pieces wait for each other, between the products) */
 #pragma unroll
-			for (int j = g * GJ; j < (g + 1) * GJ; j++)
+			for (int i = 0; i < GJ; i++) {
+				const int j = g * GJ + i;
 #pragma unroll
 				for (int q = 0; q < PARTS; q++)
 #pragma unroll
 					for (int r = 0; r < 4; r++)
 						p[PIPE ? u & 1 : 0][r] = M::mma(w[r][j], x[AHEAD ? n & 1 : 0][q][j], p[PIPE ? u & 1 : 0][r]);
+				if (AHEAD && u + 1 < NU && i > 0)
+					x_add(u + 1, i - 1);
+			}
 			if (AHEAD && u + 1 < NU)
-				x_sum(u + 1);
+				x_add(u + 1, GJ - 1);
 			if (PIPE ? u > 0 : true)
 				flush(PIPE ? u - 1 : u);
 			if constexpr (PIPE && (X == THHIP_F16 || X == THHIP_BF16)) {
 			/* the order to issue them in: what comes from LDS, then a matrix instruction and the sums' work in turn */
 			__builtin_amdgcn_sched_group_barrier(0x100, PARTS * NJ + 4, 0);
-			__builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+			if constexpr (ZP)
+				__builtin_amdgcn_sched_group_barrier(0x2, 16, 0);
 #pragma unroll
-			for (int i = 0; i < 4 * GJ * PARTS; i++) {
+			for (int i = 0; i < 5 * GJ * PARTS; i++) {
 				__builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
 				__builtin_amdgcn_sched_group_barrier(0x2, 1, 0);
 			}
-			__builtin_amdgcn_sched_group_barrier(0x8, GJ * PARTS, 0);
 			}
 		}
 		if (PIPE && !LATE)
@@ -386,6 +397,10 @@ static void w4_tile_launch(const w4_args &all)
 	constexpr size_t esx = sizeof(typename W4X<X>::E);
 	const size_t esy = thhip_esize(all.dtype);
 	constexpr int BN = W4X<X>::PARTS > 1 ? 64 : 128;
+	/* K in two halves where there are fewer tiles than CUs (1024 x 4096 -> 4096, us: 8-bit x 73 -> 57, groups of 32 130 ->
+	 * 113); half types with larger groups keep the matrix cores as busy with four wavefronts (64 and 64; with
+	 * zero points 68 and 73) */
+	constexpr bool HALVES = X == W4_X_I8 || GM == 1;
 	for (int b0 = 0; b0 < all.B; b0 += W4_TILE_ROWS) {
 		const w4_args a = w4_rows(all, b0, all.B - b0 < W4_TILE_ROWS ? all.B - b0 : W4_TILE_ROWS, esx, esy);
 		const int mtiles = (a.blocks + 7) / 8, ntiles = (a.B + BN - 1) / BN;
@@ -394,24 +409,20 @@ static void w4_tile_launch(const w4_args &all)
 		const bool dma = X != THHIP_F32 && (uintptr_t)a.x % 16 == 0 && a.ldx * esx % 16 == 0 && a.nIn * esx % 16 == 0 &&
 			a.ldx * esx * BN < (1u << 31);
 #define W4_TILE(ZP, DMA, KS) w4_tile_kernel<X, GM, ZP, DMA, KS><<<grid, dim3(KS * 256), 0, thhip_stream()>>>(a, mtiles, ntiles)
-		if constexpr (X != THHIP_F32)
-			if (dma && (long)mtiles * ntiles <= 256) {
-				if (a.zeros)
-					W4_TILE(true, true, 2);
-				else
-					W4_TILE(false, true, 2);
-				continue;
-			} else if (dma) {
-				if (a.zeros)
-					W4_TILE(true, true, 1);
-				else
-					W4_TILE(false, true, 1);
+#define W4_TILE_ZP(DMA, KS) do { if (a.zeros) W4_TILE(true, DMA, KS); else W4_TILE(false, DMA, KS); } while (0)
+		if constexpr (X != THHIP_F32) {
+			if constexpr (HALVES)
+				if (dma && (long)mtiles * ntiles <= 256) {
+					W4_TILE_ZP(true, 2);
+					continue;
+				}
+			if (dma) {
+				W4_TILE_ZP(true, 1);
 				continue;
 			}
-		if (a.zeros)
-			W4_TILE(true, false, 1);
-		else
-			W4_TILE(false, false, 1);
+		}
+		W4_TILE_ZP(false, 1);
+#undef W4_TILE_ZP
 #undef W4_TILE
 	}
 }
