@@ -135,6 +135,44 @@ def test_strides_and_offsets(hiplib, dtype, B, ldx, offx, ldy, offy):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("which", range(6))
+@pytest.mark.parametrize("B", [1, 130])
+def test_rows_that_end_with_their_allocation(hiplib, shape, which, B, dtype):
+    """x, its scales, the weights and y lie at the very end of allocations of whole pages: what a kernel asks for past the
+    last row has to stay inside."""
+    nIn, nOut, pages = 4096, 40, 8 << 20
+    g, x, b = data(650, B, nIn, nOut, dtype)
+    q = g.integers(-127, 128, (B, nIn)).astype(np.int8)
+    xs = (g.uniform(0.5, 1.5, (B, nIn // 128)) / 64).astype(np.float32)
+    layer = U.Layer.random(g, nOut, nIn, 128, dtype, True).lay(hiplib)
+    nbytes = hiplib.thhip_w4_packed_bytes(*layer.shape_args(), 1)
+    raw = layer.packed.get((nbytes,), np.uint8)
+
+    def at_end(words):
+        dev = api.DeviceArray(hiplib, nbytes=pages)
+        ptr = dev.ptr + pages - words.nbytes
+        hiplib.thhip_memcpy_h2d(ptr, words.ctypes.data, words.nbytes)
+        return dev, ptr
+
+    kind = np.uint32 if dtype == F32 else np.uint16
+    keep = [at_end(np.ascontiguousarray(w)) for w in (U.raw(x, dtype), q, xs, np.concatenate([raw, np.zeros(-nbytes % 16, np.uint8)]),
+                                                      b, np.zeros((B, nOut), kind))]
+    (_, px), (_, pq), (_, ps), (_, pw), (_, pb), (dy, py) = keep
+    shape(which)
+    tail = (pw, pb, py, nOut, B, nIn, nOut, 128, 1, 0, 0.0, 0.0, dtype)
+    out = np.zeros((B, nOut), kind)
+    G.note("at the end: B=%d shape=%d dtype=%d" % (B, which, dtype))
+    assert hiplib.thhip_linear_w4(px, nIn, *tail) == 0
+    hiplib.thhip_sync()
+    hiplib.thhip_memcpy_d2h(out.ctypes.data, py, out.nbytes)
+    U.check_linear(U.unraw(out, dtype), *U.linear64(layer, x, b), layer)
+    assert hiplib.thhip_linear_w4_i8(pq, nIn, ps, 128, *tail) == 0
+    hiplib.thhip_sync()
+    hiplib.thhip_memcpy_d2h(out.ctypes.data, py, out.nbytes)
+    U.check_linear(U.unraw(out, dtype), *U.linear64(layer, q * U.spread_x(xs.astype(np.float64), nIn, 128), b), layer)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B", [1, 18, 129])
 def test_threshold(hiplib, dtype, B):
     g, x, b = data(700, B, 384, 45, dtype)

@@ -119,10 +119,12 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 			const int r0 = wave * RPI + lane / VROW, slot = lane % VROW;
 			const int v = ES == 1 ? slot ^ (r0 >> 1 & 7) : slot ^ (r0 & 15);
 			const int k = t * ROW + v * 16;		/* (bytes) */
+			/* (the whole offset in the vector operand: a scalar one is no part of the bounds check that keeps
+			 * rows behind the last from being read) */
 #pragma unroll
 			for (int i = 0; i < BN / (4 * RPI); i++) {
 				__builtin_amdgcn_raw_ptr_buffer_load_lds(xrsrc, W4_LDS(lds + buf * STAGE + (i * 4 + wave) * 1024), 16,
-					k < a.nIn * ES ? (unsigned)(r0 * (int)a.ldx * ES + k) : 0x80000000u, i * 4 * RPI * (int)a.ldx * ES, 0, 0);
+					(k < a.nIn * ES ? (unsigned)(r0 * (int)a.ldx * ES + k) : 0x80000000u) + i * 4 * RPI * (int)a.ldx * ES, 0, 0, 0);
 			}
 		} else {
 			w4_fetch_x<X, false>(xr, xbase, a.ldx, a.nIn, t * W4_KSTEP + (tid & 15) * 8, [&](int i) {
