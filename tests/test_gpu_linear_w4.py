@@ -172,6 +172,91 @@ def test_rows_that_end_with_their_allocation(hiplib, shape, which, B, dtype):
     U.check_linear(U.unraw(out, dtype), *U.linear64(layer, q * U.spread_x(xs.astype(np.float64), nIn, 128), b), layer)
 
 
+def on_device(hiplib, nbytes, *parts):
+    """A device buffer with (byte offset, array) parts written."""
+    dev = api.DeviceArray(hiplib, nbytes=nbytes)
+    for at, a in parts:
+        hiplib.thhip_memcpy_h2d(dev.ptr + at, a.ctypes.data, a.nbytes)
+    return dev
+
+
+def from_device(hiplib, dev, at, shape, kind):
+    out = np.zeros(shape, kind)
+    hiplib.thhip_memcpy_d2h(out.ctypes.data, dev.ptr + at, out.nbytes)
+    return out
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B", [2, 3, 40])
+def test_rows_whose_distance_passes_32_bits(hiplib, dtype, B):
+    """The first rows of x, and those of y, more than 2^32 bytes after another (three of them), or 2^24 elements, which are
+    2^31 bytes for 128 rows of 8-bit codes (40)."""
+    es = U.ESIZE[dtype]
+    ld = (1 << 24) + 5 if B == 40 else (1 << 32) // es + 40
+    nIn, nOut = 300, 37
+    g, x, b = data(660, B, nIn, nOut, dtype)
+    layer = U.Layer.random(g, nOut, nIn, 64, dtype, True).lay(hiplib)
+    words, kind = U.raw(x, dtype), np.uint32 if dtype == F32 else np.uint16
+    dx = on_device(hiplib, B * ld * es, *[(i * ld * es, words[i]) for i in range(B)])
+    dy = api.DeviceArray(hiplib, nbytes=B * ld * es)
+    db = api.DeviceArray(hiplib, b)
+    G.note("far rows: B=%d ld=%d dtype=%d" % (B, ld, dtype))
+    tail = (layer.packed.ptr, db.ptr, dy.ptr, ld, B, nIn, nOut, 64, 1, 0, 0.0, 0.0, dtype)
+    assert hiplib.thhip_linear_w4(dx.ptr, ld, *tail) == 0
+    hiplib.thhip_sync()
+    out = np.concatenate([from_device(hiplib, dy, i * ld * es, (1, nOut), kind) for i in range(B)])
+    U.check_linear(U.unraw(out, dtype), *U.linear64(layer, x, b), layer)
+    q = g.integers(-127, 128, (B, nIn)).astype(np.int8)
+    xs = (g.uniform(0.5, 1.5, (B, 1)) / 64).astype(np.float32)
+    for i in range(B):
+        hiplib.thhip_memcpy_h2d(dx.ptr + i * ld, q[i].ctypes.data, nIn)
+    ds = api.DeviceArray(hiplib, xs)
+    assert hiplib.thhip_linear_w4_i8(dx.ptr, ld, ds.ptr, 0, *tail) == 0
+    hiplib.thhip_sync()
+    out = np.concatenate([from_device(hiplib, dy, i * ld * es, (1, nOut), kind) for i in range(B)])
+    U.check_linear(U.unraw(out, dtype), *U.linear64(layer, q * xs.astype(np.float64), b), layer)
+
+
+@pytest.mark.parametrize("B", [1, 2, 50])
+def test_more_outputs_than_a_launch_takes(hiplib, B):
+    """2^24 + 300 outputs: the rows before and behind the border between two launches, and the last ones."""
+    nIn, nOut, group = 40, (1 << 24) + 300, 32
+    g = U.rng(670)
+    x = U.rounded(g.standard_normal((B, nIn), dtype=np.float32), BF16)
+    codes = g.integers(0, 256, (nOut, nIn // 2), dtype=np.uint8)
+    s = U.rounded(g.uniform(0.5, 1.5, (nOut, 2)).astype(np.float32), BF16)
+    z = g.integers(0, 16, (nOut, 2), dtype=np.uint8)
+    b = g.standard_normal(nOut, dtype=np.float32)
+    dc, ds, dz, db = (api.DeviceArray(hiplib, a) for a in (codes, U.raw(s, BF16), z, b))
+    packed = api.DeviceArray(hiplib, nbytes=hiplib.thhip_w4_packed_bytes(nOut, nIn, group, BF16, 1))
+    assert hiplib.thhip_w4_pack(dc.ptr, ds.ptr, dz.ptr, packed.ptr, nOut, nIn, group, BF16) == 0
+    dx, dy = api.DeviceArray(hiplib, U.raw(x, BF16)), api.DeviceArray(hiplib, nbytes=B * nOut * 2)
+    G.note("outputs of two launches: B=%d" % B)
+    assert hiplib.thhip_linear_w4(dx.ptr, nIn, packed.ptr, db.ptr, dy.ptr, nOut, B, nIn, nOut, group, 1, 0, 0.0, 0.0, BF16) == 0
+    hiplib.thhip_sync()
+    for o in (0, (1 << 24) - 64, nOut - 128):
+        part = slice(o, o + 128)
+        layer = U.Layer(U.unpack_codes(codes[part], nIn), s[part], z[part], group, BF16)
+        got = np.concatenate([from_device(hiplib, dy, (i * nOut + o) * 2, (1, 128), np.uint16) for i in range(B)])
+        U.check_linear(U.unraw(got, BF16), *U.linear64(layer, x, b[part]), layer)
+
+
+def test_more_rows_than_a_launch_takes(hiplib):
+    """2^21 + 3 rows of four inputs and 656 outputs: more threads than one grid may have."""
+    B, nIn, nOut = (1 << 21) + 3, 4, 656
+    g = U.rng(680)
+    x = g.standard_normal((B, nIn), dtype=np.float32)
+    layer = U.Layer.random(g, nOut, nIn, 0, F32, True).lay(hiplib)
+    dx, dy = api.DeviceArray(hiplib, x), api.DeviceArray(hiplib, nbytes=B * nOut * 4)
+    G.note("rows of two launches")
+    assert hiplib.thhip_linear_w4(dx.ptr, nIn, layer.packed.ptr, None, dy.ptr, nOut, B, nIn, nOut, 0, 1, 0, 0.0, 0.0, F32) == 0
+    hiplib.thhip_sync()
+    whole = 0xffffffff // 512 // 48 * 10        # (a launch's rows, near enough: the part around the border is compared)
+    for i in (0, whole - 2000, 1 << 20, B - 3000):
+        got = from_device(hiplib, dy, i * nOut * 4, (3000, nOut), np.float32)
+        U.check_linear(got, *U.linear64(layer, x[i:i + 3000]), layer)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B", [1, 18, 129])
 def test_threshold(hiplib, dtype, B):

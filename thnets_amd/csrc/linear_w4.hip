@@ -441,11 +441,11 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args all, in
 }
 
 template <int X, int RB, int NB, int XV, int GM, bool ZP, int W, int D, bool FAR>
-static void w4_skinny_launch(const w4_args &a)
+static void w4_skinny_launch(const w4_args &all)
 {
 	typedef W4X<X> K;
 	constexpr int ES = sizeof(typename K::V) / 8, ROWS = NB * 16 / K::PARTS;
-	const int slices = (a.B + ROWS - 1) / ROWS, rows = a.B < ROWS ? a.B : ROWS;
+	const int rows = all.B < ROWS ? all.B : ROWS;
 	size_t lds = 2 * (size_t)rows * K::PARTS * (W * W4_KSTEP * ES) + W4_KSTEP * ES;
 	const size_t red = (size_t)W * RB * NB * 1024;
 	lds = lds > red ? lds : red;
@@ -455,8 +455,14 @@ static void w4_skinny_launch(const w4_args &a)
 			hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
 		raised = true;
 	}
-	const unsigned groups = (a.blocks + RB - 1) / RB;
-	w4_skinny_kernel<X, RB, NB, XV, GM, ZP, W, D, FAR><<<dim3((groups + 7) / 8 * 8 * slices), dim3(W * 64), lds, thhip_stream()>>>(a, slices);
+	/* a launch has fewer than 2^32 threads: slices of the batch at a time */
+	const unsigned groups = ((all.blocks + RB - 1) / RB + 7) / 8 * 8;
+	const long most = 0xffffffffl / (W * 64) / groups * ROWS;
+	for (long b0 = 0; b0 < all.B; b0 += most) {
+		const w4_args a = w4_rows(all, (int)b0, (int)(all.B - b0 < most ? all.B - b0 : most), sizeof(typename K::E), thhip_esize(all.dtype));
+		const unsigned slices = (a.B + ROWS - 1) / ROWS;
+		w4_skinny_kernel<X, RB, NB, XV, GM, ZP, W, D, FAR><<<dim3(groups * slices), dim3(W * 64), lds, thhip_stream()>>>(a, slices);
+	}
 }
 
 /* ---- which kernel and shape ----
@@ -503,14 +509,14 @@ static void w4_skinny(const w4_args &a, int shape, bool far)
 	constexpr int X1 = (16 / P + 3) / 4, X2 = (32 / P + 3) / 4;
 	if (far)
 		w4_skinny_launch<X, 1, 2, X2, GM, ZP, 8, 2, true>(a);
-	else if (a.B * P <= 16 && a.blocks >= 1024) {
+	else if (a.B <= 16 / P && a.blocks >= 1024) {
 		if (a.B <= 4)
 			w4_skinny_launch<X, 2, 1, 1, GM, ZP, 8, 2, false>(a);
 		else
 			w4_skinny_launch<X, 2, 1, X1, GM, ZP, 8, 2, false>(a);
 	} else if (a.B <= 4)
 		w4_skinny_launch<X, 1, 1, 1, GM, ZP, 16, 2, false>(a);
-	else if (a.B * P <= 16 || shape == W4_16x16)
+	else if (a.B <= 16 / P || shape == W4_16x16)
 		w4_skinny_launch<X, 1, 1, X1, GM, ZP, 16, 2, false>(a);
 	else if (shape == W4_32x16)
 		w4_skinny_launch<X, 2, 1, X1, GM, ZP, 16, 2, false>(a);
@@ -525,9 +531,9 @@ static void w4_skinny(const w4_args &a, int shape, bool far)
 template <int X>
 static void w4_choose(const w4_args &a)
 {
-	const bool few = a.B * W4X<X>::PARTS <= 16, small = a.group == 32 || a.group == 64;
+	const bool few = a.B <= 16 / W4X<X>::PARTS, small = a.group == 32 || a.group == 64;
 	/* rows that 32 bits do not reach in a workgroup's columns, or of less than a vector */
-	const bool far = a.nIn < 8 || a.ldx * sizeof(typename W4X<X>::E) * 128 >= 1u << 31;
+	const bool far = a.nIn < 8 || a.ldx >= (1l << 31) / (128 * (long)sizeof(typename W4X<X>::E));
 	const int shape = g_w4_shape >= 0 ? g_w4_shape : few ? W4_16x16 : w4_shape(a, W4X<X>::PARTS);
 	if (shape == W4_TILES && !far)
 		w4_tile(a, X);
@@ -536,6 +542,8 @@ static void w4_choose(const w4_args &a)
 	else
 		small ? w4_skinny<X, 1, false>(a, shape, far) : w4_skinny<X, 4, false>(a, shape, far);
 }
+
+#define W4_OUTPUTS (1 << 24)	/* of a launch, at most */
 
 static int w4_run(const char *who, w4_args &a, const void *packed, int group, int zeros, int xkind, int xgroup, int dtype)
 {
@@ -558,11 +566,10 @@ static int w4_run(const char *who, w4_args &a, const void *packed, int group, in
 	if (!a.B)
 		return 0;
 	const struct w4_layout l = w4_layout_of(a.nOut, a.nIn, group, dtype, zeros);
-	a.codes = (const unsigned char *)packed;
-	a.scales = (const char *)packed + l.scales;
-	a.zeros = zeros ? (const unsigned char *)packed + l.zeros : 0;
+	const int nOut = a.nOut;
+	const float *bias = a.bias;
+	void *y = a.y;
 	a.steps = l.steps;
-	a.blocks = l.blocks;
 	a.groups = l.groups;
 	a.group = group;
 	a.xgroups = xgroup ? l.groups : 1;
@@ -573,10 +580,20 @@ static int w4_run(const char *who, w4_args &a, const void *packed, int group, in
 			a.shift = i;
 	ThhipLaunchScope scope(THHIP_FAM_GEMV, (double)a.nOut * a.nIn / 2 + (double)a.nOut * l.groups * (es + (zeros ? 1 : 0)) +
 		(double)a.B * a.nIn * esx + (double)a.B * a.nOut * es);
-	if (xkind == W4_X_I8)
-		w4_choose<W4_X_I8>(a);
-	else
-		THHIP_DISPATCH_FLOAT(dtype, (w4_choose<DT>(a)));
+	for (int o0 = 0; o0 < nOut; o0 += W4_OUTPUTS) {	/* (a grid of them has fewer than 2^32 threads) */
+		const size_t rb = o0 / 16;
+		a.nOut = nOut - o0 < W4_OUTPUTS ? nOut - o0 : W4_OUTPUTS;
+		a.blocks = (a.nOut + 15) / 16;
+		a.codes = (const unsigned char *)packed + rb * l.steps * 1024;
+		a.scales = (const char *)packed + l.scales + rb * l.groups * 16 * es;
+		a.zeros = zeros ? (const unsigned char *)packed + l.zeros + rb * l.groups * 16 : 0;
+		a.bias = bias ? bias + o0 : 0;
+		a.y = (char *)y + o0 * es;
+		if (xkind == W4_X_I8)
+			w4_choose<W4_X_I8>(a);
+		else
+			THHIP_DISPATCH_FLOAT(dtype, (w4_choose<DT>(a)));
+	}
 	return 0;
 }
 
