@@ -49,8 +49,7 @@ static struct w4_layout w4_layout_of(int nOut, int nIn, int group, int dtype, in
 	l.groups = group ? (int)(((long)nIn + group - 1) / group) : 1;
 	l.scales = (size_t)l.blocks * l.steps * 1024;
 	l.zeros = l.scales + round16((size_t)l.blocks * l.groups * 16 * thhip_esize(dtype));
-	/* (16 bytes more: the scales' last four may be loaded with the four behind) */
-	l.bytes = l.zeros + (zeros ? (size_t)l.blocks * l.groups * 16 : 0) + 16;
+	l.bytes = l.zeros + (zeros ? (size_t)l.blocks * l.groups * 16 : 0);
 	return l;
 }
 
@@ -224,7 +223,7 @@ extern "C" void thhip_w4_set_shape(int shape)
  * bf16 from then on, and the matrix core sees columns only.  Columns past the last read a piece of zeros.
  * A 16-byte piece u of a column c's chunk lies in place u ^ c % 16, which puts the 16 columns of an operand on
  * different banks.
- * Of a 16 x 16 tile a lane holds rows 4 (lane / 16) + 0 .. 3 of column lane % 16.  The wavefronts' sums are
+ * Of a 16 x 16 tile a lane holds row lane % 16, whose scale and zero point it needs, of columns 4 (lane / 16) + 0 .. 3.  The wavefronts' sums are
  * added through LDS, in their order, and an fp32 row's three columns with them.
  * GM: matrix instructions a group spans within a step (1: groups of 32 or 64, 4: larger). */
 
@@ -237,44 +236,40 @@ __device__ __forceinline__ void w4_lds_barrier(void)
 /* What a wavefront fetches ahead of a step: the codes of its row blocks and what their groups need.  (The number of
  * loads does not depend on the call, so that the compiler can count how many may be outstanding when it needs one.) */
 template <int X, int RB, int GM, bool ZP> struct W4Step {
-	/* 8-bit x: four scales of any type, or of a half type with four more behind */
+	/* 8-bit x: the scale of a type that only the call knows, in the word it lies in */
 	typedef typename ThhipElem<X == W4_X_I8 ? THHIP_F32 : X>::T T;
-	typedef T T4 __attribute__((ext_vector_type(4)));
-	typedef T4 U4 __attribute__((aligned(8)));
 	uintx4 codes[RB];
-	T4 s[RB][4 / GM];
-	unsigned z[RB][4 / GM];
+	T s[RB][4 / GM];
+	unsigned char z[RB][4 / GM];
 	__device__ __forceinline__ void fetch(const w4_args &a, int rb0, int step, int lane)
 	{
 		if (step >= a.steps)
 			step = a.steps - 1;	/* (loaded, not used) */
-		const int esize = X == W4_X_I8 ? (a.dtype == THHIP_F32 ? 4 : 2) : (int)sizeof(T);
 #pragma unroll
 		for (int r = 0; r < RB; r++) {
 			const int rb = rb0 + r < a.blocks ? rb0 + r : a.blocks - 1;
 			codes[r] = *(const uintx4 *)(a.codes + ((size_t)rb * a.steps + step) * 1024 + lane * 16);
 #pragma unroll
 			for (int j = 0; j < 4 / GM; j++) {
-				const size_t at = ((size_t)rb * a.groups + a.group_of(step, j * GM)) * 16;
-				s[r][j] = *(const U4 *)((const char *)a.scales + at * esize + (lane >> 4) * 4 * esize);
+				const size_t at = ((size_t)rb * a.groups + a.group_of(step, j * GM)) * 16 + (lane & 15);
+				if constexpr (X != W4_X_I8)
+					s[r][j] = ((const T *)a.scales)[at];
+				else
+					s[r][j] = *(const float *)((const char *)a.scales + (a.dtype == THHIP_F32 ? at * 4 : at * 2 & ~(size_t)3));
 				if constexpr (ZP)
-					z[r][j] = *(const unsigned *)(a.zeros + at + (lane >> 4) * 4);
+					z[r][j] = a.zeros[at];
 			}
 		}
 	}
-	__device__ __forceinline__ float scale(const w4_args &a, int r, int j, int i) const
+	__device__ __forceinline__ float scale(const w4_args &a, int r, int j, int lane) const
 	{
 		if constexpr (X != W4_X_I8)
-			return (float)s[r][j][i];
+			return (float)s[r][j];
 		else {
-			const unsigned h = __float_as_uint(s[r][j][i / 2]) >> (16 * (i & 1));
+			const unsigned u = __float_as_uint(s[r][j]), h = u >> (16 * (lane & 1)) & 0xffff;
 			const float f16 = (float)__builtin_bit_cast(_Float16, (unsigned short)h);
-			return a.dtype == THHIP_F32 ? s[r][j][i] : a.dtype == THHIP_F16 ? f16 : __uint_as_float(h << 16);
+			return a.dtype == THHIP_F32 ? s[r][j] : a.dtype == THHIP_F16 ? f16 : __uint_as_float(h << 16);
 		}
-	}
-	__device__ __forceinline__ float zero(int r, int j, int i) const
-	{
-		return ZP ? (float)((z[r][j] >> (8 * i)) & 255) : 8.0f;
 	}
 };
 
@@ -323,6 +318,24 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args all, in
 						(tid % ROWV * 8 * ES ^ ((x_row(i) * K::PARTS + p) & 15) * 16)) = o[p];
 			}
 	};
+	/* 8-bit x: its rows' scales for a chunk go the same way, [buffer][part of a step][row] behind the zeros */
+	constexpr int SLOTS = W * 4 / GM, XS = X == W4_X_I8 ? (ROWS * SLOTS + T - 1) / T : 0;
+	float *lxs = (float *)(lds + 2 * buf + W4_KSTEP * ES);
+	float xs[XS + 1];
+	auto load_xs = [&](int c) {
+#pragma unroll
+		for (int i = 0; i < XS; i++) {
+			const int slot = (tid + i * T) / ROWS % SLOTS, row = (tid + i * T) % ROWS;
+			const int step = c * W + slot / (4 / GM), g = a.group_of(step < a.steps ? step : a.steps - 1, slot % (4 / GM) * GM);
+			xs[i] = a.xscale[(long)(row < a.B ? row : 0) * a.xgroups + (a.xgroups > 1 ? g : 0)];
+		}
+	};
+	auto store_xs = [&](int c) {
+#pragma unroll
+		for (int i = 0; i < XS; i++)
+			if (XS * T == ROWS * SLOTS || tid + i * T < ROWS * SLOTS)
+				lxs[(c & 1) * (ROWS * SLOTS) + tid + i * T] = a.xgroups > 1 ? 0.0625f * xs[i] : 0.0625f;
+	};
 	/* where a lane's operands lie: in either buffer, or among the zeros; of matrix instruction j at ^ j * 32 * ES */
 	int at[2][NB];
 #pragma unroll
@@ -342,13 +355,16 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args all, in
 	Step st[D];
 	/* (in the order in which the loop asks for them, so that its waits fit the first time round too) */
 	load_x(0);
+	load_xs(0);
 #pragma unroll
 	for (int d = 0; d < D - 1; d++)
 		st[d].fetch(a, rb0, d * W + wave, lane);
 	if (tid < 32 * ES)
 		((unsigned *)(lds + 2 * buf))[tid] = 0;
 	store_x(0);
+	store_xs(0);
 	load_x(1);
+	load_xs(1);
 	st[D - 1].fetch(a, rb0, (D - 1) * W + wave, lane);
 	w4_lds_barrier();
 
@@ -360,7 +376,9 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args all, in
 			if (c >= chunks)
 				break;
 			store_x(c + 1);		/* (behind K's end: zeros, which nobody reads) */
+			store_xs(c + 1);
 			load_x(c + 2);
+			load_xs(c + 2);
 			const int step = c * W + wave;
 			Step &now = st[u % D];
 			if (step < a.steps) {
@@ -375,36 +393,39 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args all, in
 					for (int n = 0; n < NB; n++) {
 						const V x = *(const V *)(lds + (at[u & 1][n] ^ j * 32 * ES));
 						if constexpr (X != W4_X_I8 || ZP)
-							sx[n] = K::mma(K::ones(), x, j % GM ? sx[n] : (A)0);
+							sx[n] = K::mma(x, K::ones(), j % GM ? sx[n] : (A)0);
 #pragma unroll
 						for (int r = 0; r < RB; r++)
-							p[r][n] = K::mma(w[r], x, j % GM ? p[r][n] : (A)0);
+							p[r][n] = K::mma(x, w[r], j % GM ? p[r][n] : (A)0);
 					}
 					if ((j + 1) % GM)
 						continue;
-					float xs[NB];
+					floatx4 xn[NB];
+					if constexpr (X == W4_X_I8)
 #pragma unroll
-					for (int n = 0; n < NB; n++) {
-						xs[n] = 1.0f;
-						if constexpr (X == W4_X_I8) {
-							const int b = n * 16 + col;
-							const float v = a.xscale[(long)(b < a.B ? b : 0) * a.xgroups + (a.xgroups > 1 ? a.group_of(step, j) : 0)];
-							xs[n] = 0.0625f * (a.xgroups > 1 ? v : 1.0f);
-						}
-					}
+						for (int n = 0; n < NB; n++)
+							xn[n] = *(const floatx4 *)(lxs + (u & 1) * (ROWS * SLOTS) + (wave * (4 / GM) + j / GM) * ROWS + n * 16 + 4 * quarter);
 #pragma unroll
-					for (int r = 0; r < RB; r++)
+					for (int r = 0; r < RB; r++) {
+						const float s = now.scale(a, r, j / GM, lane);
+						const int z = ZP ? now.z[r][j / GM] : 8;
 #pragma unroll
-						for (int i = 0; i < 4; i++) {
-							const float s = now.scale(a, r, j / GM, i), z = now.zero(r, j / GM, i);
+						for (int n = 0; n < NB; n++)
 #pragma unroll
-							for (int n = 0; n < NB; n++) {
+							for (int i = 0; i < 4; i++) {
 								if constexpr (X == W4_X_I8)
-									acc[r][n][i] += s * xs[n] * ((float)p[r][n][i] - (ZP ? (16.0f * z - 128.0f) * (float)sx[n][i] : 0.0f));
+									acc[r][n][i] += s * xn[n][i] * (float)(p[r][n][i] + (ZP ? __mul24(128 - 16 * z, sx[n][i]) : 0));
 								else
-									acc[r][n][i] += s * (p[r][n][i] - z * sx[n][i]);
+									acc[r][n][i] += s * (p[r][n][i] - (float)z * sx[n][i]);
 							}
-						}
+					}
+					/* (now, not at the end of the step, for which the registers do not last) */
+					if constexpr (GM == 1)
+#pragma unroll
+						for (int r = 0; r < RB; r++)
+#pragma unroll
+							for (int n = 0; n < NB; n++)
+								asm("" : "+v"(acc[r][n]));
 				}
 			}
 			now.fetch(a, rb0, step + D * W, lane);
@@ -429,7 +450,7 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args all, in
 #pragma unroll
 			for (int p = 0; p < K::PARTS; p++) {
 				const int c = b * K::PARTS + p;
-				y += ((const float *)&red[((w * RB + row / 16) * NB + c / 16) * 64 + (row % 16 / 4) * 16 + c % 16])[row % 4];
+				y += ((const float *)&red[((w * RB + row / 16) * NB + c / 16) * 64 + (c % 16 / 4) * 16 + row % 16])[c % 4];
 			}
 		if (X == W4_X_I8 && a.xgroups == 1)
 			y *= a.xscale[b];
@@ -447,6 +468,8 @@ static void w4_skinny_launch(const w4_args &all)
 	constexpr int ES = sizeof(typename K::V) / 8, ROWS = NB * 16 / K::PARTS;
 	const int rows = all.B < ROWS ? all.B : ROWS;
 	size_t lds = 2 * (size_t)rows * K::PARTS * (W * W4_KSTEP * ES) + W4_KSTEP * ES;
+	if (X == W4_X_I8)
+		lds += 2 * (size_t)ROWS * (W * 4 / GM) * 4;
 	const size_t red = (size_t)W * RB * NB * 1024;
 	lds = lds > red ? lds : red;
 	static bool raised;
@@ -478,20 +501,27 @@ enum { W4_16x16, W4_32x16, W4_16x32, W4_32x32, W4_64x32, W4_TILES };
 
 static int w4_shape(const w4_args &a, int parts)
 {
-	static const float round_us[2][6][2] = {	/* start, and us for 1024 k */
-		{{4.0f, 0.45f}, {5.4f, 0.7f}, {4.2f, 1.1f}, {5.0f, 1.2f}, {6.6f, 1.7f}, {9.0f, 10.0f}},
-		{{4.3f, 0.75f}, {8.0f, 1.5f}, {4.3f, 1.4f}, {6.0f, 1.9f}, {9.6f, 4.2f}, {12.0f, 23.0f}},	/* groups of 32 and 64 */
+	static const float round_us[2][5][2] = {	/* start, and us for 1024 k */
+		{{4.0f, 0.45f}, {5.4f, 0.7f}, {4.2f, 1.1f}, {5.0f, 1.2f}, {6.6f, 1.7f}},
+		{{4.3f, 0.75f}, {0, 0}, {4.3f, 1.4f}, {6.0f, 1.9f}, {0, 0}},	/* groups of 32 and 64, whose scales the registers of the others do not hold */
+	};
+	static const float tile_us[2][3][2] = {
+		{{13.0f, 10.0f}, {14.0f, 18.0f}, {15.0f, 25.0f}},	/* groups of 128 and more, 64, 32 */
+		{{8.0f, 17.0f}, {8.0f, 24.0f}, {8.0f, 31.0f}},		/* fp32 x */
 	};
 	static const int rows[5] = {1, 2, 1, 2, 4}, cols[5] = {1, 1, 2, 2, 2};	/* blocks of 16 */
 	const float (*us)[2] = round_us[a.group == 32 || a.group == 64];
+	const float *tile = tile_us[parts > 1][a.group == 32 ? 2 : a.group == 64];
 	const float k = (float)a.nIn / 1024;
-	/* tiles: 128 rows x 128 columns (fp32 x: 64 rows of x, twice the time), 512 resident, 256 a third faster */
-	const long tiles = (long)((a.blocks + 7) / 8) * ((a.B + (parts > 1 ? 63 : 127)) / (parts > 1 ? 64 : 128));
-	float best = us[5][0] + us[5][1] * k * (parts > 1 ? 2 : 1) * (tiles <= 256 ? 1.0f : 1.35f * (float)((tiles + 511) / 512));
+	/* tiles: 128 rows x 128 columns, two on a CU (one alone takes two thirds of the time of two); fp32 x 64 rows of x, one on a CU */
+	const long tiles = (long)((a.blocks + 7) / 8) * ((a.B + (parts > 1 ? 63l : 127l)) / (parts > 1 ? 64 : 128));
+	float best = (tile[0] + tile[1] * k) * (parts > 1 ? (float)((tiles + 255) / 256) : tiles <= 256 ? 1.0f : 1.45f * (float)((tiles + 511) / 512));
 	int shape = W4_TILES;
 	for (int i = 0; i < 5; i++) {
+		if (us[i][1] == 0)
+			continue;
 		const int slice = cols[i] * 16 / parts;
-		const long n = (long)((a.blocks + rows[i] - 1) / rows[i]) * ((a.B + slice - 1) / slice);
+		const long n = (long)((a.blocks + rows[i] - 1) / rows[i]) * (((long)a.B + slice - 1) / slice);
 		const float t = (float)((n + 255) / 256) * (us[i][0] + us[i][1] * k);
 		if (t < best) {
 			best = t;

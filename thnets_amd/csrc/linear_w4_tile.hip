@@ -68,7 +68,7 @@ __device__ __forceinline__ float w4_get(const void *p, long i, int dtype)
 	}
 }
 
-template <int X, int GM, bool ZP, bool DMA, int KS>
+template <int X, int GM, bool ZP, bool XG, bool DMA, int KS>
 __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == THHIP_F32 ? 1 : 2, 2))) void w4_tile_kernel(const w4_args a, int mtiles, int ntiles)
 {
 	typedef W4X<X> K;
@@ -84,13 +84,15 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 	constexpr int CORR = X != W4_X_I8;
 	constexpr int NG = 4 / GM;				/* groups of a step */
 	/* One array: between the loads into LDS and reads of another array the compiler waits for all of the loads.  x; the
-	 * 128 rows' scales of a step's groups; and zeros: -z, or (8-bit x) 128 - 16 z as an int */
-	constexpr int SCALES = 2 * NG * 512, ZEROS = ZP ? SCALES : 0;
-	__shared__ __align__(16) unsigned char all_lds[KS * (2 * STAGE + SCALES + ZEROS)];
+	 * 128 rows' scales of a step's groups; zeros: -z, or (8-bit x) 128 - 16 z as an int; and the scales of x where a
+	 * row has several */
+	constexpr int SCALES = 2 * NG * 512, ZEROS = ZP ? SCALES : 0, XSCALES = XG ? SCALES : 0;
+	__shared__ __align__(16) unsigned char all_lds[KS * (2 * STAGE + SCALES + ZEROS + XSCALES)];
 	const int part = KS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;	/* the wavefronts of one take every KS-th step */
 	const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-	unsigned char *lds = all_lds + part * (2 * STAGE + SCALES + ZEROS);
+	unsigned char *lds = all_lds + part * (2 * STAGE + SCALES + ZEROS + XSCALES);
 	floatx4 (*lscale)[NG][32] = (floatx4 (*)[NG][32])(lds + 2 * STAGE), (*lzero)[NG][32] = (floatx4 (*)[NG][32])(lds + 2 * STAGE + SCALES);
+	float (*lxs)[NG][BN] = (float (*)[NG][BN])(lds + 2 * STAGE + SCALES + ZEROS);
 	const int col = lane & 15, quarter = lane >> 4;
 
 	/* the tiles of an XCD (workgroups b, b + 8, ...) are neighbours, in columns of eight row tiles */
@@ -150,7 +152,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 		}
 	};
 	/* scales and zeros: thread i fetches row i % 128's, and puts them into LDS at the end of the step */
-	float gs[NG], gz[NG];
+	float gs[NG], gz[NG], gx[NG];
 	const int grb = mt * 8 + (tid >> 4 & 7) < a.blocks ? mt * 8 + (tid >> 4 & 7) : a.blocks - 1;
 	auto g_issue = [&](int t) {
 #pragma unroll
@@ -159,14 +161,18 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 			gs[g] = w4_get<X>(a.scales, at, a.dtype);
 			if constexpr (ZP)
 				gz[g] = X == W4_X_I8 ? __int_as_float(128 - 16 * (int)a.zeros[at]) : -(float)a.zeros[at];
+			if constexpr (XG)
+				gx[g] = a.xscale[(long)(b0 + ((tid & 127) < nrows ? tid & 127 : 0)) * a.xgroups + a.group_of(t, g * GM)];
 		}
 	};
 	auto g_land = [&](int buf) {
 #pragma unroll
 		for (int g = 0; g < NG; g++) {
-			((float *)lscale[buf][g])[tid & 127] = gs[g];
+			((float *)lscale[buf][g])[tid & 127] = X == W4_X_I8 ? 0.0625f * gs[g] : gs[g];	/* (codes of weights were 16 times theirs) */
 			if constexpr (ZP)
 				((float *)lzero[buf][g])[tid & 127] = gz[g];
+			if constexpr (XG)
+				lxs[buf][g][tid & 127] = gx[g];
 		}
 	};
 	uintx4 codes[4];
@@ -207,21 +213,18 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 	constexpr bool AHEAD = KS == 1;		/* ... and the next unit's operands are read */
 	const int quad = (wave & 1) * 16 + quarter;	/* where the scales of the wavefront's rows begin */
 	A p[PIPE ? 2 : 1][4];
-	/* unit u's finished sums into the result (t: its step, buf: where that one's scales are) */
-	auto flush_at = [&](int u, int t, int buf) {
+	/* unit u's finished sums into the result (buf: where its step's scales are) */
+	auto flush_at = [&](int u, int buf) {
 		const int n = u / NG, g = u % NG;
 		float xs = 1.0f;
-		if constexpr (X == W4_X_I8) {
-			const int row = c0 + n * 16 + col;
-			const float v = a.xscale[(long)(b0 + (row < nrows ? row : 0)) * a.xgroups + (a.xgroups > 1 ? a.group_of(t, g * GM) : 0)];
-			xs = 0.0625f * (a.xgroups > 1 ? v : 1.0f);
-		}
+		if constexpr (XG)
+			xs = lxs[buf][g][c0 + n * 16 + col];
 #pragma unroll
 		for (int r = 0; r < 4; r++) {
 			const floatx4 s = lscale[buf][g][quad + r * 4];
 #pragma unroll
 			for (int i = 0; i < 4; i++)
-				acc[r][n][i] += s[i] * (X == W4_X_I8 ? xs * (float)p[PIPE ? u & 1 : 0][r][i] : (float)p[PIPE ? u & 1 : 0][r][i]);
+				acc[r][n][i] += s[i] * (XG ? xs * (float)p[PIPE ? u & 1 : 0][r][i] : (float)p[PIPE ? u & 1 : 0][r][i]);
 			/* (here, not at the end of the step, where the compiler would gather all n's sums) */
 			asm("" : "+v"(acc[r][n]));
 		}
@@ -260,7 +263,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 			for (int i = 0; i < GJ; i++)
 				x_add(u, i);
 		};
-		auto flush = [&](int u) { flush_at(u, t, buf); };
+		auto flush = [&](int u) { flush_at(u, buf); };
 		__builtin_amdgcn_s_setprio(0);
 		x_issue(t1, buf ^ 1, 0);
 		x_read(0);
@@ -272,7 +275,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 		if (AHEAD)
 			x_sum(0);
 		if (LATE && i > 0)
-			flush_at(NU - 1, t - KS, buf ^ 1);
+			flush_at(NU - 1, buf ^ 1);
 		codes_issue(t1);
 		g_issue(t1);
 		__builtin_amdgcn_s_setprio(1);
@@ -344,7 +347,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 	}
 	if (LATE && part < a.steps) {
 		const int last = (a.steps - 1 - part) / KS;
-		flush_at(NU - 1, last * KS + part, last & 1);
+		flush_at(NU - 1, last & 1);
 	}
 	if constexpr (KS > 1) {		/* the parts of K, added in their order */
 		floatx4 *sums = (floatx4 *)all_lds;
@@ -374,7 +377,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 		const int b = b0 + c0 + n * 16 + col;
 		if (b >= a.B)
 			continue;
-		const float xs = X == W4_X_I8 && a.xgroups == 1 ? a.xscale[b] : 1.0f;
+		const float xs = X == W4_X_I8 && !XG ? a.xscale[b] : 1.0f;
 #pragma unroll
 		for (int r = 0; r < 4; r++) {
 			const int o = (rb0 + r) * 16 + 4 * quarter;
@@ -393,7 +396,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 /* A launch has at most this many rows of x, so that a grid stays below 2^32 threads */
 #define W4_TILE_ROWS (1 << 20)
 
-template <int X, int GM>
+template <int X, int GM, bool XG>
 static void w4_tile_launch(const w4_args &all)
 {
 	constexpr size_t esx = sizeof(typename W4X<X>::E);
@@ -410,7 +413,7 @@ static void w4_tile_launch(const w4_args &all)
 		/* rows in whole vectors, and a tile of them within the reach of a buffer descriptor */
 		const bool dma = X != THHIP_F32 && (uintptr_t)a.x % 16 == 0 && a.ldx * esx % 16 == 0 && a.nIn * esx % 16 == 0 &&
 			a.ldx * esx * BN < (1u << 31);
-#define W4_TILE(ZP, DMA, KS) w4_tile_kernel<X, GM, ZP, DMA, KS><<<grid, dim3(KS * 256), 0, thhip_stream()>>>(a, mtiles, ntiles)
+#define W4_TILE(ZP, DMA, KS) w4_tile_kernel<X, GM, ZP, XG, DMA, KS><<<grid, dim3(KS * 256), 0, thhip_stream()>>>(a, mtiles, ntiles)
 #define W4_TILE_ZP(DMA, KS) do { if (a.zeros) W4_TILE(true, DMA, KS); else W4_TILE(false, DMA, KS); } while (0)
 		if constexpr (X != THHIP_F32) {
 			if constexpr (HALVES)
@@ -429,25 +432,27 @@ static void w4_tile_launch(const w4_args &all)
 	}
 }
 
-template <int X>
+template <int X, bool XG>
 static void w4_tile_groups(const w4_args &a)
 {
 	if (a.group == 32)
-		w4_tile_launch<X, 1>(a);
+		w4_tile_launch<X, 1, XG>(a);
 	else if (a.group == 64)
-		w4_tile_launch<X, 2>(a);
+		w4_tile_launch<X, 2, XG>(a);
 	else
-		w4_tile_launch<X, 4>(a);
+		w4_tile_launch<X, 4, XG>(a);
 }
 
 void w4_tile(const w4_args &a, int xkind)
 {
-	if (xkind == W4_X_I8)
-		w4_tile_groups<W4_X_I8>(a);
+	if (xkind == W4_X_I8 && a.xgroups > 1)
+		w4_tile_groups<W4_X_I8, true>(a);
+	else if (xkind == W4_X_I8)
+		w4_tile_groups<W4_X_I8, false>(a);
 	else if (xkind == THHIP_F32)
-		w4_tile_groups<THHIP_F32>(a);
+		w4_tile_groups<THHIP_F32, false>(a);
 	else if (xkind == THHIP_F16)
-		w4_tile_groups<THHIP_F16>(a);
+		w4_tile_groups<THHIP_F16, false>(a);
 	else
-		w4_tile_groups<THHIP_BF16>(a);
+		w4_tile_groups<THHIP_BF16, false>(a);
 }
