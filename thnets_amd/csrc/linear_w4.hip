@@ -494,23 +494,26 @@ static void w4_skinny_launch(const w4_args &all)
  * eight wavefronts, two workgroups a CU (1 x 8192 -> 16384 bf16: 13.2 us; the other 19 us).
  * More columns: the shape that takes the least time by the estimate below.  A launch runs in rounds of as many
  * workgroups as the GPU holds; the time of a round was measured at K = 512, 2048 and 8192 and is a start and a
- * slope.  Of 32 columns 16 rows at a time win in small layers and short K, 64 rows in larger ones (4096 -> 4096 fp16, us:
- * 32 columns 9.5 / 7.3 / 8.7 / 9.5 / 12.9 in the order of the table, 128 columns 34 / 24.5 / 27.8 / 18.3 / 13.6, tiles
- * 53), tiles from about 512 columns on (1024 columns: 111 with 64 rows, 63 with tiles). */
+ * slope.  Few rows at a time win in small layers and short K, 64 rows in larger ones (4096 -> 4096 fp16, us, in the
+ * order of the table: 128 columns 37 / 24 / 27 / 17.4 / 12.8, tiles 50), tiles from about 512 columns on (768 columns: 81
+ * with 64 rows, 56 with tiles).  Of 78 layers drawn at random (16 to 1300 rows, 512 to 9216 inputs, 256 to 10240 outputs) the
+ * choice took 1.6 % more than the best shape, 18 % at most. */
 enum { W4_16x16, W4_32x16, W4_16x32, W4_32x32, W4_64x32, W4_TILES };
 
 static int w4_shape(const w4_args &a, int parts)
 {
-	static const float round_us[2][5][2] = {	/* start, and us for 1024 k */
-		{{4.0f, 0.45f}, {5.4f, 0.7f}, {4.2f, 1.1f}, {5.0f, 1.2f}, {6.6f, 1.7f}},
-		{{4.3f, 0.75f}, {0, 0}, {4.3f, 1.4f}, {6.0f, 1.9f}, {0, 0}},	/* groups of 32 and 64, whose scales the registers of the others do not hold */
+	static const float round_us[4][5][2] = {	/* start, and us for 1024 k */
+		{{4.0f, 0.42f}, {4.9f, 0.57f}, {3.9f, 0.93f}, {4.4f, 1.22f}, {5.5f, 1.75f}},
+		{{4.6f, 0.55f}, {5.6f, 0.87f}, {4.2f, 1.25f}, {4.8f, 1.65f}, {5.9f, 2.6f}},	/* groups of 32 and 64 */
+		{{3.9f, 0.42f}, {4.9f, 0.54f}, {3.3f, 0.73f}, {4.3f, 1.0f}, {6.3f, 1.6f}},	/* 8-bit x */
+		{{4.5f, 0.65f}, {6.0f, 1.2f}, {4.4f, 1.35f}, {5.6f, 2.2f}, {8.0f, 3.8f}},	/* ... in groups of 32 and 64 */
 	};
 	static const float tile_us[2][3][2] = {
-		{{13.0f, 10.0f}, {14.0f, 18.0f}, {15.0f, 25.0f}},	/* groups of 128 and more, 64, 32 */
+		{{13.0f, 10.0f}, {14.0f, 15.5f}, {15.0f, 23.0f}},	/* groups of 128 and more, 64, 32 */
 		{{8.0f, 17.0f}, {8.0f, 24.0f}, {8.0f, 31.0f}},		/* fp32 x */
 	};
 	static const int rows[5] = {1, 2, 1, 2, 4}, cols[5] = {1, 1, 2, 2, 2};	/* blocks of 16 */
-	const float (*us)[2] = round_us[a.group == 32 || a.group == 64];
+	const float (*us)[2] = round_us[(a.xscale ? 2 : 0) + (a.group == 32 || a.group == 64)];
 	const float *tile = tile_us[parts > 1][a.group == 32 ? 2 : a.group == 64];
 	const float k = (float)a.nIn / 1024;
 	/* tiles: 128 rows x 128 columns, two on a CU (one alone takes two thirds of the time of two); fp32 x 64 rows of x, one on a CU */
@@ -518,8 +521,6 @@ static int w4_shape(const w4_args &a, int parts)
 	float best = (tile[0] + tile[1] * k) * (parts > 1 ? (float)((tiles + 255) / 256) : tiles <= 256 ? 1.0f : 1.45f * (float)((tiles + 511) / 512));
 	int shape = W4_TILES;
 	for (int i = 0; i < 5; i++) {
-		if (us[i][1] == 0)
-			continue;
 		const int slice = cols[i] * 16 / parts;
 		const long n = (long)((a.blocks + rows[i] - 1) / rows[i]) * (((long)a.B + slice - 1) / slice);
 		const float t = (float)((n + 255) / 256) * (us[i][0] + us[i][1] * k);

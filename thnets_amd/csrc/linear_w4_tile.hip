@@ -91,7 +91,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 	const int part = KS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;	/* the wavefronts of one take every KS-th step */
 	const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	unsigned char *lds = all_lds + part * (2 * STAGE + SCALES + ZEROS + XSCALES);
-	floatx4 (*lscale)[NG][32] = (floatx4 (*)[NG][32])(lds + 2 * STAGE), (*lzero)[NG][32] = (floatx4 (*)[NG][32])(lds + 2 * STAGE + SCALES);
+	float (*lscale)[NG][128] = (float (*)[NG][128])(lds + 2 * STAGE), (*lzero)[NG][128] = (float (*)[NG][128])(lds + 2 * STAGE + SCALES);
 	float (*lxs)[NG][BN] = (float (*)[NG][BN])(lds + 2 * STAGE + SCALES + ZEROS);
 	const int col = lane & 15, quarter = lane >> 4;
 
@@ -168,9 +168,9 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 	auto g_land = [&](int buf) {
 #pragma unroll
 		for (int g = 0; g < NG; g++) {
-			((float *)lscale[buf][g])[tid & 127] = X == W4_X_I8 ? 0.0625f * gs[g] : gs[g];	/* (codes of weights were 16 times theirs) */
+			lscale[buf][g][tid & 127] = X == W4_X_I8 ? 0.0625f * gs[g] : gs[g];	/* (codes of weights were 16 times theirs) */
 			if constexpr (ZP)
-				((float *)lzero[buf][g])[tid & 127] = gz[g];
+				lzero[buf][g][tid & 127] = gz[g];
 			if constexpr (XG)
 				lxs[buf][g][tid & 127] = gx[g];
 		}
@@ -211,20 +211,20 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 	/* a unit's sums are added to the result while the next unit is multiplied, where the registers last */
 	constexpr bool PIPE = DMA && KS == 1;
 	constexpr bool AHEAD = KS == 1;		/* ... and the next unit's operands are read */
-	const int quad = (wave & 1) * 16 + quarter;	/* where the scales of the wavefront's rows begin */
+	const int own = (wave & 1) * 64 + col;	/* the lane's row of the first row block */
 	A p[PIPE ? 2 : 1][4];
 	/* unit u's finished sums into the result (buf: where its step's scales are) */
 	auto flush_at = [&](int u, int buf) {
 		const int n = u / NG, g = u % NG;
-		float xs = 1.0f;
+		floatx4 xs;
 		if constexpr (XG)
-			xs = lxs[buf][g][c0 + n * 16 + col];
+			xs = *(const floatx4 *)&lxs[buf][g][c0 + n * 16 + 4 * quarter];
 #pragma unroll
 		for (int r = 0; r < 4; r++) {
-			const floatx4 s = lscale[buf][g][quad + r * 4];
+			const float s = lscale[buf][g][own + r * 16];
 #pragma unroll
 			for (int i = 0; i < 4; i++)
-				acc[r][n][i] += s[i] * (XG ? xs * (float)p[PIPE ? u & 1 : 0][r][i] : (float)p[PIPE ? u & 1 : 0][r][i]);
+				acc[r][n][i] += (XG ? s * xs[i] : s) * (float)p[PIPE ? u & 1 : 0][r][i];
 			/* (here, not at the end of the step, where the compiler would gather all n's sums) */
 			asm("" : "+v"(acc[r][n]));
 		}
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 				for (int j = 0; j < NJ; j++)
 					x[AHEAD ? n & 1 : 0][q][j] = M::read(base + q * PLANE + n * 16 * ROW, col, j, quarter);
 		};
-		/* sum of x over unit u's group, in every row of the accumulator (without zero points -8 times that: 8 is the zero) */
+		/* sum of x over unit u's group, for every row (without zero points -8 times that: 8 is the zero) */
 		auto x_add = [&](int u, int i) {	/* the i-th of the group's GJ pieces */
 			if constexpr (CORR || ZP) {
 				const int n = u / NG, j = u % NG * GJ + i;
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 					sx[u & 1] = (A)0;
 #pragma unroll
 				for (int q = 0; q < PARTS; q++)
-					sx[u & 1] = M::mma(ZP ? M::ones() : M::minus8(), x[AHEAD ? n & 1 : 0][q][j], sx[u & 1]);
+					sx[u & 1] = M::mma(x[AHEAD ? n & 1 : 0][q][j], ZP ? M::ones() : M::minus8(), sx[u & 1]);
 			}
 		};
 		auto x_sum = [&](int u) {
@@ -297,13 +297,13 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 #pragma unroll
 			for (int r = 0; r < 4; r++) {
 				if constexpr (ZP) {
-					const floatx4 z = lzero[buf][g][quad + r * 4];
+					const float z = lzero[buf][g][own + r * 16];
 #pragma unroll
 					for (int i = 0; i < 4; i++) {
 						if constexpr (X == W4_X_I8)
-							p[PIPE ? u & 1 : 0][r][i] = __mul24(__float_as_int(z[i]), sx[u & 1][i]);
+							p[PIPE ? u & 1 : 0][r][i] = __mul24(__float_as_int(z), sx[u & 1][i]);
 						else
-							p[PIPE ? u & 1 : 0][r][i] = z[i] * sx[u & 1][i];
+							p[PIPE ? u & 1 : 0][r][i] = z * sx[u & 1][i];
 					}
 				} else if constexpr (X == W4_X_I8)
 					p[PIPE ? u & 1 : 0][r] = (A)0;
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 				for (int q = 0; q < PARTS; q++)
 #pragma unroll
 					for (int r = 0; r < 4; r++)
-						p[PIPE ? u & 1 : 0][r] = M::mma(w[r][j], x[AHEAD ? n & 1 : 0][q][j], p[PIPE ? u & 1 : 0][r]);
+						p[PIPE ? u & 1 : 0][r] = M::mma(x[AHEAD ? n & 1 : 0][q][j], w[r][j], p[PIPE ? u & 1 : 0][r]);
 				if (AHEAD && u + 1 < NU && i > 0)
 					x_add(u + 1, i - 1);
 			}
@@ -373,23 +373,21 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 	}
 
 #pragma unroll
-	for (int n = 0; n < NB; n++) {
-		const int b = b0 + c0 + n * 16 + col;
-		if (b >= a.B)
-			continue;
-		const float xs = X == W4_X_I8 && !XG ? a.xscale[b] : 1.0f;
+	for (int r = 0; r < 4; r++) {
+		const int o = (rb0 + r) * 16 + col;
+		const float bias = a.bias && o < a.nOut ? a.bias[o] : 0.0f;
 #pragma unroll
-		for (int r = 0; r < 4; r++) {
-			const int o = (rb0 + r) * 16 + 4 * quarter;
+		for (int n = 0; n < NB; n++)
 #pragma unroll
-			for (int i = 0; i < 4; i++)
-				if (o + i < a.nOut) {
-					float y = acc[r][n][i] * xs + (a.bias ? a.bias[o + i] : 0.0f);
+			for (int i = 0; i < 4; i++) {
+				const int b = b0 + c0 + n * 16 + 4 * quarter + i;
+				if (b < a.B && o < a.nOut) {
+					float y = acc[r][n][i] * (X == W4_X_I8 && !XG ? a.xscale[b] : 1.0f) + bias;
 					if (a.act)
 						y = y > a.thr ? y : a.val;
-					w4_put<X>(a.y, b * a.ldy + o + i, y, a.dtype);
+					w4_put<X>(a.y, b * a.ldy + o, y, a.dtype);
 				}
-		}
+			}
 	}
 }
 
