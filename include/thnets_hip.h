@@ -728,8 +728,8 @@ void thhip_rgb2float_batch(void *dst, const unsigned char *src, int n, long src_
  *
  * thhip_quantize_w4 makes them on the device from weights of type `wtype`, rows ldw apart: without zeros
  * s = max|w| / 7 and n = rint(w / s) + 8; with zeros s = (max(w, 0) - min(w, 0)) / 15, z = rint(-min(w, 0) / s),
- * n = rint(w / s) + z, at most 15.  s is rounded to `dtype` first.  Finite weights; a group whose scale has no
- * reciprocal in fp32, or rounds to 0, becomes 0.
+ * n = rint(w / s) + z, at most 15.  s is rounded to `dtype` first, and its largest number (65504) where it would
+ * pass it; a group whose scale has no reciprocal in fp32 (under 2^-128), or rounds to 0, becomes 0.  Weights are finite.
  *
  * thhip_w4_pack lays codes, scales and zeros out in the order the kernels read them, into one buffer of
  * thhip_w4_packed_bytes(nOut, nIn, group, dtype, zeros != NULL) bytes (0 for a layer that is refused), aligned to

@@ -333,6 +333,35 @@ def test_quantize(hiplib, dtype, wtype, group, zeros, nIn):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("zeros", [0, 1])
+def test_quantize_at_the_ends_of_the_range(hiplib, dtype, zeros):
+    """Rows of weights from the smallest numbers to fp32's largest: scales are finite and codes those of w / s; a row whose
+    scale is under 2^-128, or 0 in its type, stands for 0."""
+    nIn, tops = 64, np.array([0, 1e-45, 2.0 ** -130, 2.0 ** -120, 2.0 ** -30, 2.0 ** -20, 1e5, 4e5, 1e9, 3.4e38])
+    g = U.rng(1010)
+    w = (g.uniform(-1, 1, (len(tops), nIn)) * tops[:, None]).astype(np.float32)
+    w[:, 0], w[:, 1] = tops, -tops
+    dw, dc, ds, dz = (api.DeviceArray(hiplib, nbytes=n) for n in (w.nbytes, len(tops) * 32, len(tops) * 4, len(tops)))
+    hiplib.thhip_memcpy_h2d(dw.ptr, w.ctypes.data, w.nbytes)
+    assert hiplib.thhip_quantize_w4(dw.ptr, nIn, F32, dc.ptr, ds.ptr, dz.ptr if zeros else None, len(tops), nIn, 64, dtype) == 0
+    hiplib.thhip_sync()
+    s = U.unraw(ds.get((len(tops),), np.uint32 if dtype == F32 else np.uint16), dtype).astype(np.float64)
+    codes = U.unpack_codes(dc.get((len(tops), 32), np.uint8), nIn).astype(np.float64)
+    z = dz.get((len(tops),), np.uint8).astype(np.float64) if zeros else np.full(len(tops), 8.0)
+    assert np.isfinite(s).all()
+    top = tops.astype(np.float32).astype(np.float64) * (2 / 15 if zeros else 1 / 7)
+    for i in range(len(tops)):
+        if s[i] < 2.0 ** -128:
+            assert top[i] < 2.0 ** -127 + U.TINY[dtype] * 1.01 and (codes[i] == z[i]).all()
+        else:
+            # (an fp16 scale near the smallest is off by half a step of the denormals)
+            want = min(top[i], 65504) if dtype == F16 else top[i]
+            assert abs(s[i] - want) <= 2 * U.HALF_STEP[dtype] * want + U.TINY[dtype]
+            exact = w[i].astype(np.float64) / s[i] + z[i]
+            assert (np.abs(codes[i] - np.clip(exact, 0, 15)) <= 0.5 + 1e-4).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_from_weights_to_outputs(hiplib, dtype):
     """quantise, pack and multiply in one go, as a program does; the product is that of the weights the codes stand for."""
     g, x, b = data(1100, 9, 640, 72, dtype)

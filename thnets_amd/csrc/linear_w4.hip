@@ -156,8 +156,10 @@ __global__ __launch_bounds__(256) void w4_quantize_kernel(const void *w, long ld
 			lo = fminf(lo, __shfl_xor(lo, off, 64));
 			hi = fmaxf(hi, __shfl_xor(hi, off, 64));
 		}
-		typename ThhipElem<DT>::T sr = (typename ThhipElem<DT>::T)(zeros ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f);
-		const float s = (float)sr, inv = s > 0 ? 1.0f / s : 0.0f;
+		/* (a scale that the type does not hold becomes its largest: the outermost weights are cut off) */
+		const float most = DT == THHIP_F16 ? 65504.0f : 3e38f;
+		typename ThhipElem<DT>::T sr = (typename ThhipElem<DT>::T)fminf(zeros ? hi / 15.0f - lo / 15.0f : fmaxf(hi, -lo) / 7.0f, most);
+		const float s = (float)sr, inv = s > 0 && 1.0f / s < INFINITY ? 1.0f / s : 0.0f;
 		const float z = zeros ? fminf(rintf(-lo * inv), 15.0f) : 8.0f;
 		if (lane == 0) {
 			ThhipElem<DT>::st(scales, (long)i, s);
