@@ -724,7 +724,7 @@ void thhip_rgb2float_batch(void *dst, const unsigned char *src, int n, long src_
  * Weights with 4 bits: a code n of 0 .. 15 a weight, row-major [nOut][(nIn + 1) / 2] bytes, even k in the low
  * half of a byte; `group` consecutive weights of a row (32, 64, 128 or 256; 0: the whole row) share a scale and a
  * zero point: w = s * (n - z).  scales: [nOut][groups] in `dtype`, groups = ceil(nIn / group); zeros:
- * [nOut][groups] bytes, or NULL: 8 everywhere.
+ * [nOut][groups] bytes of 0 .. 15, or NULL: 8 everywhere.
  *
  * thhip_quantize_w4 makes them on the device from weights of type `wtype`, rows ldw apart: without zeros
  * s = max|w| / 7 and n = rint(w / s) + 8; with zeros s = (max(w, 0) - min(w, 0)) / 15, z = rint(-min(w, 0) / s),
@@ -743,7 +743,7 @@ int thhip_quantize_w4(const void *w, long ldw, int wtype, unsigned char *codes, 
 /* y[b][o] = act(bias[o] + sum_k w[o][k] * x[b][k]) for any batch: thhip_gemv, thhip_linear_batched and the 1x1
  * convolution of nn_Linear_updateOutput (Linear.c:72-113) for packed 4-bit weights.  x [B][nIn] and y [B][nOut] in
  * `dtype`, bias fp32 [nOut] or NULL; act != 0 applies the Threshold y > thr ? y : val.  Weights are never rounded:
- * the products with the codes are summed in fp32 and a group's sum is multiplied with its scale.  An infinity
+ * products with n - z are summed in fp32 and a group's sum is multiplied with its scale.  An infinity
  * or NaN in a row of x makes outputs of that row NaN (or infinite); other rows do not see it.  y may not overlap x. */
 int thhip_linear_w4(const void *x, long ldx, const void *wpacked, const float *bias, void *y, long ldy,
 	int B, int nIn, int nOut, int group, int zeros, int act, float thr, float val, int dtype);

@@ -31,7 +31,8 @@ struct w4_args {
 };
 
 /* What differs with the kind of x: the matrix core's operand of eight k, its accumulator, and how a
- * word of eight codes and eight elements of x become operands.  PARTS: operands an x vector makes. */
+ * word of eight codes and eight elements of x become operands.  PARTS: operands an x vector makes.  zero(z): a zero
+ * point as weights() takes it; ZIN: weights() are n - z, else n. */
 template <int X> struct W4X;
 
 template <> struct W4X<THHIP_F16> {
@@ -40,15 +41,16 @@ template <> struct W4X<THHIP_F16> {
 	typedef halfx8 V;
 	typedef floatx4 A;
 	static constexpr int PARTS = 1;
-	static __device__ __forceinline__ V ones() { return (V)(_Float16)1.0f; }
-	static __device__ __forceinline__ V minus8() { return (V)(_Float16)-8.0f; }
-	static __device__ __forceinline__ V weights(unsigned w)
+	static constexpr bool ZIN = true;
+	static __device__ __forceinline__ unsigned zero(int z) { return __builtin_bit_cast(unsigned short, (_Float16)-z) * 0x10001u; }
+	static __device__ __forceinline__ V weights(unsigned w, unsigned z)
 	{
 		typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 		const unsigned lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
 		const h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.0f, true);
 		const h2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.0f, true);
-		return (V){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+		const h2 m = __builtin_bit_cast(h2, z), e = a + m, f = b + m, g = c + m, h = d + m;
+		return (V){e[0], e[1], f[0], f[1], g[0], g[1], h[0], h[1]};
 	}
 	static __device__ __forceinline__ A mma(V a, V b, A c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 	static __device__ __forceinline__ void operand(const E8 x, V *out) { out[0] = x; }
@@ -60,9 +62,11 @@ template <> struct W4X<THHIP_BF16> {
 	typedef bf16x8 V;
 	typedef floatx4 A;
 	static constexpr int PARTS = 1;
+	static constexpr bool ZIN = false;
+	static __device__ __forceinline__ unsigned zero(int z) { return __float_as_uint((float)-z); }
 	static __device__ __forceinline__ V ones() { return (V)(__bf16)1.0f; }
 	static __device__ __forceinline__ V minus8() { return (V)(__bf16)-8.0f; }
-	static __device__ __forceinline__ V weights(unsigned w)
+	static __device__ __forceinline__ V weights(unsigned w, unsigned)
 	{
 		typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 		const unsigned lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
@@ -82,9 +86,11 @@ template <> struct W4X<THHIP_F32> {
 	typedef bf16x8 V;
 	typedef floatx4 A;
 	static constexpr int PARTS = 3;
+	static constexpr bool ZIN = false;
+	static __device__ __forceinline__ unsigned zero(int z) { return __float_as_uint((float)-z); }
 	static __device__ __forceinline__ V ones() { return W4X<THHIP_BF16>::ones(); }
 	static __device__ __forceinline__ V minus8() { return W4X<THHIP_BF16>::minus8(); }
-	static __device__ __forceinline__ V weights(unsigned w) { return W4X<THHIP_BF16>::weights(w); }
+	static __device__ __forceinline__ V weights(unsigned w, unsigned z) { return W4X<THHIP_BF16>::weights(w, z); }
 	static __device__ __forceinline__ A mma(V a, V b, A c) { return W4X<THHIP_BF16>::mma(a, b, c); }
 	static __device__ __forceinline__ void operand(const E8 x, V *out)
 	{
@@ -113,12 +119,13 @@ template <> struct W4X<W4_X_I8> {
 	typedef long V;
 	typedef intx4 A;
 	static constexpr int PARTS = 1;
-	static __device__ __forceinline__ V ones() { return 0x0101010101010101l; }
-	static __device__ __forceinline__ V minus8() { return 0; }	/* (codes are signed already) */
-	static __device__ __forceinline__ V weights(unsigned w)
+	static constexpr bool ZIN = true;
+	static __device__ __forceinline__ unsigned zero(int z) { return __builtin_amdgcn_perm(z, z, 0); }
+	/* (128 + n - z in every byte, which none borrows from another, without the 128) */
+	static __device__ __forceinline__ V weights(unsigned w, unsigned z)
 	{
-		const unsigned s = w ^ 0x88888888u;
-		return (V)((unsigned long)((s << 4) & 0xf0f0f0f0u) | (unsigned long)(s & 0xf0f0f0f0u) << 32);
+		const unsigned lo = ((w & 0x0f0f0f0fu) | 0x80808080u) - z, hi = ((w >> 4 & 0x0f0f0f0fu) | 0x80808080u) - z;
+		return (V)((unsigned long)(lo ^ 0x80808080u) | (unsigned long)(hi ^ 0x80808080u) << 32);
 	}
 	static __device__ __forceinline__ A mma(V a, V b, A c) { return __builtin_amdgcn_mfma_i32_16x16x32_i8(a, b, c, 0, 0, 0); }
 	static __device__ __forceinline__ void operand(const E8 x, V *out) { out[0] = __builtin_bit_cast(V, x); }

@@ -8,16 +8,18 @@
  * fp32 scales, x[b][k] = sx[b][g'] * q[b][k].  The reference's Linear (modules/Linear.c:72-113)
  * knows fp32 weights only; its 8-bit path (lowp_basic.c:299-321) one range for the whole matrix.
  *
- * Arithmetic.  Inside a group the matrix cores sum n * x with the codes as they are (0 .. 15 is
- * exact in every type) and, with a matrix of ones, sum x; both in fp32 (int32 for 8-bit x, where
- * they are exact).  A finished group adds s * (sum n x - z * sum x) to the fp32 result, so a
- * weight is never rounded and the scale is applied once a group.  fp32 x is cut into three bf16
- * parts of eight bits each that add up to it exactly.
+ * Arithmetic.  Inside a group the matrix cores sum (n - z) * x, whole numbers that every type holds, in
+ * fp32 (int32 for 8-bit x, where the sum is exact).  A finished group adds s times that to the fp32
+ * result, so a weight is never rounded and the scale is applied once a group.  z is taken from the codes where
+ * an instruction does it for two or four of them (fp16 and 8-bit x); with bf16 operands the sums are of n x and,
+ * by a matrix of ones, of x, and a group adds s * (sum n x - z * sum x) (4096 x 8192 -> 8192 with zero points, us:
+ * fp16 one way 532, the other 610).  fp32 x is cut into three bf16 parts of eight bits each that add up to it exactly.
  *
  * A code becomes a half value without an integer conversion: the byte 0000nnnn read as an e4m3
  * number is n * 2^-9 for all sixteen codes (eight denormals, eight of the first binade), and
- * v_cvt_scalef32_pk_{f16,bf16}_fp8 widens two of them with a factor of 2^9.  For 8-bit x the
- * nibble goes to the high half of its byte, where it is 16 (n - 8) once its top bit is flipped.
+ * v_cvt_scalef32_pk_{f16,bf16}_fp8 widens two of them with a factor of 2^9.  For 8-bit x z is taken
+ * from four bytes 128 + n in one subtraction, in which none borrows from another, and a flipped top bit takes the
+ * 128 away.
  *
  * Weights are packed by thhip_w4_pack into one buffer:
  *   codes   [16-row block][step of 128 k][lane][4 words], word j of lane l: row l % 16,
@@ -336,7 +338,7 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args all, in
 #pragma unroll
 		for (int i = 0; i < XS; i++)
 			if (XS * T == ROWS * SLOTS || tid + i * T < ROWS * SLOTS)
-				lxs[(c & 1) * (ROWS * SLOTS) + tid + i * T] = a.xgroups > 1 ? 0.0625f * xs[i] : 0.0625f;
+				lxs[(c & 1) * (ROWS * SLOTS) + tid + i * T] = a.xgroups > 1 ? xs[i] : 1.0f;
 	};
 	/* where a lane's operands lie: in either buffer, or among the zeros; of matrix instruction j at ^ j * 32 * ES */
 	int at[2][NB];
@@ -390,11 +392,11 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args all, in
 					V w[RB];
 #pragma unroll
 					for (int r = 0; r < RB; r++)
-						w[r] = K::weights(now.codes[r][j]);
+						w[r] = K::weights(now.codes[r][j], K::zero(ZP ? now.z[r][j / GM] : 8));
 #pragma unroll
 					for (int n = 0; n < NB; n++) {
 						const V x = *(const V *)(lds + (at[u & 1][n] ^ j * 32 * ES));
-						if constexpr (X != W4_X_I8 || ZP)
+						if constexpr (!K::ZIN)
 							sx[n] = K::mma(x, K::ones(), j % GM ? sx[n] : (A)0);
 #pragma unroll
 						for (int r = 0; r < RB; r++)
@@ -410,15 +412,17 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args all, in
 #pragma unroll
 					for (int r = 0; r < RB; r++) {
 						const float s = now.scale(a, r, j / GM, lane);
-						const int z = ZP ? now.z[r][j / GM] : 8;
+						const float z = ZP ? (float)now.z[r][j / GM] : 8.0f;
 #pragma unroll
 						for (int n = 0; n < NB; n++)
 #pragma unroll
 							for (int i = 0; i < 4; i++) {
 								if constexpr (X == W4_X_I8)
-									acc[r][n][i] += s * xn[n][i] * (float)(p[r][n][i] + (ZP ? __mul24(128 - 16 * z, sx[n][i]) : 0));
+									acc[r][n][i] += s * xn[n][i] * (float)p[r][n][i];
+								else if constexpr (K::ZIN)
+									acc[r][n][i] += s * p[r][n][i];
 								else
-									acc[r][n][i] += s * (p[r][n][i] - (float)z * sx[n][i]);
+									acc[r][n][i] += s * (p[r][n][i] - z * sx[n][i]);
 							}
 					}
 					/* (now, not at the end of the step, for which the registers do not last) */

@@ -4,9 +4,9 @@
  * A workgroup of four wavefronts computes 128 rows for BN columns, a wavefront 64 rows x BN / 2.  x goes
  * through LDS a step of 128 k at a time (two buffers); codes go from memory to registers, one step ahead, and
  * become operands there: the operands of a whole step stay (64 registers) while its columns are walked 16 at a
- * time, so that the sums of one group of 16 columns are all there is beside the result.  During a step's last
- * columns its operands are replaced, one after the other, by the next step's.  The sums of a group start at
- * -z * sum x, so that what is left when it ends is one multiply-add a value.
+ * time, so that the sums of one group of 16 columns (of two, the last one's being added to the result while the next
+ * are multiplied) are all there is beside the result.  The sums of a group start at 0 or, where
+ * z is not in the operands, at -z * sum x, so that what is left when it ends is one multiply-add a value.
  * fp32 x is three planes of bf16 in LDS (BN = 64); 8-bit x is multiplied 64 k at a time (32 for groups of 32).
  * LDS rows are 128 k of a column; a 16-byte vector v of row r lies in slot v ^ r % 16 (8-bit x: v ^ r / 2 % 8),
  * which puts the 16 columns of an operand on different banks.  DMA: rows that memory holds in whole, aligned
@@ -20,9 +20,7 @@ template <int X, bool WIDE> struct W4Tile {		/* operands of 32 k, as W4X has the
 	typedef typename W4X<X>::V V;
 	typedef typename W4X<X>::A A;
 	static constexpr int MK = 32;
-	static __device__ __forceinline__ V ones() { return W4X<X>::ones(); }
-	static __device__ __forceinline__ V minus8() { return W4X<X>::minus8(); }
-	static __device__ __forceinline__ V weights(const uintx4 &c, int j) { return W4X<X>::weights(c[j]); }
+	static __device__ __forceinline__ V weights(const uintx4 &c, int j, unsigned z) { return W4X<X>::weights(c[j], z); }
 	static __device__ __forceinline__ A mma(V a, V b, A c) { return W4X<X>::mma(a, b, c); }
 	/* at: the row's address; r: the row in the tile; q: lane / 16 */
 	static __device__ __forceinline__ V read(const unsigned char *at, int r, int j, int q)
@@ -43,9 +41,7 @@ template <> struct W4Tile<W4_X_I8, true> {		/* 8-bit operands of 64 k: two of 32
 	{
 		return (V){(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
 	}
-	static __device__ __forceinline__ V ones() { return (V)0x01010101; }
-	static __device__ __forceinline__ V minus8() { return (V)0; }		/* (codes are signed already) */
-	static __device__ __forceinline__ V weights(const uintx4 &c, int j) { return join(H::weights(c, 2 * j), H::weights(c, 2 * j + 1)); }
+	static __device__ __forceinline__ V weights(const uintx4 &c, int j, unsigned z) { return join(H::weights(c, 2 * j, z), H::weights(c, 2 * j + 1, z)); }
 	static __device__ __forceinline__ A mma(V a, V b, A c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 	static __device__ __forceinline__ V read(const unsigned char *at, int r, int j, int q)
 	{
@@ -81,17 +77,17 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 	constexpr int PLANE = BN * ROW, STAGE = PARTS * PLANE;
 	constexpr int NJ = W4_KSTEP / M::MK, GJ = GM * 32 / M::MK;	/* matrix instructions of a step, of a group */
 	constexpr int PIECES = BN * 16 / 256;			/* vectors of eight k a thread moves a step */
-	constexpr int CORR = X != W4_X_I8;
+	constexpr bool CORR = !K::ZIN;
 	constexpr int NG = 4 / GM;				/* groups of a step */
 	/* One array: between the loads into LDS and reads of another array the compiler waits for all of the loads.  x; the
-	 * 128 rows' scales of a step's groups; zeros: -z, or (8-bit x) 128 - 16 z as an int; and the scales of x where a
-	 * row has several */
+	 * 128 rows' scales of a step's groups; zeros as zero() makes them; and the scales of x where a row has several */
 	constexpr int SCALES = 2 * NG * 512, ZEROS = ZP ? SCALES : 0, XSCALES = XG ? SCALES : 0;
 	__shared__ __align__(16) unsigned char all_lds[KS * (2 * STAGE + SCALES + ZEROS + XSCALES)];
 	const int part = KS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;	/* the wavefronts of one take every KS-th step */
 	const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	unsigned char *lds = all_lds + part * (2 * STAGE + SCALES + ZEROS + XSCALES);
-	float (*lscale)[NG][128] = (float (*)[NG][128])(lds + 2 * STAGE), (*lzero)[NG][128] = (float (*)[NG][128])(lds + 2 * STAGE + SCALES);
+	float (*lscale)[NG][128] = (float (*)[NG][128])(lds + 2 * STAGE);
+	unsigned (*lzero)[NG][128] = (unsigned (*)[NG][128])(lds + 2 * STAGE + SCALES);
 	float (*lxs)[NG][BN] = (float (*)[NG][BN])(lds + 2 * STAGE + SCALES + ZEROS);
 	const int col = lane & 15, quarter = lane >> 4;
 
@@ -152,7 +148,8 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 		}
 	};
 	/* scales and zeros: thread i fetches row i % 128's, and puts them into LDS at the end of the step */
-	float gs[NG], gz[NG], gx[NG];
+	float gs[NG], gx[NG];
+	unsigned char gz[NG];
 	const int grb = mt * 8 + (tid >> 4 & 7) < a.blocks ? mt * 8 + (tid >> 4 & 7) : a.blocks - 1;
 	auto g_issue = [&](int t) {
 #pragma unroll
@@ -160,7 +157,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 			const long at = ((long)grb * a.groups + a.group_of(t, g * GM)) * 16 + (tid & 15);
 			gs[g] = w4_get<X>(a.scales, at, a.dtype);
 			if constexpr (ZP)
-				gz[g] = X == W4_X_I8 ? __int_as_float(128 - 16 * (int)a.zeros[at]) : -(float)a.zeros[at];
+				gz[g] = a.zeros[at];
 			if constexpr (XG)
 				gx[g] = a.xscale[(long)(b0 + ((tid & 127) < nrows ? tid & 127 : 0)) * a.xgroups + a.group_of(t, g * GM)];
 		}
@@ -168,9 +165,9 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 	auto g_land = [&](int buf) {
 #pragma unroll
 		for (int g = 0; g < NG; g++) {
-			lscale[buf][g][tid & 127] = X == W4_X_I8 ? 0.0625f * gs[g] : gs[g];	/* (codes of weights were 16 times theirs) */
+			lscale[buf][g][tid & 127] = gs[g];
 			if constexpr (ZP)
-				lzero[buf][g][tid & 127] = gz[g];
+				lzero[buf][g][tid & 127] = K::zero(gz[g]);
 			if constexpr (XG)
 				lxs[buf][g][tid & 127] = gx[g];
 		}
@@ -249,13 +246,13 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 		};
 		/* sum of x over unit u's group, for every row (without zero points -8 times that: 8 is the zero) */
 		auto x_add = [&](int u, int i) {	/* the i-th of the group's GJ pieces */
-			if constexpr (CORR || ZP) {
+			if constexpr (CORR) {
 				const int n = u / NG, j = u % NG * GJ + i;
 				if (i == 0)
 					sx[u & 1] = (A)0;
 #pragma unroll
 				for (int q = 0; q < PARTS; q++)
-					sx[u & 1] = M::mma(x[AHEAD ? n & 1 : 0][q][j], ZP ? M::ones() : M::minus8(), sx[u & 1]);
+					sx[u & 1] = M::mma(x[AHEAD ? n & 1 : 0][q][j], ZP ? K::ones() : K::minus8(), sx[u & 1]);
 			}
 		};
 		auto x_sum = [&](int u) {
@@ -268,10 +265,14 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 		x_issue(t1, buf ^ 1, 0);
 		x_read(0);
 #pragma unroll
-		for (int j = 0; j < NJ; j++)
+		for (int g = 0; g < NG; g++)
 #pragma unroll
-			for (int r = 0; r < 4; r++)
-				w[r][j] = M::weights(codes[r], j);
+			for (int r = 0; r < 4; r++) {
+				const unsigned z = K::ZIN && ZP ? lzero[buf][g][own + r * 16] : K::zero(8);
+#pragma unroll
+				for (int j = 0; j < GJ; j++)
+					w[r][g * GJ + j] = M::weights(codes[r], g * GJ + j, z);
+			}
 		if (AHEAD)
 			x_sum(0);
 		if (LATE && i > 0)
@@ -296,18 +297,14 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 				x_sum(u);
 #pragma unroll
 			for (int r = 0; r < 4; r++) {
-				if constexpr (ZP) {
-					const float z = lzero[buf][g][own + r * 16];
-#pragma unroll
-					for (int i = 0; i < 4; i++) {
-						if constexpr (X == W4_X_I8)
-							p[PIPE ? u & 1 : 0][r][i] = __mul24(__float_as_int(z), sx[u & 1][i]);
-						else
-							p[PIPE ? u & 1 : 0][r][i] = z * sx[u & 1][i];
-					}
-				} else if constexpr (X == W4_X_I8)
+				if constexpr (!CORR)
 					p[PIPE ? u & 1 : 0][r] = (A)0;
-				else
+				else if constexpr (ZP) {
+					const float z = __uint_as_float(lzero[buf][g][own + r * 16]);
+#pragma unroll
+					for (int i = 0; i < 4; i++)
+						p[PIPE ? u & 1 : 0][r][i] = z * sx[u & 1][i];
+				} else
 					p[PIPE ? u & 1 : 0][r] = sx[u & 1];
 			}
 			/* (the next unit's sum of x, whose pieces wait for each other, between the products) */
