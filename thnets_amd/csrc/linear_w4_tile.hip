@@ -1,9 +1,11 @@
 /*
  * 4-bit Linear layers (linear_w4.hip) for larger batches: bound by the matrix cores.
  *
- * A workgroup of four wavefronts computes 128 rows for BN columns, a wavefront 64 rows x BN / 2.  x goes
+ * A workgroup of four wavefronts computes 128 rows for BN columns, a wavefront 64 rows x BN / 2 or, where the operands
+ * hold the zero points and no sums of x are needed, 32 rows x BN, for which half as many codes become
+ * operands (4096 x 8192 -> 8192 fp16 550 -> 505 us; bf16, whose sums of x would be twice as many, stays).  x goes
  * through LDS a step of 128 k at a time (two buffers); codes go from memory to registers, one step ahead, and
- * become operands there: the operands of a whole step stay (64 registers) while its columns are walked 16 at a
+ * become operands there: those of a whole step stay (32 or 64 registers) while its columns are walked 16 at a
  * time, so that the sums of one group of 16 columns (of two, the last one's being added to the result while the next
  * are multiplied) are all there is beside the result.  The sums of a group start at 0 or, where
  * z is not in the operands, at -z * sum x, so that what is left when it ends is one multiply-add a value.
@@ -64,14 +66,23 @@ __device__ __forceinline__ float w4_get(const void *p, long i, int dtype)
 	}
 }
 
+/* Wavefronts of a SIMD: with 8-bit x LDS has room for three workgroups (4096 x 8192 -> 8192, us: 387 with two, 352), with
+ * fp32 x for one or two */
+constexpr int w4_tile_waves(int x, bool dma, int ks, bool most)
+{
+	return x == W4_X_I8 && dma && ks == 1 ? 3 : x == THHIP_F32 && !most ? 1 : 2;
+}
+
 template <int X, int GM, bool ZP, bool XG, bool DMA, int KS>
-__global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == THHIP_F32 ? 1 : 2, 2))) void w4_tile_kernel(const w4_args a, int mtiles, int ntiles)
+__global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_tile_waves(X, DMA, KS, false), w4_tile_waves(X, DMA, KS, true)))) void w4_tile_kernel(const w4_args a, int mtiles, int ntiles)
 {
 	typedef W4X<X> K;
 	typedef W4Tile<X, X == W4_X_I8 && GM >= 2> M;
 	typedef typename M::V V;
 	typedef typename M::A A;
-	constexpr int PARTS = K::PARTS, NB = PARTS > 1 ? 2 : 4, BN = 32 * NB;
+	constexpr int PARTS = K::PARTS, BN = PARTS > 1 ? 64 : 128;
+	/* row blocks of a wavefront, and blocks of 16 columns */
+	constexpr int R = K::ZIN ? 2 : 4, NB = BN / (8 * R);
 	constexpr int ES = sizeof(typename K::V) / 8;
 	constexpr int ROW = W4_KSTEP * ES;			/* bytes of a row in LDS */
 	constexpr int PLANE = BN * ROW, STAGE = PARTS * PLANE;
@@ -103,7 +114,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 	}
 	const int mt = id / ntiles, nt = id - mt * ntiles;
 	const int b0 = nt * BN, nrows = a.B - b0 < BN ? a.B - b0 : BN;
-	const int rb0 = mt * 8 + (wave & 1) * 4, c0 = (wave >> 1) * NB * 16;
+	const int wrow = wave % (8 / R), rb0 = mt * 8 + wrow * R, c0 = wave / (8 / R) * NB * 16;
 
 	const typename K::E *xbase = (const typename K::E *)a.x + (long)b0 * a.ldx;
 	const unsigned xend = DMA ? (unsigned)(((nrows - 1) * a.ldx + a.nIn) * (long)sizeof(typename K::E)) : 0;
@@ -172,10 +183,10 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 				lxs[buf][g][tid & 127] = gx[g];
 		}
 	};
-	uintx4 codes[4];
+	uintx4 codes[R];
 	auto codes_issue = [&](int t) {
 #pragma unroll
-		for (int r = 0; r < 4; r++) {
+		for (int r = 0; r < R; r++) {
 			const int rb = rb0 + r < a.blocks ? rb0 + r : a.blocks - 1;
 			codes[r] = *(const uintx4 *)(a.codes + ((size_t)rb * a.steps + t) * 1024 + lane * 16);
 		}
@@ -185,9 +196,9 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 		asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 	};
 
-	floatx4 acc[4][NB];
+	floatx4 acc[R][NB];
 #pragma unroll
-	for (int r = 0; r < 4; r++)
+	for (int r = 0; r < R; r++)
 #pragma unroll
 		for (int n = 0; n < NB; n++)
 			acc[r][n] = (floatx4)0.0f;
@@ -206,10 +217,10 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 
 	constexpr int NU = NB * NG;		/* units of a step: 16 columns x one group */
 	/* a unit's sums are added to the result while the next unit is multiplied, where the registers last */
-	constexpr bool PIPE = DMA && KS == 1;
-	constexpr bool AHEAD = KS == 1;		/* ... and the next unit's operands are read */
-	const int own = (wave & 1) * 64 + col;	/* the lane's row of the first row block */
-	A p[PIPE ? 2 : 1][4];
+	constexpr bool PIPE = DMA && (KS == 1 || K::ZIN);
+	constexpr bool AHEAD = KS == 1 || K::ZIN;		/* ... and the next unit's operands are read */
+	const int own = wrow * R * 16 + col;	/* the lane's row of the first row block */
+	A p[PIPE ? 2 : 1][R];
 	/* unit u's finished sums into the result (buf: where its step's scales are) */
 	auto flush_at = [&](int u, int buf) {
 		const int n = u / NG, g = u % NG;
@@ -217,7 +228,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 		if constexpr (XG)
 			xs = *(const floatx4 *)&lxs[buf][g][c0 + n * 16 + 4 * quarter];
 #pragma unroll
-		for (int r = 0; r < 4; r++) {
+		for (int r = 0; r < R; r++) {
 			const float s = lscale[buf][g][own + r * 16];
 #pragma unroll
 			for (int i = 0; i < 4; i++)
@@ -226,7 +237,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 			asm("" : "+v"(acc[r][n]));
 		}
 	};
-	constexpr bool LATE = PIPE && NG == 1 && PARTS == 1;	/* a step's last sums are added at the start of the next */
+	constexpr bool LATE = PIPE && KS == 1 && NG == 1 && PARTS == 1;	/* a step's last sums are added at the start of the next */
 	const int rounds = (a.steps + KS - 1) / KS;
 	for (int i = 0; i < rounds; i++) {
 		const int t = i * KS + part, buf = i & 1, t1 = t + KS < a.steps ? t + KS : a.steps - 1;
@@ -235,7 +246,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 			break;
 		}
 		const unsigned char *base = lds + buf * STAGE + (c0 + col) * ROW;
-		V w[4][NJ], x[AHEAD ? 2 : 1][PARTS][NJ];
+		V w[R][NJ], x[AHEAD ? 2 : 1][PARTS][NJ];
 		A sx[2];
 		auto x_read = [&](int n) {
 #pragma unroll
@@ -267,7 +278,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 #pragma unroll
 		for (int g = 0; g < NG; g++)
 #pragma unroll
-			for (int r = 0; r < 4; r++) {
+			for (int r = 0; r < R; r++) {
 				const unsigned z = K::ZIN && ZP ? lzero[buf][g][own + r * 16] : K::zero(8);
 #pragma unroll
 				for (int j = 0; j < GJ; j++)
@@ -296,7 +307,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 			if (!AHEAD)
 				x_sum(u);
 #pragma unroll
-			for (int r = 0; r < 4; r++) {
+			for (int r = 0; r < R; r++) {
 				if constexpr (!CORR)
 					p[PIPE ? u & 1 : 0][r] = (A)0;
 				else if constexpr (ZP) {
@@ -314,7 +325,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 #pragma unroll
 				for (int q = 0; q < PARTS; q++)
 #pragma unroll
-					for (int r = 0; r < 4; r++)
+					for (int r = 0; r < R; r++)
 						p[PIPE ? u & 1 : 0][r] = M::mma(x[AHEAD ? n & 1 : 0][q][j], w[r][j], p[PIPE ? u & 1 : 0][r]);
 				if (AHEAD && u + 1 < NU && i > 0)
 					x_add(u + 1, i - 1);
@@ -325,11 +336,11 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 				flush(PIPE ? u - 1 : u);
 			if constexpr (PIPE && (X == THHIP_F16 || X == THHIP_BF16)) {
 			/* the order to issue them in: what comes from LDS, then a matrix instruction and the sums' work in turn */
-			__builtin_amdgcn_sched_group_barrier(0x100, PARTS * NJ + 4, 0);
+			__builtin_amdgcn_sched_group_barrier(0x100, PARTS * NJ + R, 0);
 			if constexpr (ZP)
 				__builtin_amdgcn_sched_group_barrier(0x2, 16, 0);
 #pragma unroll
-			for (int i = 0; i < 5 * GJ * PARTS; i++) {
+			for (int i = 0; i < (R + CORR) * GJ * PARTS; i++) {
 				__builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
 				__builtin_amdgcn_sched_group_barrier(0x2, 1, 0);
 			}
@@ -353,24 +364,24 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(X == T
 		for (int p = 1; p < KS; p++)
 			if (part == p)
 #pragma unroll
-				for (int r = 0; r < 4; r++)
+				for (int r = 0; r < R; r++)
 #pragma unroll
 					for (int n = 0; n < NB; n++)
-						sums[(((p - 1) * 4 + r) * NB + n) * 256 + tid] = acc[r][n];
+						sums[(((p - 1) * R + r) * NB + n) * 256 + tid] = acc[r][n];
 		barrier();
 		if (part)
 			return;
 #pragma unroll
 		for (int p = 1; p < KS; p++)
 #pragma unroll
-			for (int r = 0; r < 4; r++)
+			for (int r = 0; r < R; r++)
 #pragma unroll
 				for (int n = 0; n < NB; n++)
-					acc[r][n] += sums[(((p - 1) * 4 + r) * NB + n) * 256 + tid];
+					acc[r][n] += sums[(((p - 1) * R + r) * NB + n) * 256 + tid];
 	}
 
 #pragma unroll
-	for (int r = 0; r < 4; r++) {
+	for (int r = 0; r < R; r++) {
 		const int o = (rb0 + r) * 16 + col;
 		const float bias = a.bias && o < a.nOut ? a.bias[o] : 0.0f;
 #pragma unroll
@@ -397,10 +408,10 @@ static void w4_tile_launch(const w4_args &all)
 	constexpr size_t esx = sizeof(typename W4X<X>::E);
 	const size_t esy = thhip_esize(all.dtype);
 	constexpr int BN = W4X<X>::PARTS > 1 ? 64 : 128;
-	/* K in two halves where there are fewer tiles than CUs (1024 x 4096 -> 4096, us: 8-bit x 73 -> 57, groups of 32 130 ->
-	 * 113); half types with larger groups keep the matrix cores as busy with four wavefronts (64 and 64; with
-	 * zero points 68 and 73) */
-	constexpr bool HALVES = X == W4_X_I8 || GM == 1;
+	/* K in two halves where there are fewer tiles than CUs (1024 x 4096 -> 4096, us, without and with: 8-bit x 73 -> 57, fp16
+	 * groups of 64 65 -> 54, bf16 groups of 32 130 -> 113); bf16 with larger groups keeps the matrix cores as busy
+	 * with four wavefronts (64 and 64; with zero points 68 and 73) */
+	constexpr bool HALVES = X != THHIP_F32 && (W4X<X>::ZIN || GM == 1);
 	for (int b0 = 0; b0 < all.B; b0 += W4_TILE_ROWS) {
 		const w4_args a = w4_rows(all, b0, all.B - b0 < W4_TILE_ROWS ? all.B - b0 : W4_TILE_ROWS, esx, esy);
 		const int mtiles = (a.blocks + 7) / 8, ntiles = (a.B + BN - 1) / BN;
