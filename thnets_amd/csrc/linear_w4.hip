@@ -229,7 +229,12 @@ extern "C" void thhip_w4_set_shape(int shape)
  * different banks.
  * Of a 16 x 16 tile a lane holds row lane % 16, whose scale and zero point it needs, of columns 4 (lane / 16) + 0 .. 3.  The wavefronts' sums are
  * added through LDS, in their order, and an fp32 row's three columns with them.
- * GM: matrix instructions a group spans within a step (1: groups of 32 or 64, 4: larger). */
+ * GM: matrix instructions a group spans within a step (1: groups of 32 or 64, 4: larger).
+ *
+ * Bound by memory where the layer is large: 1 x 8192 -> 32768 bf16 25.4 us (138 MB, 5.4 TB/s; a large copy moves 5.1),
+ * 1 x 25088 -> 4096 fp32 14.1 us (53 MB, 3.8 TB/s: 256 workgroups, one a CU, whose start and end do not overlap), 1 x
+ * 4096 -> 16384 with 8-bit x 9.3 us (35 MB, 3.7 TB/s).  By the vector unit (codes to operands) and the L2's x from about
+ * 32 columns on: 128 x 4096 -> 4096 fp16 12.8 us (338 TFLOP/s). */
 
 /* The workgroup's LDS traffic so far is done, for everybody (loads from memory may still be on their way) */
 __device__ __forceinline__ void w4_lds_barrier(void)

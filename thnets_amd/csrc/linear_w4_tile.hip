@@ -1,5 +1,8 @@
 /*
- * 4-bit Linear layers (linear_w4.hip) for larger batches: bound by the matrix cores.
+ * 4-bit Linear layers (linear_w4.hip) for larger batches: bound by the matrix cores and by the instructions between
+ * theirs, of which a wavefront issues one where it could issue a matrix instruction (codes to operands, a group's sums to
+ * the result).  4096 x 8192 -> 8192, us and 10^12 a second: fp16 490 to 505 and 1100, bf16 527 to 610 and 900 to 1040 (a library's
+ * product of 8192^3: 1150 and 1201), 8-bit x 350 and 1570 (1779); fp32 x 2200 and 250 (149).
  *
  * A workgroup of four wavefronts computes 128 rows for BN columns, a wavefront 64 rows x BN / 2 or, where the operands
  * hold the zero points and no sums of x are needed, 32 rows x BN, for which half as many codes become
@@ -14,6 +17,8 @@
  * which puts the 16 columns of an operand on different banks.  DMA: rows that memory holds in whole, aligned
  * 16-byte vectors are loaded straight into LDS; others go through registers.
  * KS: where there are fewer tiles than CUs, eight wavefronts share a tile, four taking every other step of K.
+ * Instructions of 32 x 32 outputs in place of 16 x 16 took as long (fp16 490 -> 504 us, 8-bit x 342 -> 384): what they
+ * save in issue they need in registers, of which 8-bit x then has too few for a third workgroup.
  */
 #include <stdint.h>
 #include "linear_w4.h"

@@ -18,6 +18,10 @@
  * h w and its maximum; where the fp32 quotient is next to the middle between two
  * codes it is taken again in 64 bits, so that the value goes to the nearer one: without
  * that one value in 30000 of fp16 rows did not.
+ *
+ * Time alone on the GPU, us (a large copy moves 5.1 TB/s): norm of 16384 rows of 8192 bf16 with a residual 182 (1074 MB,
+ * 5.9 TB/s), of 333 rows of 5003 fp32 5.7 (13 MB, 2.3 TB/s: half of it is the way of one row through the GPU, 2.4 us);
+ * with codes 8192 rows of 4096 bf16 47 (235 MB, 5.0 TB/s); codes alone 700 rows of 9216 fp16 7.7 (19 MB, 2.5 TB/s).
  */
 #include <stdint.h>
 #include <stdio.h>
@@ -40,8 +44,8 @@ struct rows_args {
 /* N consecutive elements of a row (16 bytes), which need no more than the element's alignment here.
  * fetch() loads without a branch, so that all of a thread's loads are on their way together: a vector that the
  * row's end cuts or that lies behind it is read from the row's last N elements (cols >= N), and widen() puts
- * it right afterwards, elements past the end being 0.  A branch round each load made the compiler wait for one before
- * the next: 2.5 times the time of a row of 4096. */
+ * it right afterwards, elements past the end being 0.  With a branch round each load the compiler waited for one before
+ * the next (8192 rows of 4096 bf16 with codes 56 us, without 47; codes of 700 rows of 9216 fp16 11.1 and 7.7). */
 template <int DT> struct RowVec {
 	static constexpr int N = DT == THHIP_F32 ? 4 : 8;
 	typedef typename ThhipElem<DT>::T T;
@@ -270,7 +274,9 @@ __device__ __forceinline__ void row_out(const rows_args &a, long row, int col, c
 	}
 }
 
-/* Rows of at most T * V vectors, T threads a row, each of which keeps its V vectors in registers. */
+/* Rows of at most T * V vectors, T threads a row, each of which keeps its V vectors in registers: a wavefront for rows of
+ * up to two vectors a lane (four rows a workgroup, no barrier), 256 threads up to eight, so that several rows share a CU
+ * and one's loads run under another's sums, 1024 beyond. */
 template <int DT, int MODE, int T, int V>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const rows_args a)
 {
@@ -525,7 +531,8 @@ extern "C" int thhip_quantize_rows(const void *x, long ldx, signed char *q, long
 }
 
 /* y = q * scale.  TX threads (a power of two) walk a row eight columns at a time; a group is a whole
- * number of such vectors. */
+ * number of such vectors.  Bound by memory: 8192 rows of 4096 to bf16 16.7 us (101 MB, 6.0 TB/s), 700 of 9216 to fp16
+ * 6.0 us (19 MB, 3.2 TB/s). */
 template <int DT>
 __global__ __launch_bounds__(256) void dequantize_rows_kernel(const signed char *q, long ldq, const float *scale, int group,
 	int ngroups, void *y, long ldy, long rows, int cols, int tx)
