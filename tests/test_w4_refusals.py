@@ -1,5 +1,8 @@
 """What the entry points of 4-bit layers and of norms with 8-bit outputs refuse: before anything touches a GPU, with -1
 and a message; and that no rows are no launch.  Runs without a GPU: the pointers are never followed."""
+import os
+import subprocess
+
 import pytest
 
 from thnets_amd import abi, api
@@ -110,3 +113,9 @@ def test_codes_refuse(lib, capfd):
     assert lib.thhip_quantize_rows(P, 64, P, 64, None, 32, 4, 64, F16) == -1
     assert lib.thhip_dequantize_rows(P, 64, P, 32, None, 64, 4, 64, F16) == -1
     assert lib.thhip_dequantize_rows(None, 64, P, 32, P, 64, 4, 64, F16) == -1
+
+
+def test_the_driver_refuses_other_groups():
+    exe = os.path.join(os.path.dirname(api.LIB_PATH), "thnets-hip-test")
+    out = subprocess.run([exe, "-m", "nowhere", "-i", "random", "-q", "48"], capture_output=True, text=True, timeout=60)
+    assert out.returncode and out.stderr.startswith("Syntax")

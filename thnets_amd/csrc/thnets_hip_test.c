@@ -115,7 +115,8 @@ int main(int argc, char **argv)
 		case 'M': th_minmax = 1; break;
 		}
 	}
-	if (!modelsdir || !inputfile || alg < 8 || alg > 11 || runs < 1) {
+	THHipLinear4Bit(group);		/* (a group that it does not know leaves it at 0) */
+	if (!modelsdir || !inputfile || alg < 8 || alg > 11 || runs < 1 || THHipLinear4Bit(group) != group) {
 		fprintf(stderr, "Syntax: thnets-hip-test -m <models directory> -i <input.t7 | image.ppm | random>\n");
 		fprintf(stderr, "             [-r <number of runs>] [-p(rint results)] [-P(rofile)] [-M(inmax of every layer)]\n");
 		fprintf(stderr, "             [-a <alg=8:HIP fp32 (default), 9:HIP fp16, 10:HIP bf16, 11:HIP 8bit>]\n");
@@ -139,7 +140,6 @@ int main(int argc, char **argv)
 		THMakeSpatial(net, side);
 	if (alg == 9 || alg == 10)
 		THHipHalfFloat(alg == 9 ? 1 : 2);
-	THHipLinear4Bit(group);
 	THNETWORK *dev = alg == 11 ? THCreateHipLowpNetwork(net, range) : THCreateHipNetwork(net);
 	THFreeNetwork(net);
 	net = dev;
