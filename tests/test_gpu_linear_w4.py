@@ -135,6 +135,41 @@ def test_strides_and_offsets(hiplib, dtype, B, ldx, offx, ldy, offy):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group,zeros", [(32, 1), (64, 0), (128, 1), (0, 0)])
+@pytest.mark.parametrize("B,nOut", [(129, 200), (300, 257)])
+def test_rows_of_whole_vectors_that_end_inside_a_step(hiplib, shape, B, nOut, group, zeros, dtype):
+    """Rows that begin and end on 16 bytes, but not on 128 k, with NaNs behind each: the tile kernel's loads straight into
+    LDS, for a single tile's columns and a part of a third's."""
+    nIn, ldx = 656, 672
+    g, x, b = data(620, B, nIn, nOut, dtype)
+    layer = U.Layer.random(g, nOut, nIn, group, dtype, zeros).lay(hiplib)
+    shape(5)
+    want, mag = U.linear64(layer, x, b)
+    U.check_linear(U.linear(hiplib, layer, x, b, ldx=ldx), want, mag, layer)
+    q = g.integers(-127, 128, (B, nIn)).astype(np.int8)
+    for xgroup in {0, group}:
+        xs = (g.uniform(0.5, 1.5, (B, U.groups_of(nIn, xgroup))) / 64).astype(np.float32)
+        want, mag = U.linear64(layer, q * U.spread_x(xs.astype(np.float64), nIn, group), b)
+        U.check_linear(U.linear(hiplib, layer, q, b, ldx=ldx, xs=xs, xgroup=xgroup), want, mag, layer)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B", [1500, 2100])
+def test_more_tiles_than_the_gpu_holds_at_once(hiplib, dtype, B):
+    """Enough tiles for every form of launch that the size chooses among: one value in 50 is compared."""
+    nIn, nOut = 384, 6000
+    g, x, b = data(630, B, nIn, nOut, dtype)
+    layer = U.Layer.random(g, nOut, nIn, 128, dtype, B == 1500).lay(hiplib)
+    some = U.Layer(layer.codes[::50], layer.scales[::50], layer.zeros[::50] if layer.zeros is not None else None, 128, dtype)
+    want, mag = U.linear64(some, x, b[::50])
+    U.check_linear(U.linear(hiplib, layer, x, b)[:, ::50], want, mag, some)
+    q = g.integers(-127, 128, (B, nIn)).astype(np.int8)
+    xs = (g.uniform(0.5, 1.5, (B, 3)) / 64).astype(np.float32)
+    want, mag = U.linear64(some, q * U.spread_x(xs.astype(np.float64), nIn, 128), b[::50])
+    U.check_linear(U.linear(hiplib, layer, q, b, xs=xs, xgroup=128)[:, ::50], want, mag, some)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("which", range(6))
 @pytest.mark.parametrize("B", [1, 130])
 def test_rows_that_end_with_their_allocation(hiplib, shape, which, B, dtype):

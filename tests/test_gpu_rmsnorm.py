@@ -207,6 +207,48 @@ def test_more_rows_than_a_launch_has(hiplib, rows):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [5, 300, 5000, 70000])
+def test_rows_whose_distance_passes_32_bits(hiplib, dtype, cols):
+    """Three rows of x, the residual, both outputs and the codes, 2^32 bytes of x or 2^31 codes and more after one another."""
+    es = U.ESIZE[dtype]
+    ld = (1 << 32) // es + 40
+    x, r, w = inputs(75, 3, cols, dtype, True, True)
+    near_call = Call(hiplib, x, r, w, dtype)
+    near_codes = Call(hiplib, x, r, w, dtype, group=32)
+    kind = word(dtype)
+
+    def far(a):
+        dev = api.DeviceArray(hiplib, nbytes=2 * ld * a.itemsize + a.shape[1] * a.itemsize)
+        for i in range(3):
+            hiplib.thhip_memcpy_h2d(dev.ptr + i * ld * a.itemsize, np.ascontiguousarray(a[i]).ctypes.data, a[i].nbytes)
+        return dev
+
+    def back(dev, like):
+        out = np.empty_like(like)
+        for i in range(3):
+            hiplib.thhip_memcpy_d2h(out[i].ctypes.data, dev.ptr + i * ld * like.itemsize, like[i].nbytes)
+        return out
+
+    dx, dr, dw = far(U.raw(x, dtype)), far(U.raw(r, dtype)), api.DeviceArray(hiplib, w)
+    empty = np.zeros((3, cols), kind)
+    ds, dy, dq = far(empty), far(empty), far(empty.astype(np.int8))
+    n = U.groups_of(cols, 32)
+    dscale = api.DeviceArray(hiplib, nbytes=3 * n * 4)
+    G.note("far rows 3x%d dtype=%d" % (cols, dtype))
+    assert hiplib.thhip_rmsnorm(dx.ptr, ld, dr.ptr, ld, dw.ptr, EPS, ds.ptr, ld, dy.ptr, ld, 3, cols, dtype) == 0
+    hiplib.thhip_sync()
+    assert np.array_equal(U.unraw(back(ds, empty), dtype), near_call.sum) and np.array_equal(U.unraw(back(dy, empty), dtype), near_call.y)
+    assert hiplib.thhip_rmsnorm_i8(dx.ptr, ld, dr.ptr, ld, dw.ptr, EPS, None, 0, dq.ptr, ld, dscale.ptr, 32, 3, cols, dtype) == 0
+    hiplib.thhip_sync()
+    assert np.array_equal(back(dq, empty.astype(np.int8)), near_codes.q)
+    assert np.array_equal(dscale.get((3, n), np.float32), near_codes.scale)
+    assert hiplib.thhip_dequantize_rows(dq.ptr, ld, dscale.ptr, 32, dy.ptr, ld, 3, cols, dtype) == 0
+    hiplib.thhip_sync()
+    spread = np.repeat(near_codes.scale, 32, 1)[:, :cols]
+    assert np.array_equal(back(dy, empty), U.raw(near_codes.q.astype(np.float32) * spread, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B", [1, 6, 70])
 def test_a_block_of_a_network(hiplib, dtype, B):
     """The operators one after the other, as a network of Linear layers runs them: norm -> 8 bits -> 4-bit layer with
