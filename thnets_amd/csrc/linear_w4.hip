@@ -11,9 +11,10 @@
  * Arithmetic.  Inside a group the matrix cores sum (n - z) * x, whole numbers that every type holds, in
  * fp32 (int32 for 8-bit x, where the sum is exact).  A finished group adds s times that to the fp32
  * result, so a weight is never rounded and the scale is applied once a group.  z is taken from the codes where
- * an instruction does it for two or four of them (fp16 and 8-bit x); with bf16 operands the sums are of n x and,
- * by a matrix of ones, of x, and a group adds s * (sum n x - z * sum x) (4096 x 8192 -> 8192 with zero points, us:
- * fp16 one way 532, the other 610).  fp32 x is cut into three bf16 parts of eight bits each that add up to it exactly.
+ * an instruction does it for two or four of them (fp16 and 8-bit x: 4096 x 8192 -> 8192 with zero points 610 -> 532 us).
+ * bf16 has none: for few rows of x the sums are of n x and, by a matrix of ones, of x, and a group adds
+ * s * (sum n x - z * sum x); larger batches make n - z of the bytes by sign and magnitude.  fp32 x is cut into three
+ * bf16 parts of eight bits each that add up to it exactly.
  *
  * A code becomes a half value without an integer conversion: the byte 0000nnnn read as an e4m3
  * number is n * 2^-9 for all sixteen codes (eight denormals, eight of the first binade), and
@@ -508,7 +509,7 @@ static void w4_skinny_launch(const w4_args &all)
  * slope.  Few rows at a time win in small layers and short K, 64 rows in larger ones (4096 -> 4096 fp16, us, in the
  * order of the table: 128 columns 37 / 24 / 27 / 17.4 / 12.8, tiles 50), tiles from about 512 columns on (768 columns: 81
  * with 64 rows, 56 with tiles).  Of 78 layers drawn at random (16 to 1300 rows, 512 to 9216 inputs, 256 to 10240 outputs) the
- * choice took 1.6 % more than the best shape, 18 % at most. */
+ * choice took 1.7 % more than the best shape, 27 % at most. */
 enum { W4_16x16, W4_32x16, W4_16x32, W4_32x32, W4_64x32, W4_TILES };
 
 static int w4_shape(const w4_args &a, int parts)
@@ -520,8 +521,8 @@ static int w4_shape(const w4_args &a, int parts)
 		{{4.5f, 0.65f}, {6.0f, 1.2f}, {4.4f, 1.35f}, {5.6f, 2.2f}, {8.0f, 3.8f}},	/* ... in groups of 32 and 64 */
 	};
 	static const float tile_us[2][3][2] = {
-		{{13.0f, 10.0f}, {14.0f, 15.5f}, {15.0f, 23.0f}},	/* groups of 128 and more, 64, 32 */
-		{{8.0f, 17.0f}, {8.0f, 24.0f}, {8.0f, 31.0f}},		/* fp32 x */
+		{{13.0f, 10.0f}, {13.0f, 10.7f}, {14.0f, 13.7f}},	/* groups of 128 and more, 64, 32 */
+		{{8.0f, 17.0f}, {8.0f, 19.5f}, {8.0f, 23.0f}},		/* fp32 x */
 	};
 	static const int rows[5] = {1, 2, 1, 2, 4}, cols[5] = {1, 1, 2, 2, 2};	/* blocks of 16 */
 	const float (*us)[2] = round_us[(a.xscale ? 2 : 0) + (a.group == 32 || a.group == 64)];

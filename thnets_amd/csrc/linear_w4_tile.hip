@@ -1,12 +1,12 @@
 /*
  * 4-bit Linear layers (linear_w4.hip) for larger batches: bound by the matrix cores and by the instructions between
  * theirs, of which a wavefront issues one where it could issue a matrix instruction (codes to operands, a group's sums to
- * the result).  4096 x 8192 -> 8192, us and 10^12 a second: fp16 490 to 505 and 1100, bf16 527 to 610 and 900 to 1040 (a library's
+ * the result).  4096 x 8192 -> 8192, us and 10^12 a second: fp16 490 to 505 and 1100, bf16 520 to 535 and 1040 (a library's
  * product of 8192^3: 1150 and 1201), 8-bit x 350 and 1570 (1779); fp32 x 2200 and 250 (149).
  *
  * A workgroup of four wavefronts computes 128 rows for BN columns, a wavefront 64 rows x BN / 2 or, where the operands
- * hold the zero points and no sums of x are needed, 32 rows x BN, for which half as many codes become
- * operands (4096 x 8192 -> 8192 fp16 550 -> 505 us; bf16, whose sums of x would be twice as many, stays).  x goes
+ * are n - z and no sums of x are needed, 32 rows x BN, for which half as many codes become operands (4096 x 8192 ->
+ * 8192 fp16 550 -> 505 us): all but fp32 x with groups longer than 32, whose sums of x would be twice as many.  x goes
  * through LDS a step of 128 k at a time (two buffers); codes go from memory to registers, one step ahead, and
  * become operands there: those of a whole step stay (32 or 64 registers) while its columns are walked 16 at a
  * time, so that the sums of one group of 16 columns (of two, the last one's being added to the result while the next
@@ -21,13 +21,17 @@
  * save in issue they need in registers, of which 8-bit x then has too few for a third workgroup.
  */
 #include <stdint.h>
+#include <type_traits>
 #include "linear_w4.h"
 
-template <int X, bool WIDE> struct W4Tile {		/* operands of 32 k, as W4X has them */
+template <int X, bool SIGNED, bool WIDE> struct W4Tile {		/* operands of 32 k, as W4X has them, or of n - z */
+	typedef typename std::conditional<SIGNED, W4Signed, W4X<X>>::type K;
+	static constexpr bool ZIN = K::ZIN;
 	typedef typename W4X<X>::V V;
 	typedef typename W4X<X>::A A;
 	static constexpr int MK = 32;
-	static __device__ __forceinline__ V weights(const uintx4 &c, int j, unsigned z) { return W4X<X>::weights(c[j], z); }
+	static __device__ __forceinline__ unsigned zero(int z) { return K::zero(z); }
+	static __device__ __forceinline__ V weights(const uintx4 &c, int j, unsigned z) { return K::weights(c[j], z); }
 	static __device__ __forceinline__ A mma(V a, V b, A c) { return W4X<X>::mma(a, b, c); }
 	/* at: the row's address; r: the row in the tile; q: lane / 16 */
 	static __device__ __forceinline__ V read(const unsigned char *at, int r, int j, int q)
@@ -39,11 +43,13 @@ template <int X, bool WIDE> struct W4Tile {		/* operands of 32 k, as W4X has the
 	}
 };
 
-template <> struct W4Tile<W4_X_I8, true> {		/* 8-bit operands of 64 k: two of 32 side by side */
+template <> struct W4Tile<W4_X_I8, false, true> {		/* 8-bit operands of 64 k: two of 32 side by side */
 	typedef intx4 V;
 	typedef intx4 A;
-	typedef W4Tile<W4_X_I8, false> H;
+	typedef W4Tile<W4_X_I8, false, false> H;
+	static constexpr bool ZIN = true;
 	static constexpr int MK = 64;
+	static __device__ __forceinline__ unsigned zero(int z) { return H::zero(z); }
 	static __device__ __forceinline__ V join(long lo, long hi)
 	{
 		return (V){(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
@@ -71,6 +77,13 @@ __device__ __forceinline__ float w4_get(const void *p, long i, int dtype)
 	}
 }
 
+/* Operands n - z of bf16 (4096 x 8192 -> 8192, us: 545 -> 532, with zero points 590 -> 535, groups of 32 880 -> 754), and
+ * of fp32 x where its groups are short (2048 rows: 32 1810 -> 1535, but 128 1090 -> 1176: three products for each code) */
+constexpr bool w4_tile_signed(int x, int gm)
+{
+	return x == THHIP_BF16 || (x == THHIP_F32 && gm == 1);
+}
+
 /* Wavefronts of a SIMD: with 8-bit x LDS has room for three workgroups (4096 x 8192 -> 8192, us: 387 with two, 352), with
  * fp32 x for one or two */
 constexpr int w4_tile_waves(int x, bool dma, int ks, bool most)
@@ -82,18 +95,18 @@ template <int X, int GM, bool ZP, bool XG, bool DMA, int KS>
 __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_tile_waves(X, DMA, KS, false), w4_tile_waves(X, DMA, KS, true)))) void w4_tile_kernel(const w4_args a, int mtiles, int ntiles)
 {
 	typedef W4X<X> K;
-	typedef W4Tile<X, X == W4_X_I8 && GM >= 2> M;
+	typedef W4Tile<X, w4_tile_signed(X, GM), X == W4_X_I8 && GM >= 2> M;
 	typedef typename M::V V;
 	typedef typename M::A A;
 	constexpr int PARTS = K::PARTS, BN = PARTS > 1 ? 64 : 128;
 	/* row blocks of a wavefront, and blocks of 16 columns */
-	constexpr int R = K::ZIN ? 2 : 4, NB = BN / (8 * R);
+	constexpr int R = M::ZIN ? 2 : 4, NB = BN / (8 * R);
 	constexpr int ES = sizeof(typename K::V) / 8;
 	constexpr int ROW = W4_KSTEP * ES;			/* bytes of a row in LDS */
 	constexpr int PLANE = BN * ROW, STAGE = PARTS * PLANE;
 	constexpr int NJ = W4_KSTEP / M::MK, GJ = GM * 32 / M::MK;	/* matrix instructions of a step, of a group */
 	constexpr int PIECES = BN * 16 / 256;			/* vectors of eight k a thread moves a step */
-	constexpr bool CORR = !K::ZIN;
+	constexpr bool CORR = !M::ZIN;
 	constexpr int NG = 4 / GM;				/* groups of a step */
 	/* One array: between the loads into LDS and reads of another array the compiler waits for all of the loads.  x; the
 	 * 128 rows' scales of a step's groups; zeros as zero() makes them; and the scales of x where a row has several */
@@ -183,7 +196,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_til
 		for (int g = 0; g < NG; g++) {
 			lscale[buf][g][tid & 127] = gs[g];
 			if constexpr (ZP)
-				lzero[buf][g][tid & 127] = K::zero(gz[g]);
+				lzero[buf][g][tid & 127] = M::zero(gz[g]);
 			if constexpr (XG)
 				lxs[buf][g][tid & 127] = gx[g];
 		}
@@ -222,8 +235,8 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_til
 
 	constexpr int NU = NB * NG;		/* units of a step: 16 columns x one group */
 	/* a unit's sums are added to the result while the next unit is multiplied, where the registers last */
-	constexpr bool PIPE = DMA && (KS == 1 || K::ZIN);
-	constexpr bool AHEAD = KS == 1 || K::ZIN;		/* ... and the next unit's operands are read */
+	constexpr bool PIPE = DMA && (KS == 1 || M::ZIN);
+	constexpr bool AHEAD = KS == 1 || M::ZIN;		/* ... and the next unit's operands are read */
 	const int own = wrow * R * 16 + col;	/* the lane's row of the first row block */
 	A p[PIPE ? 2 : 1][R];
 	/* unit u's finished sums into the result (buf: where its step's scales are) */
@@ -284,7 +297,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_til
 		for (int g = 0; g < NG; g++)
 #pragma unroll
 			for (int r = 0; r < R; r++) {
-				const unsigned z = K::ZIN && ZP ? lzero[buf][g][own + r * 16] : K::zero(8);
+				const unsigned z = M::ZIN && ZP ? lzero[buf][g][own + r * 16] : M::zero(8);
 #pragma unroll
 				for (int j = 0; j < GJ; j++)
 					w[r][g * GJ + j] = M::weights(codes[r], g * GJ + j, z);
@@ -414,9 +427,8 @@ static void w4_tile_launch(const w4_args &all)
 	const size_t esy = thhip_esize(all.dtype);
 	constexpr int BN = W4X<X>::PARTS > 1 ? 64 : 128;
 	/* K in two halves where there are fewer tiles than CUs (1024 x 4096 -> 4096, us, without and with: 8-bit x 73 -> 57, fp16
-	 * groups of 64 65 -> 54, bf16 groups of 32 130 -> 113); bf16 with larger groups keeps the matrix cores as busy
-	 * with four wavefronts (64 and 64; with zero points 68 and 73) */
-	constexpr bool HALVES = X != THHIP_F32 && (W4X<X>::ZIN || GM == 1);
+	 * groups of 64 65 -> 54, bf16 groups of 64 68 -> 56) */
+	constexpr bool HALVES = X != THHIP_F32;
 	for (int b0 = 0; b0 < all.B; b0 += W4_TILE_ROWS) {
 		const w4_args a = w4_rows(all, b0, all.B - b0 < W4_TILE_ROWS ? all.B - b0 : W4_TILE_ROWS, esx, esy);
 		const int mtiles = (a.blocks + 7) / 8, ntiles = (a.B + BN - 1) / BN;
