@@ -114,6 +114,19 @@ def test_norm_i8(hiplib, i, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(3, 4500), (2, 5120), (3, 5121), (2, 6144), (3, 6145), (3, 9000), (2, 10240), (3, 10243), (2, 12288), (3, 12290)])
+def test_norms_of_rows_between_four_and_eight_vectors_a_thread(hiplib, dtype, rows, cols):
+    x, r, w = inputs(90 + cols, rows, cols, dtype, True, True)
+    h, y = norm64(x, r, w)
+    err = chain(cols) + 8 * 2.0 ** -24
+    c = Call(hiplib, x, r, w, dtype)
+    near(c.sum, h, U.HALF_STEP[dtype] * (1 + 2.0 ** -8) + 2.0 ** -24, dtype, "sum")
+    near(c.y, y, U.HALF_STEP[dtype] * (1 + 2.0 ** -8) + err, dtype, "y")
+    for group in (0, 64):
+        check_codes(Call(hiplib, x, r, w, dtype, group=group), y, cols, group, err)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("group", [0, 32, 64, 128, 256])
 @pytest.mark.parametrize("cols", [40, 600, 1000, 5000, 20000, 66000])
 def test_codes_of_rows_and_back(hiplib, dtype, group, cols):

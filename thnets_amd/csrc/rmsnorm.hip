@@ -276,7 +276,9 @@ __device__ __forceinline__ void row_out(const rows_args &a, long row, int col, c
 
 /* Rows of at most T * V vectors, T threads a row, each of which keeps its V vectors in registers: a wavefront for rows of
  * up to two vectors a lane (four rows a workgroup, no barrier), 256 threads up to eight, so that several rows share a CU
- * and one's loads run under another's sums, 1024 beyond. */
+ * and one's loads run under another's sums, 1024 beyond.  V = 5 and 6 as well as 4 and 8: the registers of unused vectors
+ * are rows that do not fit beside (4096 rows of 9216 bf16, V = 8 and 5, us: norm 55 and 49, with codes 70 and 49); 3
+ * and 7 changed nothing. */
 template <int DT, int MODE, int T, int V>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const rows_args a)
 {
@@ -435,7 +437,8 @@ template <int DT, int MODE>
 static void rows_launch(rows_args &a)
 {
 	if (rows_try<DT, MODE, 64, 1>(a) || rows_try<DT, MODE, 64, 2>(a) || rows_try<DT, MODE, 256, 1>(a) ||
-	    rows_try<DT, MODE, 256, 2>(a) || rows_try<DT, MODE, 256, 4>(a) || rows_try<DT, MODE, 256, 8>(a) ||
+	    rows_try<DT, MODE, 256, 2>(a) || rows_try<DT, MODE, 256, 4>(a) || rows_try<DT, MODE, 256, 5>(a) ||
+	    rows_try<DT, MODE, 256, 6>(a) || rows_try<DT, MODE, 256, 8>(a) ||
 	    rows_try<DT, MODE, 1024, 4>(a))
 		return;
 	rows_long_kernel<DT, MODE><<<dim3((unsigned)a.rows), dim3(1024), 0, thhip_stream()>>>(a);
