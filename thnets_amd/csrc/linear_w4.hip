@@ -72,24 +72,34 @@ extern "C" size_t thhip_w4_packed_bytes(int nOut, int nIn, int group, int dtype,
 	return w4_bad(nOut, nIn, group, dtype) ? 0 : w4_layout_of(nOut, nIn, group, dtype, zeros).bytes;
 }
 
-/* ---- laying out and making weights ---- */
+/* ---- laying out and making weights ----
+ *
+ * Once a layer, bound by memory: a thread makes one word of eight codes from four bytes (8192 -> 32768: 268 MB in 103 us, 2.6
+ * TB/s; code by code it was 477). */
 
 __global__ __launch_bounds__(256) void w4_pack_codes_kernel(const unsigned char *codes, unsigned *out, int nOut, int nIn,
 	int steps, size_t words)
 {
+	typedef unsigned U __attribute__((aligned(1)));
 	const size_t row_bytes = ((size_t)nIn + 1) / 2;
 	for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (size_t)gridDim.x * 256) {
 		const int j = i & 3, lane = (i >> 2) & 63;
 		const size_t step = i >> 8;
 		const long row = (long)(step / steps) * 16 + (lane & 15);
 		const long k0 = (long)(step % steps) * W4_KSTEP + 32 * j + 8 * (lane >> 4);
-		unsigned w = 0;
-		if (row < nOut)
-			for (int e = 0; e < 8; e++)
-				if (k0 + e < nIn) {
-					const unsigned n = (codes[row * row_bytes + (k0 + e) / 2] >> (4 * ((k0 + e) & 1))) & 15;
-					w |= n << (8 * (e & 3) + 4 * (e >> 2));
-				}
+		/* eight codes of the row: four of its bytes, or what is left of them and zeros */
+		unsigned u = 0, w = 0;
+		if (row < nOut && k0 < nIn) {
+			const unsigned char *from = codes + row * row_bytes + k0 / 2;
+			if (k0 + 8 <= nIn)
+				u = *(const U *)from;
+			else
+				for (int e = 0; e < nIn - k0; e++)
+					u |= (unsigned)(from[e / 2] >> (4 * (e & 1)) & 15) << (4 * e);
+		}
+#pragma unroll
+		for (int e = 0; e < 8; e++)
+			w |= (u >> (4 * e) & 15) << (8 * (e & 3) + 4 * (e >> 2));
 		out[i] = w;
 	}
 }
