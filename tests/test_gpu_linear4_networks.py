@@ -94,6 +94,14 @@ def test_vgg_linears(hiplib):
     ref.free()
 
 
+def test_other_groups_are_refused(hiplib):
+    layers, _ = network(U.rng(3300), 1)
+    for group in (48, -1, 512):
+        with pytest.raises(ValueError):
+            api.HipNetwork(layers, linear4=group)
+    assert hiplib.THHipLinear4Bit(0) == 0
+
+
 def test_command_line_driver(hiplib, tmp_path):
     """-q group: the driver's printed outputs are those of the engine with that setting."""
     g = U.rng(3200)

@@ -295,10 +295,13 @@ class HipNetwork:
             self.handle = lib.THCreateHipLowpNetwork(source, C.c_float(lowp_range))
             self.dtype = abi.THHIP_U8
         else:
+            old_linear4 = lib.THHipLinear4Bit(linear4)
+            if lib.THHipLinear4Bit(linear4) != linear4:     # (what it does not know changes nothing)
+                raise ValueError("THHipLinear4Bit(%r) refused" % linear4)
             if lib.THHipHalfFloat(half) != 0:
+                lib.THHipLinear4Bit(old_linear4)
                 raise ValueError("THHipHalfFloat(%r) refused" % half)
             old_fold = lib.THHipFoldBatchNorm(1 if fold_bn else 0)
-            old_linear4 = lib.THHipLinear4Bit(linear4)
             self.handle = lib.THCreateHipNetwork(source)
             lib.THHipLinear4Bit(old_linear4)
             lib.THHipFoldBatchNorm(old_fold)
