@@ -146,6 +146,22 @@ def test_codes_of_rows_and_back(hiplib, dtype, group, cols):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols,group", [(1, 2049, 32), (1, 300001, 256), (7, 40003, 64), (511, 2100, 128), (513, 2100, 0), (1024, 2056, 32)])
+def test_back_from_codes_of_few_long_rows(hiplib, dtype, rows, cols, group):
+    """Rows that several workgroups share: every value is its code times its scale, rounded once; nothing else is written."""
+    g = U.rng(95)
+    q = g.integers(-127, 128, (rows, cols)).astype(np.int8)
+    scale = g.uniform(0.5, 1.5, (rows, U.groups_of(cols, group))).astype(np.float32)
+    dq, ds = U.Rows(hiplib, q, cols + 3, 1), api.DeviceArray(hiplib, scale)
+    dy = U.Rows(hiplib, None, cols + 5, 3, (rows, cols), word(dtype))
+    G.note("back %dx%d group=%d dtype=%d" % (rows, cols, group, dtype))
+    assert hiplib.thhip_dequantize_rows(dq.ptr, dq.ld, ds.ptr, group, dy.ptr, dy.ld, rows, cols, dtype) == 0
+    hiplib.thhip_sync()
+    dq.get()
+    assert np.array_equal(dy.get(), U.raw(q.astype(np.float32) * np.repeat(scale, group or cols, 1)[:, :cols], dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("cols", [100, 512, 3000, 17000, 70000])
 @pytest.mark.parametrize("pad,off", [(5, 3), (8, 8), (1, 0), (0, 1)])
 def test_strides_and_offsets(hiplib, dtype, cols, pad, off):

@@ -533,18 +533,20 @@ extern "C" int thhip_quantize_rows(const void *x, long ldx, signed char *q, long
 	return rows_run("thhip_quantize_rows", a, rows, cols, dtype, ROWS_QUANT);
 }
 
-/* y = q * scale.  TX threads (a power of two) walk a row eight columns at a time; a group is a whole
- * number of such vectors.  Bound by memory: 8192 rows of 4096 to bf16 16.7 us (101 MB, 6.0 TB/s), 700 of 9216 to fp16
+/* y = q * scale.  segs times tx threads (a power of two) walk a row eight columns at a time; a group is a whole
+ * number of such vectors.  Few long rows are shared by several workgroups (100 rows of 40000 to fp32 10.6 -> 6.1 us); two
+ * vectors a thread for every row took longer where there are many rows (700 of 9216 5.1 -> 6.1).  Bound by memory: 8192 rows of 4096 to bf16 16.7 us (101 MB, 6.0 TB/s), 700 of 9216 to fp16
  * 6.0 us (19 MB, 3.2 TB/s). */
 template <int DT>
 __global__ __launch_bounds__(256) void dequantize_rows_kernel(const signed char *q, long ldq, const float *scale, int group,
-	int ngroups, void *y, long ldy, long rows, int cols, int tx)
+	int ngroups, void *y, long ldy, long rows, int cols, int tx, unsigned segs)
 {
 	typedef unsigned W __attribute__((ext_vector_type(2), aligned(1)));
-	const long row = (long)blockIdx.x * (256 / tx) + threadIdx.x / tx;
+	const long row = (long)(blockIdx.x / segs) * (256 / tx) + threadIdx.x / tx;
 	if (row >= rows)
 		return;
-	for (int col = (threadIdx.x & (tx - 1)) * 8; col < cols; col += tx * 8) {
+	for (long c = ((long)(blockIdx.x % segs) * tx + (threadIdx.x & (tx - 1))) * 8; c < cols; c += (long)segs * tx * 8) {
+		const int col = (int)c;
 		const float s = scale[row * ngroups + (group ? col / group : 0)];
 		float v[8];
 		if (col + 8 <= cols) {
@@ -581,12 +583,15 @@ extern "C" int thhip_dequantize_rows(const signed char *q, long ldq, const float
 	int tx = 1;
 	while (tx < 256 && tx * 8 < cols)
 		tx *= 2;
+	/* about four workgroups a CU, and at least one vector a thread */
+	const long each = (cols - 1) / (tx * 8) + 1, want = 1024 / rows;
+	const unsigned segs = tx < 256 || want <= 1 ? 1 : (unsigned)(want < each ? want : each);
 	ThhipLaunchScope scope(THHIP_FAM_OTHER, (double)rows * cols * (1 + thhip_esize(dtype)) + 4.0 * rows * a.ngroups);
 	for (long r = 0; r < rows; r += ROWS_A_LAUNCH) {
 		const long n = rows - r < ROWS_A_LAUNCH ? rows - r : ROWS_A_LAUNCH;
-		const unsigned grid = (unsigned)((n + 256 / tx - 1) / (256 / tx));
+		const unsigned grid = (unsigned)((n + 256 / tx - 1) / (256 / tx)) * segs;
 		THHIP_DISPATCH_FLOAT(dtype, (dequantize_rows_kernel<DT><<<dim3(grid), dim3(256), 0, thhip_stream()>>>(q + r * ldq, ldq,
-			qscale + r * a.ngroups, group, a.ngroups, (char *)y + r * ldy * thhip_esize(dtype), ldy, n, (int)cols, tx)));
+			qscale + r * a.ngroups, group, a.ngroups, (char *)y + r * ldy * thhip_esize(dtype), ldy, n, (int)cols, tx, segs)));
 	}
 	return 0;
 }
