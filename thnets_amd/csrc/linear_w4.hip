@@ -518,8 +518,8 @@ static void w4_skinny_launch(const w4_args &all)
  * workgroups as the GPU holds; the time of a round was measured at K = 512, 2048 and 8192 and is a start and a
  * slope.  Few rows at a time win in small layers and short K, 64 rows in larger ones (4096 -> 4096 fp16, us, in the
  * order of the table: 128 columns 37 / 24 / 27 / 17.4 / 12.8, tiles 50), tiles from about 512 columns on (768 columns: 81
- * with 64 rows, 56 with tiles).  Of 78 layers drawn at random (16 to 1300 rows, 512 to 9216 inputs, 256 to 10240 outputs) the
- * choice took 1.7 % more than the best shape, 27 % at most. */
+ * with 64 rows, 56 with tiles).  Of three times 78 layers drawn at random (16 to 1300 rows, 512 to 9216 inputs, 256 to 10240 outputs) the
+ * choice took 0.8 to 1.7 % more than the best shape, 27 % at most. */
 enum { W4_16x16, W4_32x16, W4_16x32, W4_32x32, W4_64x32, W4_TILES };
 
 static int w4_shape(const w4_args &a, int parts)
@@ -530,17 +530,20 @@ static int w4_shape(const w4_args &a, int parts)
 		{{3.9f, 0.42f}, {4.9f, 0.54f}, {3.3f, 0.73f}, {4.3f, 1.0f}, {6.3f, 1.6f}},	/* 8-bit x */
 		{{4.5f, 0.65f}, {6.0f, 1.2f}, {4.4f, 1.35f}, {5.6f, 2.2f}, {8.0f, 3.8f}},	/* ... in groups of 32 and 64 */
 	};
-	static const float tile_us[2][3][2] = {
+	static const float tile_us[3][3][2] = {
 		{{13.0f, 10.0f}, {13.0f, 10.7f}, {14.0f, 13.7f}},	/* groups of 128 and more, 64, 32 */
-		{{8.0f, 17.0f}, {8.0f, 19.5f}, {8.0f, 23.0f}},		/* fp32 x */
+		{{8.0f, 17.0f}, {8.0f, 19.5f}, {8.0f, 22.0f}},		/* fp32 x, 128 rows */
+		{{14.0f, 20.0f}, {15.0f, 21.0f}, {15.0f, 25.0f}},	/* fp32 x, 256 rows */
 	};
 	static const int rows[5] = {1, 2, 1, 2, 4}, cols[5] = {1, 1, 2, 2, 2};	/* blocks of 16 */
 	const float (*us)[2] = round_us[(a.xscale ? 2 : 0) + (a.group == 32 || a.group == 64)];
-	const float *tile = tile_us[parts > 1][a.group == 32 ? 2 : a.group == 64];
 	const float k = (float)a.nIn / 1024;
-	/* tiles: 128 rows x 128 columns, two on a CU (one alone takes two thirds of the time of two); fp32 x 64 rows of x, one on a CU */
-	const long tiles = (long)((a.blocks + 7) / 8) * ((a.B + (parts > 1 ? 63l : 127l)) / (parts > 1 ? 64 : 128));
-	float best = (tile[0] + tile[1] * k) * (parts > 1 ? (float)((tiles + 255) / 256) : tiles <= 256 ? 1.0f : 1.45f * (float)((tiles + 511) / 512));
+	/* tiles: 128 rows x 128 columns, two on a CU (one alone takes two thirds of the time of two); fp32 x 64 rows of x, one on a
+	 * CU, of 256 rows where there are more than 256 */
+	const long wide = ((long)a.B + (parts > 1 ? 63 : 127)) / (parts > 1 ? 64 : 128), tiles = wide * ((a.blocks + 7) / 8);
+	const float *tile = tile_us[parts == 1 ? 0 : tiles <= 256 ? 1 : 2][a.group == 32 ? 2 : a.group == 64];
+	const float rounds = tiles <= 256 ? 1.0f : parts > 1 ? (float)((wide * ((a.blocks + 15) / 16) + 255) / 256) : 1.45f * (float)((tiles + 511) / 512);
+	float best = (tile[0] + tile[1] * k) * rounds;
 	int shape = W4_TILES;
 	for (int i = 0; i < 5; i++) {
 		const int slice = cols[i] * 16 / parts;

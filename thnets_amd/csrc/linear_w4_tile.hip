@@ -1,17 +1,15 @@
 /*
  * 4-bit Linear layers (linear_w4.hip) for larger batches: bound by the matrix cores and by the instructions between
  * theirs, of which a wavefront issues one where it could issue a matrix instruction (codes to operands, a group's sums to
- * the result).  4096 x 8192 -> 8192, us and 10^12 a second: fp16 490 to 505 and 1100, bf16 520 to 535 and 1040 (a library's
- * product of 8192^3: 1150 and 1201), 8-bit x 350 and 1570 (1779); fp32 x 2200 and 250 (149).
+ * the result).  4096 x 8192 -> 8192, us and 10^12 a second: fp16 490 to 505 and 1100, bf16 517 to 530 and 1050 (a library's
+ * product of 8192^3: 1150 and 1201), 8-bit x 344 to 350 and 1590 (1779); 2048 rows of fp32 x 696 to 733 and 390 (149).
  *
- * A workgroup of four wavefronts computes 128 rows for BN columns, a wavefront 64 rows x BN / 2 or, where the operands
- * are n - z and no sums of x are needed, 32 rows x BN, for which half as many codes become operands (4096 x 8192 ->
- * 8192 fp16 550 -> 505 us): all but fp32 x with groups longer than 32, whose sums of x would be twice as many.  x goes
- * through LDS a step of 128 k at a time (two buffers); codes go from memory to registers, one step ahead, and
- * become operands there: those of a whole step stay (32 or 64 registers) while its columns are walked 16 at a
- * time, so that the sums of one group of 16 columns (of two, the last one's being added to the result while the next
- * are multiplied) are all there is beside the result.  The sums of a group start at 0 or, where
- * z is not in the operands, at -z * sum x, so that what is left when it ends is one multiply-add a value.
+ * A workgroup of four wavefronts computes 128 rows for BN columns (eight 256 rows: fp32 x), a wavefront 32 rows: each code
+ * becomes an operand once (with 64 rows x BN / 2 a wavefront, twice: fp16 550 us).  All operands are n - z, so that no sum
+ * of x is needed beside the products.  x goes through LDS a step of 128 k at a time (two buffers); codes go from memory to
+ * registers, one step ahead, and become operands there: those of a whole step stay (32 registers) while its columns
+ * are walked 16 at a time, so that the sums of one group of 16 columns (of two, the last one's being added to the result
+ * while the next are multiplied) are all there is beside the result, which a group's end costs one multiply-add a value.
  * fp32 x is three planes of bf16 in LDS (BN = 64); 8-bit x is multiplied 64 k at a time (32 for groups of 32).
  * LDS rows are 128 k of a column; a 16-byte vector v of row r lies in slot v ^ r % 16 (8-bit x: v ^ r / 2 % 8),
  * which puts the 16 columns of an operand on different banks.  DMA: rows that memory holds in whole, aligned
@@ -24,9 +22,8 @@
 #include <type_traits>
 #include "linear_w4.h"
 
-template <int X, bool SIGNED, bool WIDE> struct W4Tile {		/* operands of 32 k, as W4X has them, or of n - z */
-	typedef typename std::conditional<SIGNED, W4Signed, W4X<X>>::type K;
-	static constexpr bool ZIN = K::ZIN;
+template <int X, bool WIDE> struct W4Tile {		/* operands of 32 k, of weights n - z for every kind of x */
+	typedef typename std::conditional<W4X<X>::ZIN, W4X<X>, W4Signed>::type K;
 	typedef typename W4X<X>::V V;
 	typedef typename W4X<X>::A A;
 	static constexpr int MK = 32;
@@ -43,11 +40,10 @@ template <int X, bool SIGNED, bool WIDE> struct W4Tile {		/* operands of 32 k, a
 	}
 };
 
-template <> struct W4Tile<W4_X_I8, false, true> {		/* 8-bit operands of 64 k: two of 32 side by side */
+template <> struct W4Tile<W4_X_I8, true> {		/* 8-bit operands of 64 k: two of 32 side by side */
 	typedef intx4 V;
 	typedef intx4 A;
-	typedef W4Tile<W4_X_I8, false, false> H;
-	static constexpr bool ZIN = true;
+	typedef W4Tile<W4_X_I8, false> H;
 	static constexpr int MK = 64;
 	static __device__ __forceinline__ unsigned zero(int z) { return H::zero(z); }
 	static __device__ __forceinline__ V join(long lo, long hi)
@@ -77,46 +73,38 @@ __device__ __forceinline__ float w4_get(const void *p, long i, int dtype)
 	}
 }
 
-/* Operands n - z of bf16 (4096 x 8192 -> 8192, us: 545 -> 532, with zero points 590 -> 535, groups of 32 880 -> 754), and
- * of fp32 x where its groups are short (2048 rows: 32 1810 -> 1535, but 128 1090 -> 1176: three products for each code) */
-constexpr bool w4_tile_signed(int x, int gm)
-{
-	return x == THHIP_BF16 || (x == THHIP_F32 && gm == 1);
-}
-
 /* Wavefronts of a SIMD: with 8-bit x LDS has room for three workgroups (4096 x 8192 -> 8192, us: 387 with two, 352), with
- * fp32 x for one or two */
-constexpr int w4_tile_waves(int x, bool dma, int ks, bool most)
+ * fp32 x for one of four or eight */
+constexpr int w4_tile_waves(int x, bool dma, int ks, int threads)
 {
-	return x == W4_X_I8 && dma && ks == 1 ? 3 : x == THHIP_F32 && !most ? 1 : 2;
+	return x == W4_X_I8 && dma && ks == 1 ? 3 : x == THHIP_F32 && threads == 256 ? 1 : 2;
 }
 
-template <int X, int GM, bool ZP, bool XG, bool DMA, int KS>
-__global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_tile_waves(X, DMA, KS, false), w4_tile_waves(X, DMA, KS, true)))) void w4_tile_kernel(const w4_args a, int mtiles, int ntiles)
+template <int X, int GM, bool ZP, bool XG, bool DMA, int KS, int TH>
+__global__ __launch_bounds__(KS * TH) __attribute__((amdgpu_waves_per_eu(w4_tile_waves(X, DMA, KS, TH), w4_tile_waves(X, DMA, KS, TH)))) void w4_tile_kernel(const w4_args a, int mtiles, int ntiles)
 {
 	typedef W4X<X> K;
-	typedef W4Tile<X, w4_tile_signed(X, GM), X == W4_X_I8 && GM >= 2> M;
+	typedef W4Tile<X, X == W4_X_I8 && GM >= 2> M;
 	typedef typename M::V V;
 	typedef typename M::A A;
 	constexpr int PARTS = K::PARTS, BN = PARTS > 1 ? 64 : 128;
 	/* row blocks of a wavefront, and blocks of 16 columns */
-	constexpr int R = M::ZIN ? 2 : 4, NB = BN / (8 * R);
+	constexpr int BM = TH / 2, R = 2, NB = BN / 16;
 	constexpr int ES = sizeof(typename K::V) / 8;
 	constexpr int ROW = W4_KSTEP * ES;			/* bytes of a row in LDS */
 	constexpr int PLANE = BN * ROW, STAGE = PARTS * PLANE;
 	constexpr int NJ = W4_KSTEP / M::MK, GJ = GM * 32 / M::MK;	/* matrix instructions of a step, of a group */
-	constexpr int PIECES = BN * 16 / 256;			/* vectors of eight k a thread moves a step */
-	constexpr bool CORR = !M::ZIN;
+	constexpr int PIECES = BN * 16 / TH;			/* vectors of eight k a thread moves a step */
 	constexpr int NG = 4 / GM;				/* groups of a step */
 	/* One array: between the loads into LDS and reads of another array the compiler waits for all of the loads.  x; the
-	 * 128 rows' scales of a step's groups; zeros as zero() makes them; and the scales of x where a row has several */
-	constexpr int SCALES = 2 * NG * 512, ZEROS = ZP ? SCALES : 0, XSCALES = XG ? SCALES : 0;
+	 * BM rows' scales of a step's groups; zeros as zero() makes them; and the scales of x where a row has several */
+	constexpr int SCALES = 2 * NG * BM * 4, ZEROS = ZP ? SCALES : 0, XSCALES = XG ? SCALES : 0;
 	__shared__ __align__(16) unsigned char all_lds[KS * (2 * STAGE + SCALES + ZEROS + XSCALES)];
 	const int part = KS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;	/* the wavefronts of one take every KS-th step */
-	const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	const int tid = threadIdx.x & (TH - 1), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	unsigned char *lds = all_lds + part * (2 * STAGE + SCALES + ZEROS + XSCALES);
-	float (*lscale)[NG][128] = (float (*)[NG][128])(lds + 2 * STAGE);
-	unsigned (*lzero)[NG][128] = (unsigned (*)[NG][128])(lds + 2 * STAGE + SCALES);
+	float (*lscale)[NG][BM] = (float (*)[NG][BM])(lds + 2 * STAGE);
+	unsigned (*lzero)[NG][BM] = (unsigned (*)[NG][BM])(lds + 2 * STAGE + SCALES);
 	float (*lxs)[NG][BN] = (float (*)[NG][BN])(lds + 2 * STAGE + SCALES + ZEROS);
 	const int col = lane & 15, quarter = lane >> 4;
 
@@ -132,7 +120,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_til
 	}
 	const int mt = id / ntiles, nt = id - mt * ntiles;
 	const int b0 = nt * BN, nrows = a.B - b0 < BN ? a.B - b0 : BN;
-	const int wrow = wave % (8 / R), rb0 = mt * 8 + wrow * R, c0 = wave / (8 / R) * NB * 16;
+	const int wrow = wave % (BM / 16 / R), rb0 = mt * (BM / 16) + wrow * R, c0 = wave / (BM / 16 / R) * NB * 16;
 
 	const typename K::E *xbase = (const typename K::E *)a.x + (long)b0 * a.ldx;
 	const unsigned xend = DMA ? (unsigned)(((nrows - 1) * a.ldx + a.nIn) * (long)sizeof(typename K::E)) : 0;
@@ -155,7 +143,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_til
 			}
 		} else {
 			w4_fetch_x<X, false>(xr, xbase, a.ldx, a.nIn, t * W4_KSTEP + (tid & 15) * 8, [&](int i) {
-				const int r = (tid + (half * (PIECES / 2) + i) * 256) >> 4;
+				const int r = (tid + (half * (PIECES / 2) + i) * TH) >> 4;
 				return (long)(r < nrows ? r : nrows - 1);
 			});
 		}
@@ -166,7 +154,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_til
 				w4_fix_x<X>(xr, a.nIn, t * W4_KSTEP + (tid & 15) * 8);
 #pragma unroll
 			for (int i = 0; i < PIECES / 2; i++) {
-				const int p = tid + (half * (PIECES / 2) + i) * 256, r = p >> 4, v = p & 15;
+				const int p = tid + (half * (PIECES / 2) + i) * TH, r = p >> 4, v = p & 15;
 				typename K::V o[PARTS];
 				K::operand(xr[i], o);
 				const int to = ES == 1 ? ((v >> 1) ^ (r >> 1 & 7)) * 16 + (v & 1) * 8 : (v ^ (r & 15)) * 16;
@@ -176,10 +164,10 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_til
 			}
 		}
 	};
-	/* scales and zeros: thread i fetches row i % 128's, and puts them into LDS at the end of the step */
+	/* scales and zeros: thread i fetches row i % BM's, and puts them into LDS at the end of the step */
 	float gs[NG], gx[NG];
 	unsigned char gz[NG];
-	const int grb = mt * 8 + (tid >> 4 & 7) < a.blocks ? mt * 8 + (tid >> 4 & 7) : a.blocks - 1;
+	const int gb = mt * (BM / 16) + (tid >> 4 & (BM / 16 - 1)), grb = gb < a.blocks ? gb : a.blocks - 1;
 	auto g_issue = [&](int t) {
 #pragma unroll
 		for (int g = 0; g < NG; g++) {
@@ -194,9 +182,9 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_til
 	auto g_land = [&](int buf) {
 #pragma unroll
 		for (int g = 0; g < NG; g++) {
-			lscale[buf][g][tid & 127] = gs[g];
+			lscale[buf][g][tid & (BM - 1)] = gs[g];
 			if constexpr (ZP)
-				lzero[buf][g][tid & 127] = M::zero(gz[g]);
+				lzero[buf][g][tid & (BM - 1)] = M::zero(gz[g]);
 			if constexpr (XG)
 				lxs[buf][g][tid & 127] = gx[g];
 		}
@@ -234,9 +222,9 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_til
 	barrier();
 
 	constexpr int NU = NB * NG;		/* units of a step: 16 columns x one group */
-	/* a unit's sums are added to the result while the next unit is multiplied, where the registers last */
-	constexpr bool PIPE = DMA && (KS == 1 || M::ZIN);
-	constexpr bool AHEAD = KS == 1 || M::ZIN;		/* ... and the next unit's operands are read */
+	/* a unit's sums are added to the result while the next unit is multiplied (with eight wavefronts of fp32 x the other one of
+	 * a SIMD multiplies meanwhile: 2048 x 8192 -> 8192 696 us so, 700 with it) */
+	constexpr bool PIPE = DMA || (X == THHIP_F32 && TH == 256);
 	const int own = wrow * R * 16 + col;	/* the lane's row of the first row block */
 	A p[PIPE ? 2 : 1][R];
 	/* unit u's finished sums into the result (buf: where its step's scales are) */
@@ -264,30 +252,13 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_til
 			break;
 		}
 		const unsigned char *base = lds + buf * STAGE + (c0 + col) * ROW;
-		V w[R][NJ], x[AHEAD ? 2 : 1][PARTS][NJ];
-		A sx[2];
+		V w[R][NJ], x[2][PARTS][NJ];
 		auto x_read = [&](int n) {
 #pragma unroll
 			for (int q = 0; q < PARTS; q++)
 #pragma unroll
 				for (int j = 0; j < NJ; j++)
-					x[AHEAD ? n & 1 : 0][q][j] = M::read(base + q * PLANE + n * 16 * ROW, col, j, quarter);
-		};
-		/* sum of x over unit u's group, for every row (without zero points -8 times that: 8 is the zero) */
-		auto x_add = [&](int u, int i) {	/* the i-th of the group's GJ pieces */
-			if constexpr (CORR) {
-				const int n = u / NG, j = u % NG * GJ + i;
-				if (i == 0)
-					sx[u & 1] = (A)0;
-#pragma unroll
-				for (int q = 0; q < PARTS; q++)
-					sx[u & 1] = M::mma(x[AHEAD ? n & 1 : 0][q][j], ZP ? K::ones() : K::minus8(), sx[u & 1]);
-			}
-		};
-		auto x_sum = [&](int u) {
-#pragma unroll
-			for (int i = 0; i < GJ; i++)
-				x_add(u, i);
+					x[n & 1][q][j] = M::read(base + q * PLANE + n * 16 * ROW, col, j, quarter);
 		};
 		auto flush = [&](int u) { flush_at(u, buf); };
 		__builtin_amdgcn_s_setprio(0);
@@ -297,13 +268,11 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_til
 		for (int g = 0; g < NG; g++)
 #pragma unroll
 			for (int r = 0; r < R; r++) {
-				const unsigned z = M::ZIN && ZP ? lzero[buf][g][own + r * 16] : M::zero(8);
+				const unsigned z = ZP ? lzero[buf][g][own + r * 16] : M::zero(8);
 #pragma unroll
 				for (int j = 0; j < GJ; j++)
 					w[r][g * GJ + j] = M::weights(codes[r], g * GJ + j, z);
 			}
-		if (AHEAD)
-			x_sum(0);
 		if (LATE && i > 0)
 			flush_at(NU - 1, buf ^ 1);
 		codes_issue(t1);
@@ -318,25 +287,11 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_til
 				x_land(t1, buf ^ 1, 0);
 				x_issue(t1, buf ^ 1, 1);
 			}
-			if (!AHEAD && g == 0 && n)
-				x_read(n);
-			if (AHEAD && g == 0 && n + 1 < NB)
+			if (g == 0 && n + 1 < NB)
 				x_read(n + 1);
-			if (!AHEAD)
-				x_sum(u);
 #pragma unroll
-			for (int r = 0; r < R; r++) {
-				if constexpr (!CORR)
-					p[PIPE ? u & 1 : 0][r] = (A)0;
-				else if constexpr (ZP) {
-					const float z = __uint_as_float(lzero[buf][g][own + r * 16]);
-#pragma unroll
-					for (int i = 0; i < 4; i++)
-						p[PIPE ? u & 1 : 0][r][i] = z * sx[u & 1][i];
-				} else
-					p[PIPE ? u & 1 : 0][r] = sx[u & 1];
-			}
-			/* (the next unit's sum of x, whose pieces wait for each other, between the products) */
+			for (int r = 0; r < R; r++)
+				p[PIPE ? u & 1 : 0][r] = (A)0;
 #pragma unroll
 			for (int i = 0; i < GJ; i++) {
 				const int j = g * GJ + i;
@@ -344,21 +299,15 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_til
 				for (int q = 0; q < PARTS; q++)
 #pragma unroll
 					for (int r = 0; r < R; r++)
-						p[PIPE ? u & 1 : 0][r] = M::mma(x[AHEAD ? n & 1 : 0][q][j], w[r][j], p[PIPE ? u & 1 : 0][r]);
-				if (AHEAD && u + 1 < NU && i > 0)
-					x_add(u + 1, i - 1);
+						p[PIPE ? u & 1 : 0][r] = M::mma(x[n & 1][q][j], w[r][j], p[PIPE ? u & 1 : 0][r]);
 			}
-			if (AHEAD && u + 1 < NU)
-				x_add(u + 1, GJ - 1);
 			if (PIPE ? u > 0 : true)
 				flush(PIPE ? u - 1 : u);
 			if constexpr (PIPE && (X == THHIP_F16 || X == THHIP_BF16)) {
 			/* the order to issue them in: what comes from LDS, then a matrix instruction and the sums' work in turn */
 			__builtin_amdgcn_sched_group_barrier(0x100, PARTS * NJ + R, 0);
-			if constexpr (ZP)
-				__builtin_amdgcn_sched_group_barrier(0x2, 16, 0);
 #pragma unroll
-			for (int i = 0; i < (R + CORR) * GJ * PARTS; i++) {
+			for (int i = 0; i < R * GJ * PARTS; i++) {
 				__builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
 				__builtin_amdgcn_sched_group_barrier(0x2, 1, 0);
 			}
@@ -385,7 +334,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_til
 				for (int r = 0; r < R; r++)
 #pragma unroll
 					for (int n = 0; n < NB; n++)
-						sums[(((p - 1) * R + r) * NB + n) * 256 + tid] = acc[r][n];
+						sums[(((p - 1) * R + r) * NB + n) * TH + tid] = acc[r][n];
 		barrier();
 		if (part)
 			return;
@@ -395,7 +344,7 @@ __global__ __launch_bounds__(KS * 256) __attribute__((amdgpu_waves_per_eu(w4_til
 			for (int r = 0; r < R; r++)
 #pragma unroll
 				for (int n = 0; n < NB; n++)
-					acc[r][n] += sums[(((p - 1) * R + r) * NB + n) * 256 + tid];
+					acc[r][n] += sums[(((p - 1) * R + r) * NB + n) * TH + tid];
 	}
 
 #pragma unroll
@@ -426,30 +375,35 @@ static void w4_tile_launch(const w4_args &all)
 	constexpr size_t esx = sizeof(typename W4X<X>::E);
 	const size_t esy = thhip_esize(all.dtype);
 	constexpr int BN = W4X<X>::PARTS > 1 ? 64 : 128;
-	/* K in two halves where there are fewer tiles than CUs (1024 x 4096 -> 4096, us, without and with: 8-bit x 73 -> 57, fp16
-	 * groups of 64 65 -> 54, bf16 groups of 64 68 -> 56) */
-	constexpr bool HALVES = X != THHIP_F32;
 	for (int b0 = 0; b0 < all.B; b0 += W4_TILE_ROWS) {
 		const w4_args a = w4_rows(all, b0, all.B - b0 < W4_TILE_ROWS ? all.B - b0 : W4_TILE_ROWS, esx, esy);
-		const int mtiles = (a.blocks + 7) / 8, ntiles = (a.B + BN - 1) / BN;
-		const dim3 grid((unsigned)mtiles * ntiles);
+		const int ntiles = (a.B + BN - 1) / BN;
+		const bool few = (long)((a.blocks + 7) / 8) * ntiles <= 256;	/* tiles of 128 rows: at most one a CU */
 		/* rows in whole vectors, and a tile of them within the reach of a buffer descriptor */
 		const bool dma = X != THHIP_F32 && (uintptr_t)a.x % 16 == 0 && a.ldx * esx % 16 == 0 && a.nIn * esx % 16 == 0 &&
 			a.ldx * esx * BN < (1u << 31);
-#define W4_TILE(ZP, DMA, KS) w4_tile_kernel<X, GM, ZP, XG, DMA, KS><<<grid, dim3(KS * 256), 0, thhip_stream()>>>(a, mtiles, ntiles)
-#define W4_TILE_ZP(DMA, KS) do { if (a.zeros) W4_TILE(true, DMA, KS); else W4_TILE(false, DMA, KS); } while (0)
-		if constexpr (X != THHIP_F32) {
-			if constexpr (HALVES)
-				if (dma && (long)mtiles * ntiles <= 256) {
-					W4_TILE_ZP(true, 2);
-					continue;
-				}
-			if (dma) {
-				W4_TILE_ZP(true, 1);
-				continue;
-			}
+#define W4_TILE(ZP, DMA, KS, TH) do { \
+	const int mtiles = (a.blocks + TH / 32 - 1) / (TH / 32); \
+	w4_tile_kernel<X, GM, ZP, XG, DMA, KS, TH><<<dim3((unsigned)mtiles * ntiles), dim3(KS * TH), 0, thhip_stream()>>>(a, mtiles, ntiles); \
+} while (0)
+#define W4_TILE_ZP(DMA, KS, TH) do { if (a.zeros) W4_TILE(true, DMA, KS, TH); else W4_TILE(false, DMA, KS, TH); } while (0)
+		if constexpr (X == THHIP_F32) {
+			/* eight wavefronts and 256 rows, so that two share a SIMD (LDS holds one workgroup's x): 2048 x 8192 -> 8192
+			 * 1092 -> 733 us, but 512 x 4096 -> 4096, where half the CUs then have nothing to do, 76 -> 92 */
+			if (few)
+				W4_TILE_ZP(false, 1, 256);
+			else
+				W4_TILE_ZP(false, 1, 512);
+		} else {
+			/* K in two halves where there are fewer tiles than CUs (1024 x 4096 -> 4096, us, without and with: 8-bit x 73 ->
+			 * 57, fp16 groups of 64 65 -> 54, bf16 groups of 64 68 -> 56) */
+			if (dma && few)
+				W4_TILE_ZP(true, 2, 256);
+			else if (dma)
+				W4_TILE_ZP(true, 1, 256);
+			else
+				W4_TILE_ZP(false, 1, 256);
 		}
-		W4_TILE_ZP(false, 1);
 #undef W4_TILE_ZP
 #undef W4_TILE
 	}
