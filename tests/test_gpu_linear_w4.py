@@ -170,6 +170,30 @@ def test_more_tiles_than_the_gpu_holds_at_once(hiplib, dtype, B):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("zeros", [0, 1])
+@pytest.mark.parametrize("group", GROUPS)
+def test_scales_of_neighbouring_steps_in_large_launches(hiplib, shape, group, zeros, dtype):
+    """More tiles than the GPU holds CUs, thirteen steps of K, the last one a part of one: a group's scales (and those of 8-bit x)
+    are four or sixteen times those of its neighbours and of the groups two steps on, so that sums which met the scales of
+    another step show.  Whole numbers times powers of two below 2^24 units: every output is compared, bit by bit."""
+    B, nIn, nOut = 1100, 1552, 3750
+    g = U.rng(640 + group)
+    n = U.groups_of(nIn, group)
+    scales = 0.25 ** ((np.arange(n)[None, :] + np.arange(nOut)[:, None]) % 3)
+    z = g.integers(0, 16, (nOut, n)).astype(np.uint8) if zeros else None
+    layer = U.Layer(g.integers(0, 16, (nOut, nIn)).astype(np.uint8), scales, z, group, dtype).lay(hiplib)
+    w = layer.weights().astype(np.float32)
+    x = g.integers(-4, 5, (B, nIn)).astype(np.float32)
+    shape(5)
+    # units of 2^-4 (with scales of 8-bit x 2^-5): 1552 * 15 * 4 * 2^5 < 2^24, so that fp32 sums are exact in any order
+    assert np.array_equal(U.linear(hiplib, layer, x), U.rounded(x @ w.T, dtype))
+    for xgroup in (0, group) if group else (0,):
+        xs = (0.5 ** ((np.arange(U.groups_of(nIn, xgroup))[None, :] + np.arange(B)[:, None]) // 2 % 2)).astype(np.float32)
+        want = (x * U.spread_x(xs, nIn, group)) @ w.T
+        assert np.array_equal(U.linear(hiplib, layer, x.astype(np.int8), xs=xs, xgroup=xgroup), U.rounded(want, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("which", range(6))
 @pytest.mark.parametrize("B", [1, 130])
 def test_rows_that_end_with_their_allocation(hiplib, shape, which, B, dtype):

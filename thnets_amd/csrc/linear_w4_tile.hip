@@ -14,6 +14,8 @@
  * LDS rows are 128 k of a column; a 16-byte vector v of row r lies in slot v ^ r % 16 (8-bit x: v ^ r / 2 % 8),
  * which puts the 16 columns of an operand on different banks.  DMA: rows that memory holds in whole, aligned
  * 16-byte vectors are loaded straight into LDS; others go through registers.
+ * One barrier a step: what is read of a step's buffers (x, scales, zeros) is read before the barrier at its end, and written
+ * again for the step after next behind that barrier.
  * KS: where there are fewer tiles than CUs, eight wavefronts share a tile, four taking every other step of K.
  * Instructions of 32 x 32 outputs in place of 16 x 16 took as long (fp16 490 -> 504 us, 8-bit x 342 -> 384): what they
  * save in issue they need in registers, of which 8-bit x then has too few for a third workgroup.
@@ -227,23 +229,36 @@ __global__ __launch_bounds__(KS * TH) __attribute__((amdgpu_waves_per_eu(w4_tile
 	constexpr bool PIPE = DMA || (X == THHIP_F32 && TH == 256);
 	const int own = wrow * R * 16 + col;	/* the lane's row of the first row block */
 	A p[PIPE ? 2 : 1][R];
-	/* unit u's finished sums into the result (buf: where its step's scales are) */
-	auto flush_at = [&](int u, int buf) {
-		const int n = u / NG, g = u % NG;
-		floatx4 xs;
+	/* the scales that unit u's sums take, from where its step's are */
+	struct unit_scales {
+		float w[R];
+		floatx4 x;
+	};
+	auto scales_of = [&](int u, int buf) {
+		unit_scales s;
+#pragma unroll
+		for (int r = 0; r < R; r++)
+			s.w[r] = lscale[buf][u % NG][own + r * 16];
 		if constexpr (XG)
-			xs = *(const floatx4 *)&lxs[buf][g][c0 + n * 16 + 4 * quarter];
+			s.x = *(const floatx4 *)&lxs[buf][u % NG][c0 + u / NG * 16 + 4 * quarter];
+		return s;
+	};
+	/* unit u's finished sums into the result */
+	auto flush = [&](int u, const unit_scales &s) {
+		const int n = u / NG;
 #pragma unroll
 		for (int r = 0; r < R; r++) {
-			const float s = lscale[buf][g][own + r * 16];
 #pragma unroll
 			for (int i = 0; i < 4; i++)
-				acc[r][n][i] += (XG ? s * xs[i] : s) * (float)p[PIPE ? u & 1 : 0][r][i];
+				acc[r][n][i] += (XG ? s.w[r] * s.x[i] : s.w[r]) * (float)p[PIPE ? u & 1 : 0][r][i];
 			/* (here, not at the end of the step, where the compiler would gather all n's sums) */
 			asm("" : "+v"(acc[r][n]));
 		}
 	};
-	constexpr bool LATE = PIPE && KS == 1 && NG == 1 && PARTS == 1;	/* a step's last sums are added at the start of the next */
+	/* A step's last sums are added at the start of the next, with scales read before the barrier between the two: behind it
+	 * another wavefront may already have put the scales of the step after into that buffer. */
+	constexpr bool LATE = PIPE && KS == 1 && NG == 1 && PARTS == 1;
+	unit_scales late;
 	const int rounds = (a.steps + KS - 1) / KS;
 	for (int i = 0; i < rounds; i++) {
 		const int t = i * KS + part, buf = i & 1, t1 = t + KS < a.steps ? t + KS : a.steps - 1;
@@ -260,7 +275,6 @@ __global__ __launch_bounds__(KS * TH) __attribute__((amdgpu_waves_per_eu(w4_tile
 				for (int j = 0; j < NJ; j++)
 					x[n & 1][q][j] = M::read(base + q * PLANE + n * 16 * ROW, col, j, quarter);
 		};
-		auto flush = [&](int u) { flush_at(u, buf); };
 		__builtin_amdgcn_s_setprio(0);
 		x_issue(t1, buf ^ 1, 0);
 		x_read(0);
@@ -274,7 +288,7 @@ __global__ __launch_bounds__(KS * TH) __attribute__((amdgpu_waves_per_eu(w4_tile
 					w[r][g * GJ + j] = M::weights(codes[r], g * GJ + j, z);
 			}
 		if (LATE && i > 0)
-			flush_at(NU - 1, buf ^ 1);
+			flush(NU - 1, late);
 		codes_issue(t1);
 		g_issue(t1);
 		__builtin_amdgcn_s_setprio(1);
@@ -302,7 +316,7 @@ __global__ __launch_bounds__(KS * TH) __attribute__((amdgpu_waves_per_eu(w4_tile
 						p[PIPE ? u & 1 : 0][r] = M::mma(x[n & 1][q][j], w[r][j], p[PIPE ? u & 1 : 0][r]);
 			}
 			if (PIPE ? u > 0 : true)
-				flush(PIPE ? u - 1 : u);
+				flush(PIPE ? u - 1 : u, scales_of(PIPE ? u - 1 : u, buf));
 			if constexpr (PIPE && (X == THHIP_F16 || X == THHIP_BF16)) {
 			/* the order to issue them in: what comes from LDS, then a matrix instruction and the sums' work in turn */
 			__builtin_amdgcn_sched_group_barrier(0x100, PARTS * NJ + R, 0);
@@ -314,16 +328,16 @@ __global__ __launch_bounds__(KS * TH) __attribute__((amdgpu_waves_per_eu(w4_tile
 			}
 		}
 		if (PIPE && !LATE)
-			flush(NU - 1);
+			flush(NU - 1, scales_of(NU - 1, buf));
+		if (LATE)
+			late = scales_of(NU - 1, buf);
 		__builtin_amdgcn_sched_barrier(0);
 		x_land(t1, buf ^ 1, DMA ? 0 : 1);
 		g_land(buf ^ 1);
 		barrier();
 	}
-	if (LATE && part < a.steps) {
-		const int last = (a.steps - 1 - part) / KS;
-		flush_at(NU - 1, last & 1);
-	}
+	if (LATE)
+		flush(NU - 1, late);
 	if constexpr (KS > 1) {		/* the parts of K, added in their order */
 		floatx4 *sums = (floatx4 *)all_lds;
 		barrier();
