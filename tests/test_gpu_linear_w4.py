@@ -316,6 +316,26 @@ def test_more_rows_than_a_launch_takes(hiplib):
         U.check_linear(got, *U.linear64(layer, x[i:i + 3000]), layer)
 
 
+def test_the_largest_batch(hiplib, shape):
+    """2^31 - 5 rows in tiles: the first, those around 2^30 and the last ones; a launch's first row is counted past 32 bits."""
+    B, nIn, nOut = (1 << 31) - 5, 8, 1
+    g = U.rng(690)
+    layer = U.Layer.random(g, nOut, nIn, 0, F16, True).lay(hiplib)
+    dx, dy = api.DeviceArray(hiplib, nbytes=B * nIn * 2), api.DeviceArray(hiplib, nbytes=B * 2)
+    x = U.rounded(g.standard_normal((3000, nIn), dtype=np.float32), F16)
+    words = U.raw(x, F16)
+    some = (0, (1 << 30) - 1500, B - 3000)
+    for i in some:
+        hiplib.thhip_memcpy_h2d(dx.ptr + i * nIn * 2, words.ctypes.data, words.nbytes)
+    G.note("the largest batch")
+    shape(5)
+    assert hiplib.thhip_linear_w4(dx.ptr, nIn, layer.packed.ptr, None, dy.ptr, nOut, B, nIn, nOut, 0, 1, 0, 0.0, 0.0, F16) == 0
+    hiplib.thhip_sync()
+    want = U.linear64(layer, x)
+    for i in some:
+        U.check_linear(U.unraw(from_device(hiplib, dy, i * 2, (3000, nOut), np.uint16), F16), *want, layer)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B", [1, 18, 129])
 def test_threshold(hiplib, dtype, B):

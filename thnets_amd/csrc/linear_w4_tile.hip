@@ -389,8 +389,8 @@ static void w4_tile_launch(const w4_args &all)
 	constexpr size_t esx = sizeof(typename W4X<X>::E);
 	const size_t esy = thhip_esize(all.dtype);
 	constexpr int BN = W4X<X>::PARTS > 1 ? 64 : 128;
-	for (int b0 = 0; b0 < all.B; b0 += W4_TILE_ROWS) {
-		const w4_args a = w4_rows(all, b0, all.B - b0 < W4_TILE_ROWS ? all.B - b0 : W4_TILE_ROWS, esx, esy);
+	for (long b0 = 0; b0 < all.B; b0 += W4_TILE_ROWS) {	/* (a batch may have up to 2^31 - 1 rows) */
+		const w4_args a = w4_rows(all, (int)b0, (int)(all.B - b0 < W4_TILE_ROWS ? all.B - b0 : W4_TILE_ROWS), esx, esy);
 		const int ntiles = (a.B + BN - 1) / BN;
 		const bool few = (long)((a.blocks + 7) / 8) * ntiles <= 256;	/* tiles of 128 rows: at most one a CU */
 		/* rows in whole vectors, and a tile of them within the reach of a buffer descriptor */
