@@ -302,3 +302,37 @@ def test_a_block_of_a_network(hiplib, dtype, B):
     last = Call(hiplib, out, first.sum, w, dtype)
     h, y = norm64(out, first.sum, w)
     near(last.y, y, U.HALF_STEP[dtype] * (1 + 2.0 ** -8) + chain(D) + 8 * 2.0 ** -24 + 2.0 ** -22 * 8, dtype, "y")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cols", [5, 200, 3000, 9216, 70000])
+def test_codes_of_the_largest_values(hiplib, dtype, cols):
+    """Rows whose largest value is between 2^125 and the type's last number, or a mask of the type's lowest one beside ordinary
+    values: every code is the nearest to x / scale."""
+    g = U.rng(61)
+    top = np.finfo(np.float32).max if dtype == F32 else np.float32((2 - 2.0 ** -7) * 2.0 ** 127)
+    x = g.uniform(-1, 1, (6, cols)) * np.array([2.0 ** 125, 2.0 ** 126, 1.5 * 2.0 ** 126, 2.0 ** 127, float(top), 1])[:, None]
+    x[:5, 0] = [2.0 ** 125, 2.0 ** 126 * 1.25, 2.0 ** 126 * 1.75, 2.0 ** 127, top]
+    x[5, ::32] = -top
+    x = U.rounded(x, dtype)
+    for group in (0, 32, 256):
+        check_codes(Call(hiplib, x, None, None, dtype, group=group, norm=False), x.astype(np.float64), cols, group, 0.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cols", [5, 200, 3000, 9216, 70000])
+@pytest.mark.parametrize("e,eps,weight", [(-121, 1e-5, 0), (-121, 1e-5, 1), (-20, 1e-5, -101), (-130, 1e-12, 0), (-100, 1e-5, 0), (-101, 1e-8, 1)])
+def test_codes_of_norms_of_tiny_rows(hiplib, dtype, cols, e, eps, weight):
+    """Rows of values around 2^e, which eps makes larger: |y| is above 2^-116, where codes are promised, though 127 / max|h w| is
+    past fp32's largest number (or h itself is a denormal).  weight: none, about 1, or about 2^weight."""
+    g = U.rng(62)
+    x = U.rounded(g.uniform(-1, 1, (4, cols)) * 2.0 ** e, dtype)
+    x[:, 0] = 2.0 ** e
+    r = U.rounded(g.uniform(-0.25, 0.25, (4, cols)) * 2.0 ** e, dtype)
+    w = ((1 + 0.2 * g.uniform(-1, 1, cols)) * 2.0 ** (weight if weight < 0 else 0)).astype(np.float32) if weight else None
+    _, y = norm64(x, r, w, eps)
+    for group in (0, 32, 256):
+        step = group or cols
+        assert all(np.abs(y[:, i:i + step]).max(1).min() > 2.0 ** -116 for i in range(0, cols, step)) or cols % step
+        c = Call(hiplib, x, r, w, dtype, group=group, eps=eps)
+        check_codes(c, y, cols, group, chain(cols) + 8 * 2.0 ** -24)

@@ -101,16 +101,21 @@ template <int DT> struct RowVec {
 };
 
 /* What a row's or group's values become codes by.  top is the largest |h w|, top * rstd the largest |y|: below
- * 2^-116 (where an fp32 scale loses bits) it counts as nothing, reciprocal 0, codes 0. */
+ * 2^-116 (where an fp32 scale loses bits) it counts as nothing, codes 0.  Near either end of the range 127 / top passes
+ * fp32's largest number or 1 / top is a denormal, and products next to the lower end lose bits: there all codes are taken
+ * in 64 bits. */
 struct code_step {
-	float top, inv;		/* inv: 127 / top, off by at most 1.5 units */
+	float top, inv;		/* inv: 127 / top, off by at most 1.5 units, or 0 */
+	float sure;		/* a quotient this far from its code or further is taken again in 64 bits */
 };
 
 __device__ __forceinline__ struct code_step code_step_of(float top, float rstd)
 {
+	const bool none = top * rstd < 1.2e-35f, end = top < 0x1p-100f || (top > 0x1p125f && top < INFINITY);
 	struct code_step c;
 	c.top = top;
-	c.inv = top * rstd < 1.2e-35f ? 0.0f : 127.0f * __builtin_amdgcn_rcpf(top);	/* (a NaN stays one) */
+	c.inv = none || end ? 0.0f : 127.0f * __builtin_amdgcn_rcpf(top);	/* (a NaN stays one) */
+	c.sure = none ? 1.0f : end ? -1.0f : 0.5f - 0x1p-14f;
 	return c;
 }
 
@@ -131,7 +136,7 @@ __device__ __forceinline__ void store_codes(signed char *p, long base, int col, 
 		off = fmaxf(off, fabsf(fmaf(x, c.inv, whole - y)));
 		u[i] = __float_as_uint(y);
 	}
-	if (off > 0.5f - 0x1p-14f && c.inv > 0) {
+	if (off > c.sure) {
 		/* v * w / step in 64 bits, by the reciprocal and what the product says is left */
 		const double step = (double)c.top * (1.0 / 127.0);
 		double inv = __builtin_amdgcn_rcp(step);
@@ -330,7 +335,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const rows_args
 		}
 	}
 	float s = 0, rstd = 1;
-	struct code_step step = {0, 0};
+	struct code_step step = {0, 0, 1};
 	unsigned m = 0;
 #pragma unroll
 	for (int v = 0; v < V; v++) {
@@ -379,7 +384,7 @@ __global__ __launch_bounds__(1024) void rows_long_kernel(const rows_args a)
 	const int t = threadIdx.x;
 	const int steps = (a.cols - 1) / (T * N) + 1;
 	float h[N], w[N], r[N], s = 0, rstd = 1;
-	struct code_step step = {0, 0};
+	struct code_step step = {0, 0, 1};
 	unsigned m = 0;
 	for (int walk = 0; walk < 2; walk++) {
 		for (int v = 0; v < steps; v++) {
