@@ -336,3 +336,21 @@ def test_codes_of_norms_of_tiny_rows(hiplib, dtype, cols, e, eps, weight):
         assert all(np.abs(y[:, i:i + step]).max(1).min() > 2.0 ** -116 for i in range(0, cols, step)) or cols % step
         c = Call(hiplib, x, r, w, dtype, group=group, eps=eps)
         check_codes(c, y, cols, group, chain(cols) + 8 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("group", [0, 32])
+@pytest.mark.parametrize("cols", [5, 3000, 70000])
+def test_the_largest_number_comes_back_from_its_code(hiplib, cols, group):
+    """Codes of rows with masks of fp32's lowest or largest value, and back: finite, each value within half a step of its group
+    and what two roundings (the scale's, here up to a whole unit, and the product's) move 127 steps by."""
+    g = U.rng(63)
+    x = g.uniform(-1, 1, (3, cols)).astype(np.float32)
+    x[:, 1::64] = np.array([np.finfo(np.float32).max, np.finfo(np.float32).min, 1e38], np.float32)[:, None]
+    c = Call(hiplib, x, None, None, F32, group=group, norm=False)
+    dq, ds, dy = U.Rows(hiplib, c.q), api.DeviceArray(hiplib, c.scale), U.Rows(hiplib, None, None, 0, x.shape, np.uint32)
+    assert hiplib.thhip_dequantize_rows(dq.ptr, cols, ds.ptr, group, dy.ptr, cols, 3, cols, F32) == 0
+    hiplib.thhip_sync()
+    y = U.unraw(dy.get(), F32)
+    assert np.isfinite(y).all()
+    step = U.spread_x(c.scale.astype(np.float64), cols, group)
+    assert (np.abs(y - x.astype(np.float64)) <= step * (0.5 + 127 * 3 * 2.0 ** -23)).all()

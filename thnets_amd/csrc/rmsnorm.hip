@@ -175,10 +175,11 @@ __device__ __forceinline__ unsigned abs_bits(float v)
 	return __float_as_uint(v) & 0x7fffffffu;
 }
 
+/* (at most what 127 times of is a number: of FLT_MAX the nearest to top / 127 is not) */
 __device__ __forceinline__ float code_scale(float top)
 {
 	const float s = top * (1.0f / 127.0f);
-	return top < 1.2e-35f ? 0.0f : top < INFINITY ? fmaf(fmaf(-s, 127.0f, top), 1.0f / 127.0f, s) : s;
+	return top < 1.2e-35f ? 0.0f : top < INFINITY ? fminf(fmaf(fmaf(-s, 127.0f, top), 1.0f / 127.0f, s), 0x1.020406p+121f) : s;
 }
 
 /* v of the lane that differs in bits `by` of its number (by = 1, 2), that is mirrored in its half row of 8 lanes (4) or row
