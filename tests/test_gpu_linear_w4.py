@@ -362,6 +362,27 @@ def test_a_row_with_nan_stays_alone(hiplib, dtype, B):
     assert np.array_equal(got[rest], clean[rest]) and np.array_equal(got[0], clean[0])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("group,zeros", [(32, 1), (128, 0), (128, 1), (0, 1)])
+@pytest.mark.parametrize("B,which", [(1, -1), (5, -1), (16, -1), (40, 0), (40, 1), (40, 2), (40, 3), (40, 4), (40, 5), (200, 5)])
+def test_x_at_the_ends_of_the_range(hiplib, shape, B, which, group, zeros, dtype):
+    """Rows of the type's lowest and largest values, alone or as a few masks beside ordinary values, in a layer whose outputs are
+    numbers (1300 * 15 * 2^-16 of the largest one at most); and rows of values around 2^-100 and 2^-112."""
+    nIn, nOut = 1300, 50
+    g = U.rng(850)
+    top = np.finfo(np.float32).max if dtype == F32 else np.float32((2 - 2.0 ** -7) * 2.0 ** 127)
+    layer = U.Layer.random(g, nOut, nIn, group, dtype, zeros)
+    layer = U.Layer(layer.codes, 2.0 ** -17 * g.uniform(1, 2, layer.scales.shape), layer.zeros, group, dtype).lay(hiplib)
+    shape(which)
+    x = g.standard_normal((B, nIn), dtype=np.float32)
+    x[:, 3::97] = -top
+    for v in (x, np.full((B, nIn), top), g.choice([-top, top, top / 2], (B, nIn)), g.standard_normal((B, nIn)) * 2.0 ** -100,
+              g.standard_normal((B, nIn)) * 2.0 ** -112):
+        v = U.rounded(v, dtype)
+        want, mag = U.linear64(layer, v)
+        U.check_linear(U.linear(hiplib, layer, v), want, mag, layer)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B", [1, 40, 300])
 def test_twice_the_same_bits_and_nothing_allocated(hiplib, dtype, B):

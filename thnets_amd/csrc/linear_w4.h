@@ -32,8 +32,13 @@ struct w4_args {
 
 /* What differs with the kind of x: the matrix core's operand of eight k, its accumulator, and how a
  * word of eight codes and eight elements of x become operands.  PARTS: operands an x vector makes.  zero(z): a zero
- * point as weights() takes it; ZIN: weights() are n - z, else n. */
+ * point as weights() takes it; ZIN: weights() are n - z, else n.  UNIT: what a code of 1 is multiplied as.  Elements of bf16
+ * and fp32 x may be as large as the sums they go into: with 2^-11 the 128 products of a step, at most 15 x 2^-11 each, stay
+ * below fp32's largest number, as the result does that is kept in the same unit until it is written.  (What that costs at
+ * the other end, denormal sums of x below 2^-114, is under half a step of y while y is above 2^-114.) */
 template <int X> struct W4X;
+
+#define W4_UNIT 0x1p-11f	/* of bf16 operands */
 
 template <> struct W4X<THHIP_F16> {
 	typedef _Float16 E;
@@ -41,6 +46,7 @@ template <> struct W4X<THHIP_F16> {
 	typedef halfx8 V;
 	typedef floatx4 A;
 	static constexpr int PARTS = 1;
+	static constexpr float UNIT = 1.0f;
 	static constexpr bool ZIN = true;
 	static __device__ __forceinline__ unsigned zero(int z) { return __builtin_bit_cast(unsigned short, (_Float16)-z) * 0x10001u; }
 	static __device__ __forceinline__ V weights(unsigned w, unsigned z)
@@ -62,15 +68,16 @@ template <> struct W4X<THHIP_BF16> {
 	typedef bf16x8 V;
 	typedef floatx4 A;
 	static constexpr int PARTS = 1;
+	static constexpr float UNIT = W4_UNIT;
 	static constexpr bool ZIN = false;
 	static __device__ __forceinline__ unsigned zero(int z) { return __float_as_uint((float)-z); }
-	static __device__ __forceinline__ V ones() { return (V)(__bf16)1.0f; }
+	static __device__ __forceinline__ V ones() { return (V)(__bf16)W4_UNIT; }
 	static __device__ __forceinline__ V weights(unsigned w, unsigned)
 	{
 		typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 		const unsigned lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
-		const b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, true);
-		const b2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, true);
+		const b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f * W4_UNIT, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f * W4_UNIT, true);
+		const b2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f * W4_UNIT, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f * W4_UNIT, true);
 		return (V){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 	}
 	static __device__ __forceinline__ A mma(V a, V b, A c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -85,6 +92,7 @@ template <> struct W4X<THHIP_F32> {
 	typedef bf16x8 V;
 	typedef floatx4 A;
 	static constexpr int PARTS = 3;
+	static constexpr float UNIT = W4_UNIT;
 	static constexpr bool ZIN = false;
 	static __device__ __forceinline__ unsigned zero(int z) { return __float_as_uint((float)-z); }
 	static __device__ __forceinline__ V ones() { return W4X<THHIP_BF16>::ones(); }
@@ -117,6 +125,7 @@ template <> struct W4X<W4_X_I8> {
 	typedef long V;
 	typedef intx4 A;
 	static constexpr int PARTS = 1;
+	static constexpr float UNIT = 1.0f;
 	static constexpr bool ZIN = true;
 	static __device__ __forceinline__ unsigned zero(int z) { return __builtin_amdgcn_perm(z, z, 0); }
 	/* (128 + n - z in every byte, which none borrows from another, without the 128) */
@@ -145,8 +154,8 @@ struct W4Signed : W4X<THHIP_BF16> {
 	{
 		typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 		const unsigned lo = signed_bytes(w & 0x0f0f0f0fu, z), hi = signed_bytes(w >> 4 & 0x0f0f0f0fu, z);
-		const b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f, true);
-		const b2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f, true);
+		const b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f * W4_UNIT, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.0f * W4_UNIT, true);
+		const b2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f * W4_UNIT, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.0f * W4_UNIT, true);
 		return (V){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 	}
 };

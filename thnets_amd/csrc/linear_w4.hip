@@ -18,7 +18,8 @@
  *
  * A code becomes a half value without an integer conversion: the byte 0000nnnn read as an e4m3
  * number is n * 2^-9 for all sixteen codes (eight denormals, eight of the first binade), and
- * v_cvt_scalef32_pk_{f16,bf16}_fp8 widens two of them with a factor of 2^9.  For 8-bit x z is taken
+ * v_cvt_scalef32_pk_{f16,bf16}_fp8 widens two of them with a factor of 2^9 (bf16: of 2^-2, as its sums
+ * are kept in units of 2^-11; W4_UNIT).  For 8-bit x z is taken
  * from four bytes 128 + n in one subtraction, in which none borrows from another, and a flipped top bit takes the
  * 128 away.
  *
@@ -476,6 +477,7 @@ __global__ __launch_bounds__(W * 64) void w4_skinny_kernel(const w4_args all, in
 			}
 		if (X == W4_X_I8 && a.xgroups == 1)
 			y *= a.xscale[b];
+		y *= 1.0f / K::UNIT;
 		y += a.bias ? a.bias[o] : 0.0f;
 		if (a.act)
 			y = y > a.thr ? y : a.val;

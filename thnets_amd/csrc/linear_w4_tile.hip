@@ -371,7 +371,7 @@ __global__ __launch_bounds__(KS * TH) __attribute__((amdgpu_waves_per_eu(w4_tile
 			for (int i = 0; i < 4; i++) {
 				const int b = b0 + c0 + n * 16 + 4 * quarter + i;
 				if (b < a.B && o < a.nOut) {
-					float y = acc[r][n][i] * (X == W4_X_I8 && !XG ? a.xscale[b] : 1.0f) + bias;
+					float y = acc[r][n][i] * (X == W4_X_I8 && !XG ? a.xscale[b] : 1.0f / K::UNIT) + bias;
 					if (a.act)
 						y = y > a.thr ? y : a.val;
 					w4_put<X>(a.y, b * a.ldy + o, y, a.dtype);
