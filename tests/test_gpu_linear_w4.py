@@ -462,6 +462,32 @@ def test_quantize_at_the_ends_of_the_range(hiplib, dtype, zeros):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("zeros", [0, 1])
+def test_quantize_in_the_middle_between_codes(hiplib, dtype, zeros):
+    """Scales that are odd numbers, so that w / s is a whole number and a half without any rounding, and weights a unit of fp32
+    beside those: every code and zero point is rint(w / s) (the even one in the middle), as a quotient in 64 bits has it."""
+    s0 = np.arange(1, 256, 2)
+    nIn, nOut = 64, len(s0)
+    w = np.zeros((nOut, nIn), np.float32)
+    halves = np.arange(-7, 7) + 0.5
+    w[:, 1:15] = halves * s0[:, None]
+    w[:, 15:29], w[:, 29:43] = np.nextafter(w[:, 1:15], np.float32(99999)), np.nextafter(w[:, 1:15], np.float32(-99999))
+    w[:, 0] = (8 if zeros else 7) * s0
+    w[:, 43] = -7 * s0
+    dw, dc, ds, dz = (api.DeviceArray(hiplib, nbytes=n) for n in (w.nbytes, nOut * 32, nOut * 4, nOut))
+    hiplib.thhip_memcpy_h2d(dw.ptr, w.ctypes.data, w.nbytes)
+    assert hiplib.thhip_quantize_w4(dw.ptr, nIn, F32, dc.ptr, ds.ptr, dz.ptr if zeros else None, nOut, nIn, 64, dtype) == 0
+    hiplib.thhip_sync()
+    s = U.unraw(ds.get((nOut,), np.uint32 if dtype == F32 else np.uint16), dtype).astype(np.float64)[:, None]
+    assert (np.abs(s[:, 0] - s0) <= 2.0 ** -23 * s0).all() and (zeros or (s[:, 0] == s0).all())
+    z = dz.get((nOut,), np.uint8).astype(np.float64)[:, None] if zeros else 8
+    if zeros:
+        assert np.array_equal(z, np.rint(7 * s0[:, None] / s))
+    codes = U.unpack_codes(dc.get((nOut, 32), np.uint8), nIn)
+    assert np.array_equal(codes, np.clip(np.rint(w.astype(np.float64) / s) + z, 0, 15))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_from_weights_to_outputs(hiplib, dtype):
     """quantise, pack and multiply in one go, as a program does; the product is that of the weights the codes stand for."""
     g, x, b = data(1100, 9, 640, 72, dtype)

@@ -147,6 +147,14 @@ extern "C" int thhip_w4_pack(const unsigned char *codes, const void *scales, con
 	return 0;
 }
 
+/* rint(v / s).  v times the reciprocal of s is off by at most 2^-23 of it, 2^-19 for quotients up to 15 (larger ones are cut
+ * off): next to the middle between two whole numbers the quotient itself is taken, in 64 bits. */
+__device__ __forceinline__ float w4_nearest(float v, float s, float inv)
+{
+	const float q = v * inv, n = rintf(q);
+	return fabsf(q - n) > 0.5f - 0x1p-18f ? (float)rint((double)v / (double)s) : n;
+}
+
 /* One wavefront a (row, group): the group's extremes, its scale rounded to the type it is kept in,
  * and the codes nearest to w / scale (+ zero).  Two weights of a byte belong to one lane. */
 template <int WDT, int DT>
@@ -174,7 +182,7 @@ __global__ __launch_bounds__(256) void w4_quantize_kernel(const void *w, long ld
 		const float most = DT == THHIP_F16 ? 65504.0f : 3e38f;
 		typename ThhipElem<DT>::T sr = (typename ThhipElem<DT>::T)fminf(zeros ? hi / 15.0f - lo / 15.0f : fmaxf(hi, -lo) / 7.0f, most);
 		const float s = (float)sr, inv = s > 0 && 1.0f / s < INFINITY ? 1.0f / s : 0.0f;
-		const float z = zeros ? fminf(rintf(-lo * inv), 15.0f) : 8.0f;
+		const float z = zeros ? fminf(w4_nearest(-lo, s, inv), 15.0f) : 8.0f;
 		if (lane == 0) {
 			ThhipElem<DT>::st(scales, (long)i, s);
 			if (zeros)
@@ -184,7 +192,7 @@ __global__ __launch_bounds__(256) void w4_quantize_kernel(const void *w, long ld
 			unsigned b = 0;
 			for (int e = 0; e < 2 && k + e < k1; e++) {
 				const float v = ThhipElem<WDT>::ld(w, row * ldw + k + e);
-				b |= (unsigned)(int)fminf(fmaxf(rintf(v * inv) + z, 0.0f), 15.0f) << (4 * e);
+				b |= (unsigned)(int)fminf(fmaxf(w4_nearest(v, s, inv) + z, 0.0f), 15.0f) << (4 * e);
 			}
 			codes[row * (((long)nIn + 1) / 2) + k / 2] = (unsigned char)b;
 		}
