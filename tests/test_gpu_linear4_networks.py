@@ -117,3 +117,21 @@ def test_command_line_driver(hiplib, tmp_path):
     want = net.process_float(x)
     net.free()
     assert len(printed) == want.size and np.abs(np.array(printed) - want).max() <= 1e-6 + 1e-6 * np.abs(want).max()
+
+
+def test_the_setting_holds_for_networks_that_name_none(hiplib):
+    """A network made without linear4 has what THHipLinear4Bit says; one made with it has its own, and the setting stays."""
+    layers, x = network(U.rng(3400), 3)
+    nets = [api.HipNetwork(layers, linear4=0), api.HipNetwork(layers, linear4=64)]
+    assert hiplib.THHipLinear4Bit(64) == 0
+    try:
+        nets += [api.HipNetwork(layers), api.HipNetwork(layers, linear4=0)]
+        with pytest.raises(ValueError):
+            api.HipNetwork(layers, linear4=48)
+        assert hiplib.THHipLinear4Bit(-1) == 64
+    finally:
+        hiplib.THHipLinear4Bit(0)
+    plain, four, by_setting, named = (n.process_float(x) for n in nets)
+    assert not np.array_equal(plain, four) and np.array_equal(by_setting, four) and np.array_equal(named, plain)
+    for n in nets:
+        n.free()

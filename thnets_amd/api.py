@@ -271,10 +271,12 @@ def from_device_dtype(dev, shape, dtype):
 
 class HipNetwork:
     """A network on the engine, made from a layer list (see netbuild) or from a
-    Torch7 model directory (``model.net`` + ``stat.t7``, read by ``THLoadNetwork``)."""
+    Torch7 model directory (``model.net`` + ``stat.t7``, read by ``THLoadNetwork``).
+
+    ``linear4``: THHipLinear4Bit for this network (0, 32, 64, 128 or 256); None leaves the setting as it is."""
 
     def __init__(self, layers, mean=(0.0, 0.0, 0.0), std=(1.0, 1.0, 1.0), half=0, lowp_range=None,
-                 make_spatial=None, fold_bn=True, linear4=0):
+                 make_spatial=None, fold_bn=True, linear4=None):
         self.lib = lib = load_library()
         lib.THInit()
         loaded = None
@@ -295,9 +297,12 @@ class HipNetwork:
             self.handle = lib.THCreateHipLowpNetwork(source, C.c_float(lowp_range))
             self.dtype = abi.THHIP_U8
         else:
-            old_linear4 = lib.THHipLinear4Bit(linear4)
-            if lib.THHipLinear4Bit(linear4) != linear4:     # (what it does not know changes nothing)
-                raise ValueError("THHipLinear4Bit(%r) refused" % linear4)
+            old_linear4 = lib.THHipLinear4Bit(-1)       # (what it does not know changes nothing)
+            if linear4 is not None:
+                lib.THHipLinear4Bit(linear4)
+                if lib.THHipLinear4Bit(-1) != linear4:
+                    lib.THHipLinear4Bit(old_linear4)
+                    raise ValueError("THHipLinear4Bit(%r) refused" % linear4)
             if lib.THHipHalfFloat(half) != 0:
                 lib.THHipLinear4Bit(old_linear4)
                 raise ValueError("THHipHalfFloat(%r) refused" % half)
