@@ -119,3 +119,11 @@ def test_the_driver_refuses_other_groups():
     exe = os.path.join(os.path.dirname(api.LIB_PATH), "thnets-hip-test")
     out = subprocess.run([exe, "-m", "nowhere", "-i", "random", "-q", "48"], capture_output=True, text=True, timeout=60)
     assert out.returncode and out.stderr.startswith("Syntax")
+
+
+def test_the_uint8_engine_has_no_4_bit_weights():
+    exe = os.path.join(os.path.dirname(api.LIB_PATH), "thnets-hip-test")
+    out = subprocess.run([exe, "-m", "nowhere", "-i", "random", "-a", "11", "-q", "64"], capture_output=True, text=True, timeout=60)
+    assert out.returncode and out.stderr.startswith("Syntax")
+    with pytest.raises(ValueError, match="uint8"):
+        api.HipNetwork([], lowp_range=4.0, linear4=64)

@@ -277,6 +277,8 @@ class HipNetwork:
 
     def __init__(self, layers, mean=(0.0, 0.0, 0.0), std=(1.0, 1.0, 1.0), half=0, lowp_range=None,
                  make_spatial=None, fold_bn=True, linear4=None):
+        if linear4 and lowp_range is not None:
+            raise ValueError("linear4 is a setting of the float engines, not of the uint8 one (lowp_range)")
         self.lib = lib = load_library()
         lib.THInit()
         loaded = None

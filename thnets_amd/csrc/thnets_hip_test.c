@@ -116,7 +116,7 @@ int main(int argc, char **argv)
 		}
 	}
 	THHipLinear4Bit(group);		/* (a group that it does not know leaves it at 0) */
-	if (!modelsdir || !inputfile || alg < 8 || alg > 11 || runs < 1 || THHipLinear4Bit(group) != group) {
+	if (!modelsdir || !inputfile || alg < 8 || alg > 11 || runs < 1 || THHipLinear4Bit(group) != group || (group && alg == 11)) {
 		fprintf(stderr, "Syntax: thnets-hip-test -m <models directory> -i <input.t7 | image.ppm | random>\n");
 		fprintf(stderr, "             [-r <number of runs>] [-p(rint results)] [-P(rofile)] [-M(inmax of every layer)]\n");
 		fprintf(stderr, "             [-a <alg=8:HIP fp32 (default), 9:HIP fp16, 10:HIP bf16, 11:HIP 8bit>]\n");
