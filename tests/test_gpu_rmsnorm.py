@@ -354,3 +354,32 @@ def test_the_largest_number_comes_back_from_its_code(hiplib, cols, group):
     assert np.isfinite(y).all()
     step = U.spread_x(c.scale.astype(np.float64), cols, group)
     assert (np.abs(y - x.astype(np.float64)) <= step * (0.5 + 127 * 3 * 2.0 ** -23)).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cols", [5, 200, 3000, 9216, 16388, 70000])
+@pytest.mark.parametrize("kind,eps", [("masks", 1e-5), ("masks", 0.0), ("largest", 1e-5), (70, 1e-5), (-46, 0.0), (-60, 0.0), (-60, 2.0 ** -118),
+                                      (-105, 0.0), (-126, 0.0), (-126, 1e-38)])
+def test_norms_whose_squares_leave_fp32(hiplib, dtype, cols, kind, eps):
+    """Masks of the type's lowest value beside ordinary ones, rows of the largest values, and rows whose squares are past fp32's
+    smallest number with an eps that does not make up for them: sums, norms and codes are the formula's all the same."""
+    g = U.rng(64)
+    top = np.finfo(np.float32).max if dtype == F32 else np.float32((2 - 2.0 ** -7) * 2.0 ** 127)
+    x = g.uniform(1, 2, (5, cols)) * g.choice([-1, 1], (5, cols))
+    if kind == "masks":
+        x[:4] *= 1024
+        x[:4, 1::64] = -top         # (the last row has none)
+    elif kind == "largest":
+        x[:4] = top * np.sign(x[:4])
+    else:
+        x[:4] *= 2.0 ** kind
+    x = U.rounded(x, dtype)
+    w = (1 + 0.2 * g.uniform(-1, 1, cols)).astype(np.float32)
+    h, y = norm64(x, None, w, eps)
+    err = chain(cols) + 8 * 2.0 ** -24
+    c = Call(hiplib, x, None, w, dtype, eps=eps)
+    assert np.array_equal(c.sum, x)
+    near(c.y, y, U.HALF_STEP[dtype] * (1 + 2.0 ** -8) + err, dtype, "y")
+    c = Call(hiplib, x, None, w, dtype, group=0, eps=eps)
+    assert np.array_equal(c.sum, x)
+    check_codes(c, y, cols, 0, err)

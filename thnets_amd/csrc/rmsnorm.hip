@@ -250,6 +250,17 @@ __device__ __forceinline__ void row_reduce(float &s, unsigned &m)
 	}
 }
 
+/* The squares are fp32: where their mean (with eps) is past its largest number, as with a mask of the type's lowest value in the
+ * row, or so small that squares have lost bits, the row is taken again times a power of two, eps with it.  (fp16 values
+ * are never that large or small.) */
+#define NORM_FACTOR(DT, MODE) (DT != THHIP_F16 && MODE != ROWS_QUANT)
+
+__device__ __forceinline__ float norm_factor(float mean)
+{
+	const float f = mean < 0x1p-96f ? 0x1p96f : mean < INFINITY ? 1.0f : 0x1p-96f;
+	return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(f)));
+}
+
 /* One vector of a row on its way out: y, or codes and (by the group's first lane) its scale */
 template <int DT, int MODE>
 __device__ __forceinline__ void row_out(const rows_args &a, long row, int col, const float *h, const float *w, float rstd,
@@ -335,27 +346,53 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const rows_args
 				w[v][i] = 1.0f;
 		}
 	}
-	float s = 0, rstd = 1;
+	float s, rstd = 1, eps = a.eps;
 	struct code_step step = {0, 0, 1};
-	unsigned m = 0;
+	unsigned m;
+	bool summed = false;	/* a.sum is written */
+	auto sums = [&]() {
+		s = 0;
+		m = 0;
 #pragma unroll
-	for (int v = 0; v < V; v++) {
-		if (v && v * T * N >= a.cols)
-			break;
+		for (int v = 0; v < V; v++) {
+			if (v && v * T * N >= a.cols)
+				break;
 #pragma unroll
-		for (int i = 0; i < N; i++) {
-			if constexpr (MODE != ROWS_QUANT)
-				s += h[v][i] * h[v][i];
-			if constexpr (MODE != ROWS_NORM) {
-				const unsigned b = abs_bits(MODE == ROWS_QUANT ? h[v][i] : h[v][i] * w[v][i]);
-				m = b > m ? b : m;
+			for (int i = 0; i < N; i++) {
+				if constexpr (MODE != ROWS_QUANT)
+					s += h[v][i] * h[v][i];
+				if constexpr (MODE != ROWS_NORM) {
+					const unsigned b = abs_bits(MODE == ROWS_QUANT ? h[v][i] : h[v][i] * w[v][i]);
+					m = b > m ? b : m;
+				}
 			}
 		}
+		if (MODE != ROWS_QUANT || !a.group)
+			row_reduce<T>(s, m);
+	};
+	sums();
+	if constexpr (NORM_FACTOR(DT, MODE)) {
+		const float f = norm_factor(s / (float)a.cols + eps);
+		if (f != 1.0f) {	/* (the same for the whole row) */
+			summed = a.sum;
+#pragma unroll
+			for (int v = 0; v < V; v++) {
+				if (v && v * T * N >= a.cols)
+					break;
+				if (a.sum)
+					RowVec<DT>::store(a.sum, row * a.lds, (v * T + t) * N, a.cols, h[v]);
+#pragma unroll
+				for (int i = 0; i < N; i++)
+					h[v][i] *= f;
+			}
+			eps = eps * f * f;
+			if (T > 64)
+				__syncthreads();	/* row_reduce's LDS is used again */
+			sums();
+		}
 	}
-	if (MODE != ROWS_QUANT || !a.group)
-		row_reduce<T>(s, m);
 	if constexpr (MODE != ROWS_QUANT)
-		rstd = 1.0f / sqrtf(s / (float)a.cols + a.eps);
+		rstd = 1.0f / sqrtf(s / (float)a.cols + eps);
 	if constexpr (MODE != ROWS_NORM) {
 		if (!a.group) {
 			step = code_step_of(__uint_as_float(m), rstd);
@@ -368,7 +405,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const rows_args
 		if (v && v * T * N >= a.cols)
 			break;
 		const int col = (v * T + t) * N;
-		if (a.sum)
+		if (a.sum && !summed)
 			RowVec<DT>::store(a.sum, row * a.lds, col, a.cols, h[v]);
 		row_out<DT, MODE>(a, row, col, h[v], w[v], rstd, step);
 	}
@@ -384,7 +421,7 @@ __global__ __launch_bounds__(1024) void rows_long_kernel(const rows_args a)
 	const long row = blockIdx.x;
 	const int t = threadIdx.x;
 	const int steps = (a.cols - 1) / (T * N) + 1;
-	float h[N], w[N], r[N], s = 0, rstd = 1;
+	float h[N], w[N], r[N], s = 0, rstd = 1, f = 1, eps = a.eps;
 	struct code_step step = {0, 0, 1};
 	unsigned m = 0;
 	for (int walk = 0; walk < 2; walk++) {
@@ -400,6 +437,12 @@ __global__ __launch_bounds__(1024) void rows_long_kernel(const rows_args a)
 #pragma unroll
 			for (int i = 0; i < N; i++)
 				w[i] = MODE != ROWS_QUANT && a.w && col + i < a.cols ? a.w[col + i] : 1.0f;
+			if (walk == 1 && a.sum)
+				RowVec<DT>::store(a.sum, row * a.lds, col, a.cols, h);
+			if constexpr (NORM_FACTOR(DT, MODE))
+#pragma unroll
+				for (int i = 0; i < N; i++)
+					h[i] *= f;
 			if (walk == 0) {
 #pragma unroll
 				for (int i = 0; i < N; i++) {
@@ -407,16 +450,25 @@ __global__ __launch_bounds__(1024) void rows_long_kernel(const rows_args a)
 					const unsigned b = abs_bits(h[i] * w[i]);
 					m = b > m ? b : m;
 				}
-			} else {
-				if (a.sum)
-					RowVec<DT>::store(a.sum, row * a.lds, col, a.cols, h);
+			} else
 				row_out<DT, MODE>(a, row, col, h, w, rstd, step);
-			}
 		}
 		if (walk == 0) {
 			row_reduce<T>(s, m);
+			if constexpr (NORM_FACTOR(DT, MODE))
+				if (f == 1.0f) {
+					f = norm_factor(s / (float)a.cols + eps);
+					if (f != 1.0f) {	/* (the same for the whole row) */
+						eps = eps * f * f;
+						s = 0;
+						m = 0;
+						walk = -1;
+						__syncthreads();	/* row_reduce's LDS is used again */
+						continue;
+					}
+				}
 			if constexpr (MODE != ROWS_QUANT)
-				rstd = 1.0f / sqrtf(s / (float)a.cols + a.eps);
+				rstd = 1.0f / sqrtf(s / (float)a.cols + eps);
 			if constexpr (MODE != ROWS_NORM) {
 				if (!a.group) {
 					step = code_step_of(__uint_as_float(m), rstd);
