@@ -383,3 +383,18 @@ def test_norms_whose_squares_leave_fp32(hiplib, dtype, cols, kind, eps):
     c = Call(hiplib, x, None, w, dtype, group=0, eps=eps)
     assert np.array_equal(c.sum, x)
     check_codes(c, y, cols, 0, err)
+
+
+@pytest.mark.parametrize("cols", [200, 3000, 9216, 70000])
+@pytest.mark.parametrize("sum_to,y_to", [("r", "x"), ("x", "r")])
+def test_rows_with_masks_in_place(hiplib, cols, sum_to, y_to):
+    """Rows that are taken again times a power of two, into their own inputs: the bits of the call that writes elsewhere."""
+    x, r, w = inputs(65, 4, cols, F32, True, True)
+    x[1:3, 5::64] = np.finfo(np.float32).min
+    want = Call(hiplib, x, r, w, F32)
+    bufs = {"x": U.Rows(hiplib, U.raw(x, F32)), "r": U.Rows(hiplib, U.raw(r, F32))}
+    dw = api.DeviceArray(hiplib, w)
+    assert hiplib.thhip_rmsnorm(bufs["x"].ptr, cols, bufs["r"].ptr, cols, dw.ptr, EPS, bufs[sum_to].ptr, cols, bufs[y_to].ptr, cols,
+                                4, cols, F32) == 0
+    hiplib.thhip_sync()
+    assert np.array_equal(U.unraw(bufs[sum_to].get(), F32), want.sum) and np.array_equal(U.unraw(bufs[y_to].get(), F32), want.y)
