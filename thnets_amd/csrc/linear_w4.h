@@ -34,8 +34,8 @@ struct w4_args {
  * word of eight codes and eight elements of x become operands.  PARTS: operands an x vector makes.  zero(z): a zero
  * point as weights() takes it; ZIN: weights() are n - z, else n.  UNIT: what a code of 1 is multiplied as.  Elements of bf16
  * and fp32 x may be as large as the sums they go into: with 2^-11 the 128 products of a step, at most 15 x 2^-11 each, stay
- * below fp32's largest number, as the result does that is kept in the same unit until it is written.  (What that costs at
- * the other end, denormal sums of x below 2^-114, is under half a step of y while y is above 2^-114.) */
+ * below fp32's largest number, as the result does that is kept in the same unit until it is written.  (The price: bits of y are lost
+ * where it, or the sum of a group, is below 2^-115 instead of 2^-126.) */
 template <int X> struct W4X;
 
 #define W4_UNIT 0x1p-11f	/* of bf16 operands */

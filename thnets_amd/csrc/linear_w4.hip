@@ -251,10 +251,10 @@ extern "C" void thhip_w4_set_shape(int shape)
  * added through LDS, in their order, and an fp32 row's three columns with them.
  * GM: matrix instructions a group spans within a step (1: groups of 32 or 64, 4: larger).
  *
- * Bound by memory where the layer is large: 1 x 8192 -> 32768 bf16 25.4 us (138 MB, 5.4 TB/s; a large copy moves 5.1),
- * 1 x 25088 -> 4096 fp32 14.1 us (53 MB, 3.8 TB/s: 256 workgroups, one a CU, whose start and end do not overlap), 1 x
- * 4096 -> 16384 with 8-bit x 9.3 us (35 MB, 3.7 TB/s).  By the vector unit (codes to operands) and the L2's x from about
- * 32 columns on: 128 x 4096 -> 4096 fp16 12.8 us (338 TFLOP/s). */
+ * Bound by memory where the layer is large: 1 x 8192 -> 32768 bf16 23.7 us (138 MB, 5.8 TB/s, some of it from the last-level cache; a large copy moves 5.1),
+ * 1 x 25088 -> 4096 fp32 13.0 us (53 MB, 4.1 TB/s: 256 workgroups, one a CU, whose start and end do not overlap), 1 x
+ * 4096 -> 16384 with 8-bit x 9.0 us (35 MB, 3.9 TB/s).  By the vector unit (codes to operands) and the L2's x from about
+ * 32 columns on: 128 x 4096 -> 4096 fp16 11.9 us (360 TFLOP/s). */
 
 /* The workgroup's LDS traffic so far is done, for everybody (loads from memory may still be on their way) */
 __device__ __forceinline__ void w4_lds_barrier(void)
@@ -522,8 +522,9 @@ static void w4_skinny_launch(const w4_args &all)
 
 /* ---- which kernel and shape ----
  *
- * Up to 16 columns: 16 rows a workgroup and 16 wavefronts, one workgroup a CU; from 1024 row blocks on 32 rows and
- * eight wavefronts, two workgroups a CU (1 x 8192 -> 16384 bf16: 13.2 us; the other 19 us).
+ * Up to 16 columns: 16 rows a workgroup and 16 wavefronts, of which a CU holds one (two of the forms that need no more than
+ * 64 registers: up to four rows of half types and 8-bit x); from 1024 row blocks on 32 rows and eight wavefronts, two
+ * workgroups a CU (1 x 8192 -> 16384 bf16: 13.0 us; the other 19 us.  12288 outputs, by the first form: 12.0).
  * More columns: the shape that takes the least time by the estimate below.  A launch runs in rounds of as many
  * workgroups as the GPU holds; the time of a round was measured at K = 512, 2048 and 8192 and is a start and a
  * slope.  Few rows at a time win in small layers and short K, 64 rows in larger ones (4096 -> 4096 fp16, us, in the

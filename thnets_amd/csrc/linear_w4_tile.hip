@@ -1,8 +1,9 @@
 /*
  * 4-bit Linear layers (linear_w4.hip) for larger batches: bound by the matrix cores and by the instructions between
  * theirs, of which a wavefront issues one where it could issue a matrix instruction (codes to operands, a group's sums to
- * the result).  4096 x 8192 -> 8192, us and 10^12 a second: fp16 490 to 505 and 1100, bf16 517 to 530 and 1050 (a library's
- * product of 8192^3: 1150 and 1201), 8-bit x 344 to 350 and 1590 (1779); 2048 rows of fp32 x 696 to 733 and 390 (149).
+ * the result).  4096 x 8192 -> 8192, us and 10^12 a second: fp16 485 to 505 and 1110, bf16 488 to 518 and 1090 (a library's
+ * product of 8192^3: 1150 and 1201), 8-bit x 342 to 350 and 1590 (1779); 2048 rows of fp32 x 696 to 733 and 390 (149).
+ * Groups of 64 and 32 take 560 and 680 (bf16), rows that are not whole vectors (4096 x 8190) 578 (fp16).
  *
  * A workgroup of four wavefronts computes 128 rows for BN columns (eight 256 rows: fp32 x), a wavefront 32 rows: each code
  * becomes an operand once (with 64 rows x BN / 2 a wavefront, twice: fp16 550 us).  All operands are n - z, so that no sum

@@ -19,9 +19,9 @@
  * codes it is taken again in 64 bits, so that the value goes to the nearer one: without
  * that one value in 30000 of fp16 rows did not.
  *
- * Time alone on the GPU, us (a large copy moves 5.1 TB/s): norm of 16384 rows of 8192 bf16 with a residual 182 (1074 MB,
- * 5.9 TB/s), of 333 rows of 5003 fp32 5.7 (13 MB, 2.3 TB/s: half of it is the way of one row through the GPU, 2.4 us);
- * with codes 8192 rows of 4096 bf16 47 (235 MB, 5.0 TB/s); codes alone 700 rows of 9216 fp16 7.7 (19 MB, 2.5 TB/s).
+ * Time alone on the GPU, us (a large copy moves 5.1 TB/s): norm of 16384 rows of 8192 bf16 with a residual 181 (1074 MB,
+ * 5.9 TB/s), of 333 rows of 5003 fp32 5.4 (13 MB, 2.5 TB/s: half of it is the way of one row through the GPU, 2.4 us);
+ * with codes 8192 rows of 4096 bf16 47 (235 MB, 5.0 TB/s); codes alone 700 rows of 9216 fp16 7.5 (19 MB, 2.6 TB/s).
  */
 #include <stdint.h>
 #include <stdio.h>
